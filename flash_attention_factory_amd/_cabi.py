@@ -1,5 +1,5 @@
 """ctypes binding of libfa_paged_attention.so (declarations: include/fa_paged_attention.h,
-include/fa_kv_cache.h).
+include/fa_kv_cache.h, include/fa_ragged.h).
 
 There is no fallback: if the HIP library is missing or a call fails, this raises.
 """
@@ -44,11 +44,20 @@ EXPORTS = (
     "fa_paged_attention_loop_workspace_bytes",
 )
 
+# of include/fa_ragged.h
+RAGGED_EXPORTS = (
+    "fa_kv_cache_append",
+    "fa_paged_attention_ragged",
+    "fa_paged_attention_ragged_workspace_bytes",
+    "fa_paged_attention_differential",
+)
+
 ABI_REVISION = 8
 
 FA_KV_CACHE_16BIT = 0
 FA_KV_CACHE_E5M2 = 1
 FA_KV_CACHE_E4M3 = 2
+FA_KV_CACHE_I8 = 3
 
 FA_FP8_E5M2 = 0
 FA_FP8_E4M3 = 1
@@ -151,6 +160,31 @@ class KvWriteShape(_Versioned):
     ]
 
 
+class KvAppendShape(_Versioned):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        *((name, ctypes.c_int32) for name in ("num_seqs", "num_tokens", "num_heads", "num_kv_heads", "head_size", "block_size",
+                                              "max_blocks_per_seq")),
+        *((name, ctypes.c_int64) for name in ("kv_block_stride", "kv_token_stride", "kv_head_stride", "query_token_stride",
+                                              "query_head_stride", "query_out_token_stride", "query_out_head_stride",
+                                              "key_token_stride", "key_head_stride", "value_token_stride", "value_head_stride")),
+        *((name, ctypes.c_int32) for name in ("src_dtype", "cache_dtype", "kv_scale_mode", "num_pool_blocks", "max_positions",
+                                              "rotary_dim", "interleaved")),
+        ("fp8_scale", ctypes.c_float),
+    ]
+
+
+class RaggedShape(_Versioned):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        *((name, ctypes.c_int32) for name in ("num_seqs", "num_tokens", "num_heads", "num_kv_heads", "head_size", "block_size",
+                                              "max_blocks_per_seq")),
+        *((name, ctypes.c_int64) for name in ("kv_block_stride", "kv_token_stride", "kv_head_stride", "query_token_stride",
+                                              "query_head_stride")),
+        *((name, ctypes.c_int32) for name in ("q_dtype", "cache_dtype", "num_pool_blocks", "max_query_len", "max_context_len")),
+    ]
+
+
 class SplitPlan(_Versioned):
     _fields_ = [
         ("struct_size", ctypes.c_uint32),
@@ -243,7 +277,7 @@ def load() -> ctypes.CDLL:
             f"{LIBRARY} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
             "(there is no CPU or PyTorch fallback for the paged-attention kernels)")
     L = ctypes.CDLL(LIBRARY)
-    missing = [name for name in EXPORTS if not hasattr(L, name)]
+    missing = [name for name in EXPORTS + RAGGED_EXPORTS if not hasattr(L, name)]
     if missing:
         raise RuntimeError(f"{LIBRARY} lacks {', '.join(missing)}: it was built from older sources, rebuild the library")
     P = ctypes.c_void_p
@@ -261,6 +295,16 @@ def load() -> ctypes.CDLL:
     L.fa_paged_attention_loop_workspace_bytes.restype = ctypes.c_int64
     L.fa_kv_cache_write.argtypes = [P, P, P, P, P, ctypes.POINTER(KvWriteShape), ctypes.POINTER(Options)]
     L.fa_kv_cache_write.restype = ctypes.c_int32
+    A, R, O = ctypes.POINTER(KvAppendShape), ctypes.POINTER(RaggedShape), ctypes.POINTER(Options)
+    L.fa_kv_cache_append.argtypes = [P] * 12 + [A, O]
+    L.fa_kv_cache_append.restype = ctypes.c_int32
+    L.fa_paged_attention_ragged.argtypes = [P] * 7 + [ctypes.c_float, P, ctypes.c_int64, R, O]
+    L.fa_paged_attention_ragged.restype = ctypes.c_int32
+    L.fa_paged_attention_ragged_workspace_bytes.argtypes = [R, ctypes.c_int32]
+    L.fa_paged_attention_ragged_workspace_bytes.restype = ctypes.c_int64
+    L.fa_paged_attention_differential.argtypes = [P] * 7 + [ctypes.c_float, P, P, ctypes.c_float, ctypes.c_float, P,
+                                                           ctypes.c_int64, R, O]
+    L.fa_paged_attention_differential.restype = ctypes.c_int32
     L.fa_last_error.restype = ctypes.c_char_p
     L.fa_paged_attention_abi_version.restype = ctypes.c_int32
     L.fa_paged_attention_reduce_plan.argtypes = [ctypes.POINTER(Shape), ctypes.POINTER(Options), ctypes.c_int32,

@@ -1,0 +1,261 @@
+// Host launcher of ragged paged attention and differential attention (declared in include/fa_ragged.h): argument checks, which
+// forms a call needs, work-group counts, workspace.
+#pragma once
+
+#include <algorithm>
+
+#include "../../include/fa_ragged.h"
+#include "launch_common.h"
+#include "ragged_rows_kernel.h"
+#include "ragged_tile_kernel.h"
+
+namespace fa {
+
+struct RaggedPlan {
+  bool rows, tiles;       // which forms run
+  int wavefronts;         // of a work-group of the tile form
+  int tile_rows;          // rows of its tiles
+  int64_t tile_bound;     // tiles per kv head, at most
+  int splits;
+  int row_groups;
+  int64_t row_o, row_ml, row_items, tile_o, tile_ml, bytes;  // offsets into the workspace, and its size
+};
+
+inline fa_status check_ragged_shape(const fa_ragged_shape *s, int maps) {
+  if (s->num_seqs < 0 || s->num_tokens < 0 || s->num_heads <= 0 || s->num_kv_heads <= 0 || s->max_blocks_per_seq <= 0 ||
+      s->num_pool_blocks <= 0 || s->max_query_len <= 0 || s->max_context_len < 0)
+    return fail(FA_ERR_BAD_SHAPE, "num_seqs, num_tokens and max_context_len must be >= 0; num_heads, num_kv_heads, max_blocks_per_seq, "
+                                  "num_pool_blocks and max_query_len positive");
+  if (s->q_dtype != FA_DTYPE_F16 && s->q_dtype != FA_DTYPE_BF16)
+    return fail(FA_ERR_UNSUPPORTED_DTYPE, "q_dtype %d is neither fp16 (0) nor bf16 (1)", s->q_dtype);
+  const int c = s->cache_dtype;
+  if (c != FA_KV_CACHE_16BIT && c != FA_KV_CACHE_I8 && (maps == 2 || (c != FA_KV_CACHE_E5M2 && c != FA_KV_CACHE_E4M3)))
+    return fail(FA_ERR_UNSUPPORTED_DTYPE, maps == 2 ? "cache_dtype %d is neither 16-bit (0) nor integers (3)"
+                                                    : "cache_dtype %d is none of 16-bit (0), E5M2 (1), E4M3 (2), integers (3)", c);
+  if ((s->head_size != 64 && s->head_size != 128) || s->block_size < 16 || !is_pow2(s->block_size))
+    return fail(FA_ERR_UNSUPPORTED_HEAD_OR_BLOCK_SIZE,
+                "Unsupported head size or block size (head_size %d must be 64 or 128, block_size %d a power of two >= 16)",
+                s->head_size, s->block_size);
+  if (s->num_heads % s->num_kv_heads != 0 || s->num_heads / s->num_kv_heads > kMaxGroup)
+    return fail(FA_ERR_UNSUPPORTED_GROUP, "Unsupported number of queries per token: %d heads over %d kv heads (a multiple, at most %d per kv head)",
+                s->num_heads, s->num_kv_heads, kMaxGroup);
+  if ((int64_t)s->max_blocks_per_seq * s->block_size > 0x3fffffffLL)
+    return fail(FA_ERR_BAD_SHAPE, "a block table of 2^30 tokens or more is not supported");
+  // the rows form numbers 128-key units of the whole batch, the tile form 16-row pieces of its grid
+  const int64_t keys = (int64_t)s->max_blocks_per_seq * s->block_size;
+  if ((int64_t)s->num_seqs * s->num_kv_heads * (keys / kRowUnit + 2) > 0x7fffffffLL ||
+      ((int64_t)s->num_tokens + s->num_seqs) * s->num_heads > 0x7fffffffLL)
+    return fail(FA_ERR_BAD_SHAPE, "num_seqs x num_kv_heads x keys or num_tokens x num_heads is too large");
+  return FA_OK;
+}
+
+// Which forms run, and how the work is cut; `cus`: compute units.
+inline RaggedPlan ragged_plan(const fa_ragged_shape &s, int maps, int cus) {
+  RaggedPlan r = {};
+  const int64_t T = s.num_tokens, S = s.num_seqs, Hk = s.num_kv_heads, G = s.num_heads / s.num_kv_heads, D = s.head_size;
+  if (T == 0 || S == 0) return r;
+  const int64_t most = std::min<int64_t>(s.max_query_len, T);
+  const int64_t table = (int64_t)s.max_blocks_per_seq * s.block_size;
+  const int64_t keys = s.max_context_len > 0 ? std::min<int64_t>(s.max_context_len, table) : table;
+  const bool equal = S == 1 || T == S * most;  // every sequence brings `most` tokens
+  r.tiles = most * G * maps > kRowColumns;
+  r.rows = G * maps <= kRowColumns && !(equal && r.tiles);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  if (r.rows) {
+    r.row_groups = (int)std::min<int64_t>(2 * (int64_t)cus, S * Hk * (keys / kRowUnit + 2));
+    const int64_t slots = S * Hk + r.row_groups;
+    r.row_o = take(slots * kRowColumns * D * 4);
+    r.row_ml = take(slots * 2 * kRowColumns * 4);
+    r.row_items = take(S * Hk * 8);
+  }
+  if (r.tiles) {
+    // 8 wavefronts halve what K and V cost per row; sequences that cannot fill them take 4
+    r.wavefronts = most * G * maps <= 128 ? 4 : 8;
+    r.tile_rows = r.wavefronts * 32 / maps;
+    const int64_t each = (most * G + r.tile_rows - 1) / r.tile_rows;
+    r.tile_bound = equal ? S * each : std::min(S * each, T * G / r.tile_rows + S);
+    const int64_t resident = (int64_t)cus * (r.wavefronts == 4 ? 2 : 1);
+    const int64_t steps = (keys + kTileKeys - 1) / kTileKeys;
+    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / std::max<int64_t>(1, r.tile_bound * Hk), steps / 8, 64}));
+    if (r.splits > 1) {
+      const int64_t slots = r.tile_bound * Hk * r.splits, rows = r.tile_rows * maps;
+      r.tile_o = take(slots * rows * D * 4);
+      r.tile_ml = take(slots * rows * 2 * 4);
+    }
+  }
+  r.bytes = at;
+  return r;
+}
+
+template <int D, typename OT, int KVF, int MAPS>
+inline fa_status launch_ragged_kernels(const RaggedParams &p, const RaggedPlan &plan, KernelTimer &timer, float *us) {
+  const int Hk = p.num_kv_heads;
+  auto timed = [&]() -> fa_status {
+    if (us) FA_HIP_CHECK(timer.accumulate(0, us));
+    return FA_OK;
+  };
+  fa_status st = FA_OK;
+  if (plan.tiles) {
+    const dim3 grid((unsigned)(plan.tile_bound * Hk), (unsigned)plan.splits);
+    if (plan.wavefronts == 8)
+      FA_HIP_CHECK(timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 8>, grid, dim3(512), 0, p));
+    else
+      FA_HIP_CHECK(timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 4>, grid, dim3(256), 0, p));
+    if ((st = timed()) != FA_OK) return st;
+    if (plan.splits > 1) {
+      const dim3 merge((unsigned)(plan.tile_bound * Hk), (unsigned)(plan.tile_rows / 16));
+      if (plan.wavefronts == 8)
+        FA_HIP_CHECK(timer.launch(ragged_tile_merge_kernel<D, MAPS, 256 / MAPS>, merge, dim3(256), 0, p));
+      else
+        FA_HIP_CHECK(timer.launch(ragged_tile_merge_kernel<D, MAPS, 128 / MAPS>, merge, dim3(256), 0, p));
+      if ((st = timed()) != FA_OK) return st;
+    }
+  }
+  if (plan.rows) {
+    FA_HIP_CHECK(timer.launch(ragged_rows_kernel<D, OT, KVF, MAPS>, dim3((unsigned)plan.row_groups), dim3(256), 0, p));
+    if ((st = timed()) != FA_OK) return st;
+    const int rows = std::min<int64_t>(kRowColumns / MAPS, (int64_t)p.max_query_len * p.group);
+    FA_HIP_CHECK(timer.launch(ragged_rows_merge_kernel<D, MAPS>, dim3((unsigned)(p.b.num_seqs * Hk), (unsigned)rows), dim3(256), 0, p));
+    if ((st = timed()) != FA_OK) return st;
+  }
+  return FA_OK;
+}
+
+struct DifferentialArgs {
+  const float *lambdas, *norm_weight;
+  float norm_eps, out_scale;
+};
+
+inline fa_status launch_ragged_attention(void *out, const void *query, const void *key_cache, const void *value_cache,
+                                         const int32_t *block_tables, const int32_t *query_start, const int32_t *context_lens,
+                                         float scale, void *workspace, int64_t workspace_bytes, const fa_ragged_shape *s,
+                                         const fa_paged_attention_options *o, const DifferentialArgs *diff) {
+  const int maps = diff ? 2 : 1;
+  fa_status st = check_ragged_shape(s, maps);
+  if (st != FA_OK) return st;
+  const bool nothing = s->num_tokens == 0 || s->num_seqs == 0;
+  if (!nothing && (!out || !query || !key_cache || !value_cache || !block_tables || !query_start || !context_lens))
+    return fail(FA_ERR_NULL_POINTER, "out, query, key_cache, value_cache, block_tables, query_start and context_lens must all be non-NULL");
+  const bool kv8 = s->cache_dtype != FA_KV_CACHE_16BIT;
+  const int64_t eb = kv8 ? 1 : 2;
+  if (s->kv_block_stride <= 0 || s->kv_token_stride < s->head_size || s->kv_head_stride < s->head_size)
+    return fail(FA_ERR_BAD_SHAPE, "kv strides must be positive and cover one head_size row");
+  if ((s->kv_block_stride * eb) % 16 || (s->kv_token_stride * eb) % 16 || (s->kv_head_stride * eb) % 16)
+    return fail(FA_ERR_BAD_SHAPE, "kv strides must be multiples of 16 bytes");
+  if (s->query_token_stride < s->head_size || s->query_head_stride < s->head_size || s->query_token_stride % 8 || s->query_head_stride % 8)
+    return fail(FA_ERR_BAD_SHAPE, "query strides must cover one head_size row and be multiples of 16 bytes");
+  if (((uintptr_t)out | (uintptr_t)query | (uintptr_t)key_cache | (uintptr_t)value_cache | (uintptr_t)workspace) % 16)
+    return fail(FA_ERR_BAD_SHAPE, "out, query, key_cache, value_cache and workspace must be 16-byte aligned");
+  if (((uintptr_t)block_tables | (uintptr_t)query_start | (uintptr_t)context_lens) % 4)
+    return fail(FA_ERR_BAD_SHAPE, "block_tables, query_start and context_lens must be 4-byte aligned");
+  const int flags = o ? o->mask_flags : 0;
+  if (flags & ~(FA_MASK_ALIBI | FA_MASK_SOFTCAP | FA_MASK_WINDOW))
+    return fail(FA_ERR_BAD_SHAPE, "mask_flags 0x%x has bits that mean nothing", flags);
+  if ((flags & FA_MASK_ALIBI) && !o->alibi_slopes) return fail(FA_ERR_NULL_POINTER, "FA_MASK_ALIBI needs alibi_slopes");
+  if ((flags & FA_MASK_SOFTCAP) && !(o->softcap > 0.f)) return fail(FA_ERR_BAD_SHAPE, "FA_MASK_SOFTCAP needs softcap > 0");
+  if ((flags & FA_MASK_WINDOW) && o->window_left < 0) return fail(FA_ERR_BAD_SHAPE, "FA_MASK_WINDOW needs window_left >= 0");
+  if (o && o->query_len > 1) return fail(FA_ERR_BAD_SHAPE, "query_len is not for ragged batches: query_start says which tokens are whose");
+  if (!(scale == scale) || scale - scale != 0.f) return fail(FA_ERR_BAD_SHAPE, "scale must be finite");
+  const int mode = kv8 && o ? o->kv_scale_mode : FA_KV_SCALE_TENSOR;
+  if (mode != FA_KV_SCALE_TENSOR && mode != FA_KV_SCALE_HEAD && mode != FA_KV_SCALE_BLOCK)
+    return fail(FA_ERR_BAD_SHAPE, "kv_scale_mode %d is none of tensor (0), head (1), block (2)", mode);
+  if (mode != FA_KV_SCALE_TENSOR && (!o->k_scales || !o->v_scales))
+    return fail(FA_ERR_NULL_POINTER, "kv_scale_mode %d needs k_scales and v_scales", mode);
+  if (mode != FA_KV_SCALE_TENSOR && ((uintptr_t)o->k_scales | (uintptr_t)o->v_scales) % 4)
+    return fail(FA_ERR_BAD_SHAPE, "k_scales and v_scales must be 4-byte aligned");
+  if (s->cache_dtype == FA_KV_CACHE_I8 && mode == FA_KV_SCALE_TENSOR)
+    return fail(FA_ERR_BAD_SHAPE, "pools of integers need k_scales and v_scales (kv_scale_mode head or block)");
+  if (diff) {
+    if (!nothing && !diff->lambdas) return fail(FA_ERR_NULL_POINTER, "lambdas must be non-NULL");
+    if ((uintptr_t)diff->lambdas % 4 || (uintptr_t)diff->norm_weight % 16)
+      return fail(FA_ERR_BAD_SHAPE, "lambdas must be 4-byte, norm_weight 16-byte aligned");
+    if (!(diff->norm_eps >= 0.f)) return fail(FA_ERR_BAD_SHAPE, "norm_eps must be >= 0");
+    if ((flags & (FA_MASK_ALIBI | FA_MASK_SOFTCAP)) || (o && o->sinks))
+      return fail(FA_ERR_BAD_SHAPE, "differential attention takes a window, and neither alibi_slopes, softcap nor sinks");
+  }
+  if (o && o->validate_only) return FA_OK;
+  if (o && o->elapsed_us) o->elapsed_us[0] = 0.f;
+  if (nothing) return FA_OK;
+  int cus = 0;
+  FA_HIP_CHECK(compute_units_of_current_device(&cus));
+  const RaggedPlan plan = ragged_plan(*s, maps, cus);
+  if (workspace_bytes < plan.bytes || (plan.bytes > 0 && !workspace))
+    return fail(FA_ERR_SCRATCH_TOO_SMALL, "the call works in %lld bytes of workspace, %lld were given", (long long)plan.bytes,
+                (long long)(workspace ? workspace_bytes : 0));
+
+  RaggedParams p = {};
+  p.a.key_cache = reinterpret_cast<const char *>(key_cache);
+  p.a.value_cache = reinterpret_cast<const char *>(value_cache);
+  p.a.group = kRowColumns;
+  p.a.block_shift = p.b.block_shift = ilog2(s->block_size);
+  p.a.max_block_id = p.b.max_block_id = s->num_pool_blocks - 1;
+  p.a.kv_block_bytes = s->kv_block_stride * eb;
+  p.a.kv_token_bytes = s->kv_token_stride * eb;
+  p.a.kv_head_bytes = s->kv_head_stride * eb;
+  p.b.query_start = query_start;
+  p.b.context_lens = context_lens;
+  p.b.block_tables = block_tables;
+  p.b.num_seqs = s->num_seqs;
+  p.b.num_tokens = s->num_tokens;
+  p.b.max_blocks_per_seq = s->max_blocks_per_seq;
+  p.query = reinterpret_cast<const char *>(query);
+  p.out = reinterpret_cast<char *>(out);
+  p.q_token_bytes = s->query_token_stride * 2;
+  p.q_head_bytes = s->query_head_stride * 2;
+  p.k_scales = mode != FA_KV_SCALE_TENSOR ? o->k_scales : nullptr;
+  p.v_scales = mode != FA_KV_SCALE_TENSOR ? o->v_scales : nullptr;
+  p.scale_pitch = mode == FA_KV_SCALE_BLOCK ? s->num_kv_heads : 0;
+  p.block_scales = mode == FA_KV_SCALE_BLOCK;
+  p.tensor_scale = kv8 && o && o->fp8_scale != 0.f ? o->fp8_scale : 1.0f;
+  p.sinks = o ? o->sinks : nullptr;
+  p.alibi_slopes = o ? o->alibi_slopes : nullptr;
+  p.softcap = o ? o->softcap : 0.f;
+  p.window = (flags & FA_MASK_WINDOW) ? std::min<int32_t>(o->window_left, kNoWindow) : kNoWindow;
+  p.mask_flags = flags & (FA_MASK_ALIBI | FA_MASK_SOFTCAP);
+  p.score_scale_log2 = std::max(std::abs(scale) * kLog2e, 1e-30f);  // (0 would turn masked scores into NaN)
+  p.query_flip = scale < 0.f ? 0x80008000u : 0u;
+  p.q_bf16 = s->q_dtype == FA_DTYPE_BF16;
+  p.num_heads = s->num_heads;
+  p.num_kv_heads = s->num_kv_heads;
+  p.group = s->num_heads / s->num_kv_heads;
+  p.max_query_len = s->max_query_len;
+  p.row_limit = plan.rows ? kRowColumns : 0;
+  if (diff) {
+    p.lambdas = diff->lambdas;
+    p.norm_weight = diff->norm_weight;
+    p.norm_eps = diff->norm_eps;
+    p.out_scale = diff->out_scale;
+  }
+  char *space = reinterpret_cast<char *>(workspace);
+  p.row_groups = plan.row_groups;
+  p.row_o = reinterpret_cast<float *>(space + plan.row_o);
+  p.row_ml = reinterpret_cast<float *>(space + plan.row_ml);
+  p.row_items = reinterpret_cast<int2 *>(space + plan.row_items);
+  p.splits = plan.splits;
+  p.tile_o = reinterpret_cast<float *>(space + plan.tile_o);
+  p.tile_ml = reinterpret_cast<float *>(space + plan.tile_ml);
+
+  float *us = o ? o->elapsed_us : nullptr;
+  KernelTimer timer(us != nullptr, o ? reinterpret_cast<hipStream_t>(o->stream) : nullptr);
+  const bool d128 = s->head_size == 128;
+#define FA_RAGGED(OT, KVF, MAPS)                                                       \
+  (d128 ? launch_ragged_kernels<128, OT, KVF, MAPS>(p, plan, timer, us)                \
+        : launch_ragged_kernels<64, OT, KVF, MAPS>(p, plan, timer, us))
+  const int c = s->cache_dtype;
+  if (diff) {
+    if (c == FA_KV_CACHE_I8) return FA_RAGGED(F16, kKvI8, 2);
+    return p.q_bf16 ? FA_RAGGED(BF16, kKv16, 2) : FA_RAGGED(F16, kKv16, 2);
+  }
+  if (c == FA_KV_CACHE_I8) return FA_RAGGED(F16, kKvI8, 1);
+  if (c == FA_KV_CACHE_E4M3) return FA_RAGGED(F16, kKvE4M3, 1);
+  if (c == FA_KV_CACHE_E5M2) return FA_RAGGED(F16, kKvE5M2, 1);
+  return p.q_bf16 ? FA_RAGGED(BF16, kKv16, 1) : FA_RAGGED(F16, kKv16, 1);
+#undef FA_RAGGED
+}
+
+}  // namespace fa

@@ -153,7 +153,15 @@ __device__ __forceinline__ uint32_t e5m2_adjacent_pair<BF16>(uint32_t w, int hal
 // FP8 cache formats.  kKvE5M2: 1-5-2, binary16 cut to its top byte.  kKvE4M3: 1-4-3 "fn"
 // (bias 7, no infinities, 0x7f / 0xff NaN), decoded by the CDNA4 conversion instructions;
 // both decode exactly into fp16 and bf16.
-constexpr int kKv16 = 0, kKvE5M2 = 1, kKvE4M3 = 2;
+// kKvI8: integers -127 .. 127 that a scale turns into values; into fp16 they decode exactly (fp16 operands only).
+constexpr int kKv16 = 0, kKvE5M2 = 1, kKvE4M3 = 2, kKvI8 = 3;
+
+// Integer bytes -> fp16 without a conversion instruction: 0x6400 | u is the fp16 1024 + u for u = 0 .. 255, and
+// u = b + 128 (b with its sign bit flipped), so subtracting 1152 leaves b, exactly.
+__device__ __forceinline__ uint32_t i8_debias(uint32_t two) {
+  const f16x2 bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, two) + bias);
+}
 
 // Decode byte k (0..3) of dword y into the low and byte k of dword x into the high 16-bit
 // half: the V transpose takes its two tokens from two registers.  One byte permute does the
@@ -162,7 +170,10 @@ constexpr int kKv16 = 0, kKvE5M2 = 1, kKvE4M3 = 2;
 template <int KVF, typename QT>
 __device__ __forceinline__ uint32_t fp8_pair_at(uint32_t y, uint32_t x, int k) {
   // v_perm_b32 selectors: 0..3 = bytes of the second operand, 4..7 = bytes of the first, 0x0c = 0
-  if constexpr (KVF == kKvE5M2 && std::is_same<QT, F16>::value) {
+  if constexpr (KVF == kKvI8) {
+    static_assert(std::is_same<QT, F16>::value, "integer caches decode into fp16");
+    return i8_debias(__builtin_amdgcn_perm(x, y, 0x0c000c00u | (uint32_t)k | ((uint32_t)(4 + k) << 16)) ^ 0x64806480u);
+  } else if constexpr (KVF == kKvE5M2 && std::is_same<QT, F16>::value) {
     return __builtin_amdgcn_perm(x, y, 0x000c000cu | ((uint32_t)k << 8) | ((uint32_t)(4 + k) << 24));
   } else {
     const uint32_t two = __builtin_amdgcn_perm(x, y, 0x0c0c0000u | (uint32_t)k | ((uint32_t)(4 + k) << 8));
@@ -179,7 +190,10 @@ __device__ __forceinline__ uint32_t fp8_pair_at(uint32_t y, uint32_t x, int k) {
 }
 template <int KVF, typename QT>
 __device__ __forceinline__ uint32_t fp8_adjacent_pair(uint32_t w, int half) {
-  if constexpr (KVF == kKvE4M3) {
+  if constexpr (KVF == kKvI8) {
+    static_assert(std::is_same<QT, F16>::value, "integer caches decode into fp16");
+    return i8_debias(__builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, half == 0 ? 0x04010400u : 0x04030402u));
+  } else if constexpr (KVF == kKvE4M3) {
     if constexpr (std::is_same<QT, BF16>::value) {
       const bf16x2 v = half == 0 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)
                                  : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);

@@ -112,6 +112,7 @@ constexpr int kScaleTensor = 0, kScaleHead = 1, kScaleBlock = 2;  // = fa_kv_sca
 template <int D, typename QT, int KVF, int TPC, bool STREAM, bool EXT = false, bool KROW = true>
 struct WaveAttn {
   static constexpr bool KV8 = KVF != kKv16;
+  using Operand = QT;
   static constexpr bool kExt = EXT;
   static_assert(TPC == 2 || TPC == 4, "a chunk is one or two 32-token P.V steps");
   static constexpr int ROWB = D * (KV8 ? 1 : 2);  // bytes per token row

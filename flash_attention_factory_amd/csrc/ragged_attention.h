@@ -1,0 +1,179 @@
+// What the kernels of ragged paged attention share: parameters, the split of the work, the two forms' common arithmetic.
+//
+// A row of the attention is (new token, query head[, softmax map]); the rows of one (sequence, kv head) -- new tokens times heads
+// per kv head times maps -- read the same K and V.  Sequences with few rows (one new token, or a handful) go through the rows
+// form (ragged_rows_kernel.h), bound by the bytes of K and V; the others through the tile form (ragged_tile_kernel.h), bound by the
+// matrix cores.  Both forms may run for one call; each takes the sequences that are its own.
+#pragma once
+
+#include "paged_attention_wave.h"
+#include "ragged_batch.h"
+
+namespace fa {
+
+struct RaggedParams {
+  PagedAttnParams a;            // the pools, as WaveAttn addresses them
+  RaggedBatch b;
+  const char *query;
+  char *out;
+  int64_t q_token_bytes, q_head_bytes;
+  const float *k_scales;        // byte pools: of (block, kv head) at [block * scale_pitch + kv head], scale_pitch 0: of kv heads
+  const float *v_scales;
+  int32_t scale_pitch;
+  int32_t block_scales;         // scales differ from block to block
+  float tensor_scale;           // byte pools without scale arrays
+  const void *sinks;
+  const float *alibi_slopes;
+  float softcap;
+  int32_t window;               // keys before a token's own that it sees; INT32_MAX / 2 without a window
+  int32_t mask_flags;           // kMaskAlibi | kMaskSoftcap (the window is in `window`)
+  float score_scale_log2;       // |scale| * log2(e), > 0
+  uint32_t query_flip;          // 0x80008000 for a negative scale: the queries change their sign instead
+  int32_t q_bf16;               // type of query and out: bf16, or fp16
+  int32_t num_heads, num_kv_heads, group;
+  int32_t max_query_len;
+  int32_t row_limit;            // sequences with at most so many rows per kv head go through the rows form
+  // differential attention
+  const float *lambdas;
+  const float *norm_weight;
+  float norm_eps, out_scale;
+  // rows form: work-groups, and their partial results
+  int32_t row_groups;
+  float *row_o;                 // [slot][16][D]
+  float *row_ml;                // [slot][2][16]: maxima (base-2 units), sums
+  int2 *row_items;              // [seq * kv heads + kv head]: first and last work-group of the item
+  // tile form
+  int32_t splits;               // pieces that the keys of a tile of rows are cut into
+  float *tile_o;                // [(tile * kv heads + kv head) * splits + piece][row][D]
+  float *tile_ml;               // [...][2][row]
+};
+
+constexpr int kRowColumns = 16;     // rows of the rows form: MFMA columns of a wavefront
+constexpr int kRowUnit = 128;       // keys that a work-group of the rows form takes at a time
+constexpr int kTileKeys = 64;       // keys per step of the tile form
+constexpr int kNoWindow = 0x3fffffff;
+
+// The reference that sums and weights are taken against is set kHeadroom binary orders below the maximum, and follows it only
+// when it lags by more than kRefresh (every change costs a pass over the accumulators).  Probabilities reach 2^kRefresh then: within
+// fp16's range, and its subnormal numbers, which round to 2^-25 whatever their size, begin at 2^-20 of the largest
+// instead of 2^-14.  Sums and accumulators are 32 bits wide.
+constexpr float kHeadroom = 6.0f, kRefresh = 14.0f;
+
+__device__ __forceinline__ RaggedSeq ragged_seq_cut(const RaggedParams &p, RaggedSeq q) {
+  q.n = min(q.n, p.max_query_len);
+  return q;
+}
+template <int MAPS>
+__device__ __forceinline__ bool in_rows_form(const RaggedParams &p, const RaggedSeq &q) {
+  return q.n * p.group * MAPS <= p.row_limit;
+}
+// First key that some new token of the sequence sees.
+__device__ __forceinline__ int first_key(const RaggedParams &p, const RaggedSeq &q) { return max(0, q.ctx - q.n - p.window); }
+
+// Units of keys that the rows form has to go through for one kv head of a sequence.
+template <int MAPS>
+__device__ __forceinline__ int row_units(const RaggedParams &p, RaggedSeq q) {
+  q = ragged_seq_cut(p, q);
+  if (q.n <= 0 || !in_rows_form<MAPS>(p, q)) return 0;
+  return (q.ctx + kRowUnit - 1) / kRowUnit - first_key(p, q) / kRowUnit;
+}
+// Tiles of `rows` rows that the tile form has to go through for one kv head of a sequence.
+template <int MAPS, int ROWS>
+__device__ __forceinline__ int row_tiles(const RaggedParams &p, RaggedSeq q) {
+  q = ragged_seq_cut(p, q);
+  if (q.n <= 0 || in_rows_form<MAPS>(p, q)) return 0;
+  return (q.n * p.group + ROWS - 1) / ROWS;
+}
+
+// Sixteen query bits pairs, with the sign of the scale; as fp16 for byte pools.  bf16 queries are brought into fp16's range by a
+// power of two of their own row (exact but for values 2^-22 and less of the row's largest): `e` is its exponent field, found by
+// the caller from the largest magnitude of the whole row.
+__device__ __forceinline__ uint32_t query_exponent(float largest) {
+  const uint32_t e = (__builtin_bit_cast(uint32_t, largest) >> 23) & 255u;
+  return min(max(e, 8u), 254u);
+}
+__device__ __forceinline__ u32x4 bf16_row_to_f16(u32x4 w, uint32_t e) {
+  const float mul = __builtin_bit_cast(float, (261u - e) << 23);  // the row's largest value comes to lie in [2^7, 2^8)
+  u32x4 o;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    o[k] = pack2<F16>(__builtin_bit_cast(float, w[k] << 16) * mul, __builtin_bit_cast(float, w[k] & 0xffff0000u) * mul);
+  return o;
+}
+__device__ __forceinline__ float bf16_row_scale(uint32_t e) { return __builtin_bit_cast(float, (e - 7u) << 23); }
+__device__ __forceinline__ float largest_of_bf16(u32x4 w, float most) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    most = fmaxf(most, fmaxf(fabsf(__builtin_bit_cast(float, w[k] << 16)), fabsf(__builtin_bit_cast(float, w[k] & 0xffff0000u))));
+  return most;
+}
+
+__device__ __forceinline__ uint32_t pack_out(const RaggedParams &p, float lo, float hi) {
+  return p.q_bf16 ? pack2<BF16>(lo, hi) : pack2<F16>(lo, hi);
+}
+
+// cap * tanh(x / cap) of a score in base-2 units; tanh(z) = 1 - 2 / (exp(2z) + 1)
+__device__ __forceinline__ float soft_capped(float t, float cap) {
+  const float e2 = fast_exp2(t * (2.0f / cap));  // exp(2 x / cap), x = t ln 2
+  return cap * kLog2e * (1.0f - 2.0f * __builtin_amdgcn_rcpf(e2 + 1.0f));
+}
+
+// Sink logit of a head in base-2 units.
+__device__ __forceinline__ float sink_log2(const RaggedParams &p, int head) {
+  return (p.q_bf16 ? load_scalar16<BF16>(reinterpret_cast<const char *>(p.sinks) + head * 2)
+                   : load_scalar16<F16>(reinterpret_cast<const char *>(p.sinks) + head * 2)) * kLog2e;
+}
+
+// The differential result of one row from its two maps: lane l of a wavefront holds the N elements from l * N on.
+template <int N>
+__device__ __forceinline__ void differential_row(const RaggedParams &p, int head, int lane, const float (&o1)[N], const float (&o2)[N],
+                                                 float (&x)[N]) {
+  const float lambda = p.lambdas[head];
+  float square = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    x[k] = o1[k] - lambda * o2[k];
+    square += x[k] * x[k];
+  }
+  if (p.norm_weight == nullptr) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] *= p.out_scale;
+    return;
+  }
+  const float mul = p.out_scale / sqrtf(wave_sum(square) / (64.0f * N) + p.norm_eps);
+#pragma unroll
+  for (int k = 0; k < N; ++k) x[k] *= mul * p.norm_weight[lane * N + k];
+}
+
+// N 16-bit elements from lane * N on of an output row.
+template <int N>
+__device__ __forceinline__ void store_row(const RaggedParams &p, int token, int head, int lane, const float (&x)[N]) {
+  char *dst = p.out + ((int64_t)token * p.num_heads + head) * (64 * N * 2) + lane * (N * 2);
+  if constexpr (N == 2) {
+    *reinterpret_cast<uint32_t *>(dst) = pack_out(p, x[0], x[1]);
+  } else {
+    *reinterpret_cast<uint16_t *>(dst) = (uint16_t)pack_out(p, x[0], 0.f);
+  }
+}
+
+// Partial results of one row: running maximum, sum and weighted values, merged in the order of the pieces.
+template <int N>
+struct RowMerge {
+  float m = -INFINITY, l = 0.f, o[N] = {};
+  __device__ __forceinline__ void add(float pm, float pl, const float (&po)[N]) {
+    const float to = fmaxf(m, pm);
+    const float sub = to == -INFINITY ? 0.f : to;
+    const float mine = fast_exp2(m - sub), its = fast_exp2(pm - sub);
+    l = l * mine + pl * its;
+#pragma unroll
+    for (int k = 0; k < N; ++k) o[k] = o[k] * mine + po[k] * its;
+    m = to;
+  }
+  __device__ __forceinline__ void normalise() {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int k = 0; k < N; ++k) o[k] *= inv;
+  }
+};
+
+}  // namespace fa

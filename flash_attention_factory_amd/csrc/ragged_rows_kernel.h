@@ -1,0 +1,380 @@
+// Ragged paged attention, rows form: at most 16 rows (new token, query head, map) per (sequence, kv head), the 16 columns of an
+// MFMA tile; bound by the bytes of K and V.
+//
+// Split of the work: the keys of every (sequence, kv head) are cut into units of 128 and all units of the batch are laid end to end;
+// the resident work-groups take equal shares of that line, whatever the lengths of the sequences are.  A share may end within an item
+// (sequence, kv head); its piece of the item goes to the workspace as an unnormalised sum with its maximum, in slot
+// item + work-group (both only grow along the line, so no two pieces meet), and ragged_rows_merge_kernel joins the pieces in their
+// order.  No atomics: results do not vary from run to run.
+//
+// Within a unit each of the four wavefronts takes 32 keys (WaveAttn: operands straight from the pool, no LDS) and keeps a softmax
+// state of its own; the states merge through LDS at the end of a piece.
+//
+// Scales of the blocks of a byte pool: K's multiply the scores.  V's may not simply ride on the probabilities, which go to
+// the matrix cores in 16 bits: a block of small values next to one of large ones would lose them.  So the weights have a running
+// maximum of their own, mv = max(score + log2(V scale)): weight = 2^(score - m) 2^(m + log2(V scale) - mv), the second
+// factor once per block, and sums and weights meet at the end, in 32 bits.
+#pragma once
+
+#include "ragged_attention.h"
+
+namespace fa {
+
+// Softmax state of a wavefront: column i's maximum (mt) and reference (m), sum (l); the same for the weights of V.
+struct RowState {
+  float m, mt, l, mv, mvt;
+};
+
+// Multipliers of a chunk's two 16-key tiles.
+struct RowScales {
+  float k[2];   // raw score -> base-2 units, without the column's own factor
+  float lv[2];  // log2 of the V scale
+};
+
+template <typename W>
+struct RowColumns {
+  float mul;         // what the column's raw scores are multiplied with (fp16 queries: 1)
+  float slope_log2;
+  int pos;           // position of the column's token
+  int vis_lo, vis_hi;  // keys that every column sees
+};
+
+template <bool KV8, typename W>
+__device__ __forceinline__ typename W::Probs row_soft(W &wa, RowState &st, const RowColumns<W> &col, typename W::Chunk &R,
+                                                      const typename W::Scores &s, const RowScales &sc, int ci, int ctx,
+                                                      const RaggedParams &p) {
+  constexpr int NT = 8;
+  float t[NT];
+#pragma unroll
+  for (int e = 0; e < NT; ++e) t[e] = s.v[e >> 2][e & 3] * (sc.k[e >> 2] * col.mul);
+  const int t0 = ci * W::CT;
+  if (p.mask_flags & kMaskSoftcap) {
+#pragma unroll
+    for (int e = 0; e < NT; ++e) t[e] = soft_capped(t[e], p.softcap);
+  }
+  if (p.mask_flags & kMaskAlibi) {
+#pragma unroll
+    for (int e = 0; e < NT; ++e) t[e] += col.slope_log2 * (float)(t0 + (e >> 2) * 16 + 4 * wa.r + (e & 3) - col.pos);
+  }
+  if (t0 < col.vis_lo || t0 + W::CT - 1 > col.vis_hi) {  // the same for the wavefront
+#pragma unroll
+    for (int e = 0; e < NT; ++e) {
+      const int tok = t0 + (e >> 2) * 16 + 4 * wa.r + (e & 3);
+      if (tok > col.pos || tok < col.pos - p.window) t[e] = -INFINITY;  // select: the pool may hold NaN there
+      if (tok >= ctx) {
+#pragma unroll
+        for (int w = 0; w < W::VW; ++w) R.v[e][w] = 0u;
+      }
+    }
+  }
+  float mx[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) mx[h] = fmaxf(fmaxf(t[4 * h], t[4 * h + 1]), fmaxf(t[4 * h + 2], t[4 * h + 3]));
+  st.mt = fmaxf(st.mt, rows_max(fmaxf(mx[0], mx[1])));
+  const bool blocks = KV8 && p.block_scales;
+  if (__builtin_expect(__any(st.mt - st.m > kRefresh), 0)) {
+    const float to = st.mt - kHeadroom;
+    const float alpha = st.m == -INFINITY ? 0.f : fast_exp2(st.m - to);
+    st.l *= alpha;
+    if (!blocks) {
+#pragma unroll
+      for (int dt = 0; dt < W::NDT; ++dt) wa.acc[dt] *= alpha;
+    }
+    st.m = to;
+  }
+  const float sub = st.m == -INFINITY ? 0.f : st.m;
+  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < NT; ++e) {
+    t[e] = fast_exp2(t[e] - sub);
+    sum += t[e];
+  }
+  st.l += sum;
+  if (blocks) {
+    st.mvt = fmaxf(st.mvt, rows_max(fmaxf(mx[0] + sc.lv[0], mx[1] + sc.lv[1])));
+    if (__builtin_expect(__any(st.mvt - st.mv > kRefresh), 0)) {
+      const float to = st.mvt - kHeadroom;
+      const float alpha = st.mv == -INFINITY ? 0.f : fast_exp2(st.mv - to);
+#pragma unroll
+      for (int dt = 0; dt < W::NDT; ++dt) wa.acc[dt] *= alpha;
+      st.mv = to;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // (cut so that a weight of 0 stays 0 where the factor would overflow)
+      const float f = st.mv == -INFINITY ? 0.f : fast_exp2(fminf(sub + sc.lv[h] - st.mv, 126.0f));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[4 * h + e] *= f;
+    }
+  }
+  typename W::Probs pb;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) pb.v[0][c] = pack2<typename W::Operand>(t[2 * c], t[2 * c + 1]);
+  return pb;
+}
+
+template <int D, typename OT, int KVF, int MAPS>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ragged_rows_kernel(const RaggedParams p) {
+  constexpr bool KV8 = KVF != kKv16;
+  constexpr int NW = 4;
+  using W = WaveAttn<D, OT, KVF, 2, Pipeline<KV8>::stream_loads_loop, false, true>;
+  constexpr int NR = W::NR, NDT = W::NDT, SL = NR / NW;
+  static_assert(W::CT * NW == kRowUnit, "a unit is one chunk per wavefront");
+  __shared__ float lds[NW * (NR * 64 + 32)];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int Hk = p.num_kv_heads, G = p.group;
+
+  // this work-group's share of the line of units
+  int32_t mine = 0;
+  for (int s = lane; s < p.b.num_seqs; s += 64) mine += row_units<MAPS>(p, ragged_seq_of_lane(p.b, s));
+  const int32_t total = __builtin_amdgcn_readlane(wave_inclusive_scan(mine, lane), 63) * Hk;
+  const int groups = min(p.row_groups, total);
+  const int g = blockIdx.x;
+  if (g >= groups) return;
+  int32_t u = (int32_t)((int64_t)total * g / groups);
+  const int32_t u_end = (int32_t)((int64_t)total * (g + 1) / groups);
+  const RaggedPlace at = ragged_find(p.b.num_seqs, u, lane,
+                                     [&](int s) { return row_units<MAPS>(p, ragged_seq_of_lane(p.b, s)) * Hk; });
+  int seq = __builtin_amdgcn_readfirstlane(at.seq);
+  int32_t before = __builtin_amdgcn_readfirstlane(at.before);
+
+  W wa(p.a, lane);
+  const int r = wa.r, i = wa.i;
+  while (u < u_end) {
+    RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq));
+    const int units = row_units<MAPS>(p, q);
+    if (u >= before + units * Hk) {
+      before += units * Hk;
+      ++seq;
+      continue;
+    }
+    const int kvh = (u - before) / units;
+    const int first = (u - before) - kvh * units;
+    const int last = min(units, first + (u_end - u));
+    const int item = seq * Hk + kvh;
+    u += last - first;
+    const int base_unit = first_key(p, q) / kRowUnit;
+    const int tok_begin = (base_unit + first) * kRowUnit, tok_end = min(q.ctx, (base_unit + last) * kRowUnit);
+    const int32_t *table = p.b.block_tables + (int64_t)seq * p.b.max_blocks_per_seq;
+    const int last_col = p.b.max_blocks_per_seq - 1;
+    int ci = tok_begin / W::CT + wave;
+    const int c_end = (tok_end + W::CT - 1) / W::CT;
+
+    // block scales of a chunk; tiles past the context take 1, whatever the block that their id names holds
+    auto fetch_scales = [&](const typename W::Ids &ids, int c) {
+      RowScales x;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        x.k[t] = p.score_scale_log2;
+        x.lv[t] = 0.f;
+        if constexpr (KV8) {
+          if (p.k_scales == nullptr) {
+            x.k[t] *= p.tensor_scale;
+          } else {
+            const int64_t idx = (int64_t)ids.v[t] * p.scale_pitch + kvh;
+            const bool there = c * W::CT + t * 16 < q.ctx;
+            const float ks = load_uniform_f32(p.k_scales + idx), vs = load_uniform_f32(p.v_scales + idx);
+            x.k[t] = there ? x.k[t] * ks : x.k[t];
+            x.lv[t] = there && p.block_scales ? __builtin_amdgcn_logf(vs) : 0.f;
+          }
+        }
+      }
+      return x;
+    };
+
+    // columns
+    const int map = MAPS == 2 ? i & 1 : 0, row = MAPS == 2 ? i >> 1 : i;
+    const int j = row / G;
+    const bool valid = row < q.n * G;
+    const int head = kvh * G + (row - j * G);
+    RowColumns<W> col;
+    col.mul = 1.f;
+    col.pos = q.ctx - q.n + j;
+    col.vis_hi = q.ctx - q.n;
+    col.vis_lo = q.ctx - 1 - p.window;
+    col.slope_log2 = (p.mask_flags & kMaskAlibi) && valid ? p.alibi_slopes[head] * kLog2e : 0.f;
+    const char *qrow = p.query + (int64_t)(q.first + (valid ? j : 0)) * p.q_token_bytes + (valid ? head : 0) * p.q_head_bytes;
+    u32x4 qv[W::KSTEPS];
+#pragma unroll
+    for (int c = 0; c < W::KSTEPS; ++c) {
+      const int d0 = KV8 ? ((c >> 1) * 4 + r) * 16 + (c & 1) * 8 : (c * 4 + r) * 8;
+      u32x4 z = {0u, 0u, 0u, 0u};
+      const bool live = valid && (MAPS == 1 || (d0 >= D / 2) == (map == 1));
+      qv[c] = live ? *reinterpret_cast<const u32x4 *>(qrow + d0 * 2) : z;
+    }
+    RowState st;
+    st.m = st.mt = st.mv = st.mvt = -INFINITY;
+    st.l = 0.f;
+    if (p.sinks != nullptr && valid && first == 0 && wave == 0) {
+      st.m = st.mt = sink_log2(p, head);
+      st.l = r == 0 ? 1.f : 0.f;
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) wa.acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (ci < c_end) {
+      typename W::Chunk R;
+      typename W::Ids ids = wa.fetch_ids(table, ci, last_col);
+      wa.issue_k(R, kvh, ci, ids);
+      wa.issue_v(R, kvh, ci, ids);
+      RowScales sc = fetch_scales(ids, ci), nsc = sc;
+      ids = wa.fetch_ids(table, ci + NW, last_col);
+      if (KV8 && p.q_bf16) {
+        float most = 0.f;
+#pragma unroll
+        for (int c = 0; c < W::KSTEPS; ++c) most = largest_of_bf16(qv[c], most);
+        const uint32_t e = query_exponent(rows_max(most));
+#pragma unroll
+        for (int c = 0; c < W::KSTEPS; ++c) qv[c] = bf16_row_to_f16(qv[c], e);
+        col.mul = bf16_row_scale(e);
+      }
+#pragma unroll
+      for (int c = 0; c < W::KSTEPS; ++c)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) wa.qB[c][k] = qv[c][k] ^ p.query_flip;
+      while (ci + NW < c_end) {
+        const int cn = ci + NW;
+        const auto s = wa.qk(R);
+        wa.issue_k(R, kvh, cn, ids);
+        nsc = fetch_scales(ids, cn);
+        const auto pb = row_soft<KV8>(wa, st, col, R, s, sc, ci, q.ctx, p);
+        wa.pv(R, pb);
+        wa.issue_v(R, kvh, cn, ids);
+        ids = wa.fetch_ids(table, cn + NW, last_col);
+        sc = nsc;
+        ci = cn;
+      }
+      const auto s = wa.qk(R);
+      wa.pv(R, row_soft<KV8>(wa, st, col, R, s, sc, ci, q.ctx, p));
+    }
+
+    // Merge: sums and weights against the true maximum, then the wavefronts' states through LDS.  Wavefront w keeps the
+    // slice [w * SL, (w + 1) * SL) of every lane's NR consecutive elements.
+    {
+      const float to = st.mt == -INFINITY ? 0.f : st.mt;
+      const float from = KV8 && p.block_scales ? st.mv : st.m;
+      const float f = from == -INFINITY ? 0.f : fast_exp2(from - to);
+      st.l = rows_sum(st.l) * (st.m == -INFINITY ? 0.f : fast_exp2(st.m - to));
+      float (*sm_acc)[NR][64] = reinterpret_cast<float (*)[NR][64]>(lds);
+      float (*sm_m)[16] = reinterpret_cast<float (*)[16]>(lds + NW * NR * 64);
+      float (*sm_l)[16] = reinterpret_cast<float (*)[16]>(lds + NW * NR * 64 + NW * 16);
+      __syncthreads();  // (the piece before this one has been read)
+      if (r == 0) {
+        sm_m[wave][i] = st.mt;
+        sm_l[wave][i] = st.l;
+      }
+#pragma unroll
+      for (int k = 0; k < NR; ++k) sm_acc[wave][k][lane] = wa.acc_at(k) * f;
+      __syncthreads();
+      float M = sm_m[0][i], L = 0.f, o[SL];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) M = fmaxf(M, sm_m[w][i]);
+      const float sub = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int k = 0; k < SL; ++k) o[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float fw = fast_exp2(sm_m[w][i] - sub);
+        L += fw * sm_l[w][i];
+#pragma unroll
+        for (int k = 0; k < SL; ++k) o[k] += fw * sm_acc[w][wave * SL + k][lane];
+      }
+      const float v_mul = !KV8 ? 1.f : p.block_scales ? 1.f : p.v_scales ? load_uniform_f32(p.v_scales + kvh) : p.tensor_scale;
+      const int d0 = 4 * r * NDT + wave * SL;
+      const bool whole = first == 0 && last == units;
+      if (MAPS == 1 && whole) {
+        if (valid) {
+          const float inv = L == 0.f ? 0.f : v_mul / L;
+          char *dst = p.out + (((int64_t)(q.first + j) * p.num_heads + head) * D + d0) * 2;
+#pragma unroll
+          for (int k = 0; k < SL; k += 2) *reinterpret_cast<uint32_t *>(dst + 2 * k) = pack_out(p, o[k] * inv, o[k + 1] * inv);
+        }
+      } else {
+        const int64_t slot = (int64_t)item + g;
+        if (valid) {
+          float *dst = p.row_o + (slot * kRowColumns + i) * D + d0;
+#pragma unroll
+          for (int k = 0; k < SL; k += 4)
+            *reinterpret_cast<f32x4 *>(dst + k) = f32x4{o[k] * v_mul, o[k + 1] * v_mul, o[k + 2] * v_mul, o[k + 3] * v_mul};
+        }
+        if (wave == 0 && r == 0) {
+          p.row_ml[slot * 2 * kRowColumns + i] = M;
+          p.row_ml[slot * 2 * kRowColumns + kRowColumns + i] = L;
+        }
+      }
+      if (first == 0 && threadIdx.x == 0) {  // the work-groups that hold the item's pieces
+        const int64_t end = (int64_t)before + (int64_t)kvh * units + units;
+        p.row_items[item] = int2{g, (int)((end * groups - 1) / total)};
+      }
+    }
+  }
+}
+
+// Joins the pieces of an item's rows.  Work-group (item, row); its four wavefronts take every fourth piece each.
+template <int D, int MAPS>
+__global__ void __launch_bounds__(256) ragged_rows_merge_kernel(const RaggedParams p) {
+  constexpr int N = D / 64;
+  __shared__ float sm[MAPS][4][N + 2][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = blockIdx.x, row = blockIdx.y;
+  const int seq = item / p.num_kv_heads, kvh = item - seq * p.num_kv_heads;
+  const RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq));
+  if (row >= q.n * p.group || !in_rows_form<MAPS>(p, q)) return;
+  const int j = row / p.group, head = kvh * p.group + (row - j * p.group);
+  int2 span = {0, -1};  // (no keys: no pieces)
+  if (row_units<MAPS>(p, q) > 0) {
+    span.x = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_items + item));
+    span.y = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_items + item) + 1);
+    if (MAPS == 1 && span.x == span.y) return;  // the rows kernel has stored the result
+  }
+  RowMerge<N> of[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    const int c = MAPS == 2 ? row * 2 + m : row;
+#pragma unroll 4
+    for (int g = span.x + wave; g <= span.y; g += 4) {
+      const int64_t slot = (int64_t)item + g;
+      const float pm = p.row_ml[slot * 2 * kRowColumns + c], pl = p.row_ml[slot * 2 * kRowColumns + kRowColumns + c];
+      const float *src = p.row_o + (slot * kRowColumns + c) * D + lane * N;
+      float po[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) po[k] = src[k];
+      of[m].add(pm, pl, po);
+    }
+  }
+  if (span.y - span.x >= 1) {
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      sm[m][wave][0][lane] = of[m].m;
+      sm[m][wave][1][lane] = of[m].l;
+#pragma unroll
+      for (int k = 0; k < N; ++k) sm[m][wave][2 + k][lane] = of[m].o[k];
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        float po[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) po[k] = sm[m][w][2 + k][lane];
+        of[m].add(sm[m][w][0][lane], sm[m][w][1][lane], po);
+      }
+  }
+  if (wave != 0) return;
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) of[m].normalise();
+  if constexpr (MAPS == 2) {
+    float x[N];
+    differential_row<N>(p, head, lane, of[0].o, of[1].o, x);
+    store_row<N>(p, q.first + j, head, lane, x);
+  } else {
+    store_row<N>(p, q.first + j, head, lane, of[0].o);
+  }
+}
+
+}  // namespace fa

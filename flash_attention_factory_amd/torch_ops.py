@@ -18,6 +18,16 @@ recorded into a HIP graph (``torch.cuda.graph``) and replayed.
     torch.ops.fa_amd.paged_attention_fp8_reduce(..., scale, fp8_scale, partition_size, sinks)
     torch.ops.fa_amd.kv_cache_write(key, value, key_cache, value_cache, slot_mapping, fp8_scale)
 
+and, for ragged batches (any number of new tokens per sequence: ``query_start``, ``context_lens``),
+
+    torch.ops.fa_amd.kv_cache_append(key, value, key_cache, value_cache, block_tables, query_start,
+                                     context_lens, cos_sin, query, query_out, k_scales, v_scales)
+    torch.ops.fa_amd.paged_attention_ragged(out, query, key_cache, value_cache, block_tables,
+                                            query_start, context_lens, scale, max_query_len)
+    torch.ops.fa_amd.paged_attention_differential(out, query, key_cache, value_cache, block_tables,
+                                                  query_start, context_lens, scale, lambdas,
+                                                  norm_weight, max_query_len)
+
 Further optional arguments, all off by default: ``alibi_slopes`` (fp32 ``[heads]``), ``softcap``
 (> 0) and ``window_left`` (>= 0) apply the score modifiers -- here a modifier that is passed is
 applied, unlike ``lib.*.run``, which mirrors upstream in taking and ignoring slopes and cap; the
@@ -51,9 +61,10 @@ import torch
 from torch import Tensor
 
 from . import _build, _cabi
-from .lib import (kv_cache_write as _kv_cache_write, paged_attention_fp8_loop as _fp8_loop,
+from .lib import (kv_cache_append as _kv_cache_append, kv_cache_write as _kv_cache_write,
+                  paged_attention_differential as _differential, paged_attention_fp8_loop as _fp8_loop,
                   paged_attention_fp8_reduce as _fp8_reduce, paged_attention_loop as _loop,
-                  paged_attention_reduce as _reduce)
+                  paged_attention_ragged as _ragged, paged_attention_reduce as _reduce)
 
 _NS = "fa_amd_py"
 
@@ -153,14 +164,48 @@ def kv_cache_write(key: Tensor, value: Tensor, key_cache: Tensor, value_cache: T
                         k_scales=k_scales, v_scales=v_scales)
 
 
+@torch.library.custom_op(f"{_NS}::kv_cache_append",
+                         mutates_args=("key_cache", "value_cache", "query_out", "k_scales", "v_scales"), device_types="cuda")
+def kv_cache_append(key: Tensor, value: Tensor, key_cache: Tensor, value_cache: Tensor, block_tables: Tensor,
+                    query_start: Tensor, context_lens: Tensor, cos_sin: Optional[Tensor] = None,
+                    query: Optional[Tensor] = None, query_out: Optional[Tensor] = None,
+                    k_scales: Optional[Tensor] = None, v_scales: Optional[Tensor] = None, fp8_scale: float = 1.0,
+                    interleaved: bool = False) -> None:
+    _kv_cache_append.run(key, value, key_cache, value_cache, block_tables, query_start, context_lens, cos_sin, query,
+                         query_out, k_scales, v_scales, fp8_scale, interleaved, timed=False)
+
+
+@torch.library.custom_op(f"{_NS}::paged_attention_ragged", mutates_args=("out",), device_types="cuda")
+def paged_attention_ragged(out: Tensor, query: Tensor, key_cache: Tensor, value_cache: Tensor, block_tables: Tensor,
+                           query_start: Tensor, context_lens: Tensor, scale: float, max_query_len: int,
+                           max_context_len: int = 0, fp8_scale: float = 1.0, k_scales: Optional[Tensor] = None,
+                           v_scales: Optional[Tensor] = None, sinks: Optional[Tensor] = None,
+                           alibi_slopes: Optional[Tensor] = None, softcap: float = 0.0, window_left: int = -1) -> None:
+    _ragged.run(out, query, key_cache, value_cache, block_tables, query_start, context_lens, scale, max_query_len,
+                max_context_len, fp8_scale, k_scales, v_scales, sinks, alibi_slopes, softcap, window_left, timed=False)
+
+
+@torch.library.custom_op(f"{_NS}::paged_attention_differential", mutates_args=("out",), device_types="cuda")
+def paged_attention_differential(out: Tensor, query: Tensor, key_cache: Tensor, value_cache: Tensor, block_tables: Tensor,
+                                 query_start: Tensor, context_lens: Tensor, scale: float, lambdas: Tensor,
+                                 norm_weight: Optional[Tensor], max_query_len: int, max_context_len: int = 0,
+                                 norm_eps: float = 1e-5, out_scale: float = 1.0, k_scales: Optional[Tensor] = None,
+                                 v_scales: Optional[Tensor] = None, window_left: int = -1) -> None:
+    _differential.run(out, query, key_cache, value_cache, block_tables, query_start, context_lens, scale, lambdas,
+                      norm_weight, max_query_len, max_context_len, norm_eps, out_scale, k_scales, v_scales, window_left,
+                      timed=False)
+
+
 _NAMES = ("paged_attention_loop", "paged_attention_fp8_loop", "paged_attention_reduce", "paged_attention_fp8_reduce",
-          "kv_cache_write")
+          "kv_cache_write", "kv_cache_append", "paged_attention_ragged", "paged_attention_differential")
 
 
 def _bind(L: ctypes.CDLL) -> None:
     """The C ABI's entry points, for the native operators."""
     entries = (L.fa_paged_attention_loop, L.fa_paged_attention_fp8_loop, L.fa_paged_attention_reduce,
-               L.fa_paged_attention_fp8_reduce, L.fa_kv_cache_write, L.fa_paged_attention_loop_workspace_bytes)
+               L.fa_paged_attention_fp8_reduce, L.fa_kv_cache_write, L.fa_paged_attention_loop_workspace_bytes,
+               L.fa_kv_cache_append, L.fa_paged_attention_ragged, L.fa_paged_attention_differential,
+               L.fa_paged_attention_ragged_workspace_bytes)
     table = (ctypes.c_void_p * len(entries))(*(ctypes.cast(e, ctypes.c_void_p).value for e in entries))
     global _native
     native = ctypes.CDLL(_build.TORCH_OPS_LIBRARY)
@@ -203,5 +248,7 @@ _fragment = _load_native()
 # Shape propagation for tracing: every operator only writes into its arguments.
 for _name in _NAMES:
     globals()[_name].register_fake(lambda *args, **kwargs: None)
+    if not hasattr(torch.ops.fa_amd, _name):  # operators of other sources: loading the C ABI's library says so
+        continue
     torch.library.register_fake(f"fa_amd::{_name}", lambda *args, **kwargs: None)
     globals()[_name] = getattr(torch.ops.fa_amd, _name)
