@@ -102,10 +102,16 @@ inline fa_status launch_ragged_kernels(const RaggedParams &p, const RaggedPlan &
   fa_status st = FA_OK;
   if (plan.tiles) {
     const dim3 grid((unsigned)(plan.tile_bound * Hk), (unsigned)plan.splits);
-    if (plan.wavefronts == 8)
-      FA_HIP_CHECK(timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 8>, grid, dim3(512), 0, p));
-    else
-      FA_HIP_CHECK(timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 4>, grid, dim3(256), 0, p));
+    const auto launch = [&](auto ext) {
+      constexpr bool kExt = decltype(ext)::value;
+      return plan.wavefronts == 8 ? timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 8, kExt>, grid, dim3(512), 0, p)
+                                  : timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 4, kExt>, grid, dim3(256), 0, p);
+    };
+    if constexpr (MAPS == 1) {
+      FA_HIP_CHECK(p.mask_flags ? launch(std::true_type{}) : launch(std::false_type{}));
+    } else {
+      FA_HIP_CHECK(launch(std::false_type{}));
+    }
     if ((st = timed()) != FA_OK) return st;
     if (plan.splits > 1) {
       const dim3 merge((unsigned)(plan.tile_bound * Hk), (unsigned)(plan.tile_rows / 16));
@@ -147,6 +153,8 @@ inline fa_status launch_ragged_attention(void *out, const void *query, const voi
     return fail(FA_ERR_BAD_SHAPE, "kv strides must be positive and cover one head_size row");
   if ((s->kv_block_stride * eb) % 16 || (s->kv_token_stride * eb) % 16 || (s->kv_head_stride * eb) % 16)
     return fail(FA_ERR_BAD_SHAPE, "kv strides must be multiples of 16 bytes");
+  if (s->kv_block_stride * eb > 0xffffffffLL || s->kv_token_stride * eb > 0xffffffffLL)
+    return fail(FA_ERR_BAD_SHAPE, "kv_block_stride and kv_token_stride must be under 4 GiB");
   if (s->query_token_stride < s->head_size || s->query_head_stride < s->head_size || s->query_token_stride % 8 || s->query_head_stride % 8)
     return fail(FA_ERR_BAD_SHAPE, "query strides must cover one head_size row and be multiples of 16 bytes");
   if (((uintptr_t)out | (uintptr_t)query | (uintptr_t)key_cache | (uintptr_t)value_cache | (uintptr_t)workspace) % 16)

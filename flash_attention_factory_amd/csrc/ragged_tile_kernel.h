@@ -39,6 +39,21 @@ __device__ __forceinline__ u32x2 lds_read_transposed(const char *at) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// c + the two 16-bit values of a dword
+template <typename OT>
+__device__ __forceinline__ float add_pair(uint32_t two, float c) {
+  if constexpr (std::is_same<OT, BF16>::value) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), __builtin_bit_cast(bf16x2, 0x3f803f80u), c, false);
+  } else {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, two), __builtin_bit_cast(f16x2, 0x3c003c00u), c, false);
+  }
+}
+
 // The larger / the sum of the two lanes l and l ^ 32, in both.
 __device__ __forceinline__ float halves_max(float v) {
   const uint32_t a = __builtin_bit_cast(uint32_t, v);
@@ -74,7 +89,7 @@ struct RaggedTile {
   }
 };
 
-template <int D, typename OT, int KVF, int MAPS, int NW>
+template <int D, typename OT, int KVF, int MAPS, int NW, bool EXT>
 __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) ragged_tile_kernel(const RaggedParams p) {
   using T = RaggedTile<D, KVF, MAPS, NW>;
   constexpr bool KV8 = T::KV8;
@@ -140,7 +155,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
 #pragma unroll
       for (int k = 0; k < 4; ++k) qv[c][k] ^= p.query_flip;
   }
-  const float slope = (p.mask_flags & kMaskAlibi) ? p.alibi_slopes[head] * kLog2e : 0.f;
+  const float slope = EXT && (p.mask_flags & kMaskAlibi) ? p.alibi_slopes[head] * kLog2e : 0.f;
 
   float m = -INFINITY, mt = -INFINITY, l = 0.f, mv = -INFINITY, mvt = -INFINITY;
   if (p.sinks != nullptr && blockIdx.y == 0) {
@@ -158,211 +173,349 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const int piece = tid % T::kPerRow, load_row = tid / T::kPerRow;
   const bool loads = T::kRowsPerPass <= kTileKeys || load_row < kTileKeys;
   const int last_col = p.b.max_blocks_per_seq - 1, in_block = (1 << p.b.block_shift) - 1;
-  int32_t ids[T::kPasses];
+  const int steps = max(0, step_end - step);
+  // Blocks of this thread's rows: of the next step of K as the table has them (cut to the pool where they are used, since
+  // arithmetic here would wait for the load, and for every load before it), and of the next step of V, one step behind.
+  int32_t kid[T::kPasses], vid[T::kPasses];
   u32x4 kreg[T::kPasses], vreg[T::kPasses];
-  auto fetch_ids = [&](int st) {
+  // A thread's row within its block is the same in every step, but for what a step's first key lies into a block of more than 64.
+  const uint32_t block_bytes = (uint32_t)p.a.kv_block_bytes, token_bytes = (uint32_t)p.a.kv_token_bytes;
+  const char *k_row[T::kPasses], *v_row[T::kPasses];
+  int32_t row_col[T::kPasses];  // the thread's row in block-table columns from the step's first
+#pragma unroll
+  for (int x = 0; x < T::kPasses; ++x) {
+    const int key = x * T::kRowsPerPass + load_row;
+    const int64_t off = (int64_t)kvh * p.a.kv_head_bytes + piece * 16 + (int64_t)((uint64_t)(uint32_t)(key & in_block) * token_bytes);
+    k_row[x] = p.a.key_cache + off;
+    v_row[x] = p.a.value_cache + off;
+    row_col[x] = key >> p.b.block_shift;
+  }
+  auto fetch_id = [&](int n, int x) {
+    return table[(uint32_t)min(((step + n) * kTileKeys >> p.b.block_shift) + row_col[x], last_col)];
+  };
+  auto into_block = [&](int n) {  // bytes from the thread's row of a block's first 64 keys to its row of the step's
+    return (uint64_t)(uint32_t)((step + n) * kTileKeys & in_block) * token_bytes;
+  };
+  // Loads past the last step are sent out like the others (the table's columns and the ids are cut, so that they read a block of
+  // the pool): a condition around them would have the registers of loads in flight copied, and so waited for.
+  auto issue_k = [&](int n) {
+    const uint64_t more = into_block(n);
 #pragma unroll
     for (int x = 0; x < T::kPasses; ++x) {
-      const int key = st * kTileKeys + x * T::kRowsPerPass + load_row;
-      ids[x] = (int32_t)min((uint32_t)table[min(key >> p.b.block_shift, last_col)], (uint32_t)p.b.max_block_id);
+      vid[x] = (int32_t)min((uint32_t)kid[x], (uint32_t)p.b.max_block_id);
+      kreg[x] = *reinterpret_cast<const u32x4 *>(k_row[x] + ((uint64_t)(uint32_t)vid[x] * block_bytes + more));
     }
+#pragma unroll
+    for (int x = 0; x < T::kPasses; ++x) kid[x] = fetch_id(n + 1, x);
   };
-  auto issue = [&](int st) {
-    if (!loads) return;
+  auto issue_v = [&](int n) {  // before issue_k(n + 1)
+    const uint64_t more = into_block(n);
+#pragma unroll
+    for (int x = 0; x < T::kPasses; ++x)
+      vreg[x] = *reinterpret_cast<const u32x4 *>(v_row[x] + ((uint64_t)(uint32_t)vid[x] * block_bytes + more));
+  };
+  auto write_k = [&](int n) {
+    char *kb = lds + (n & 1) * T::kBufferBytes;
 #pragma unroll
     for (int x = 0; x < T::kPasses; ++x) {
-      const int key = st * kTileKeys + x * T::kRowsPerPass + load_row;
-      const int64_t off = (int64_t)ids[x] * p.a.kv_block_bytes + (int64_t)kvh * p.a.kv_head_bytes +
-                          (int64_t)(key & in_block) * p.a.kv_token_bytes + piece * 16;
-      kreg[x] = *reinterpret_cast<const u32x4 *>(p.a.key_cache + off);
-      vreg[x] = *reinterpret_cast<const u32x4 *>(p.a.value_cache + off);
+      const int key = x * T::kRowsPerPass + load_row;
+      if constexpr (KV8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          u32x4 w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = fp8_adjacent_pair<KVF, F16>(kreg[x][2 * h + (k >> 1)], k & 1);
+          if (loads) *reinterpret_cast<u32x4 *>(kb + T::k_at(key, 2 * piece + h)) = w;
+        }
+      } else {
+        if (loads) *reinterpret_cast<u32x4 *>(kb + T::k_at(key, piece)) = kreg[x];
+      }
     }
   };
-  auto write = [&](int st, int buf) {
-    if (!loads) return;
-    char *kb = lds + buf * 2 * T::kBufferBytes, *vb = kb + T::kBufferBytes;
+  auto write_v = [&](int n) {
+    char *vb = lds + (2 + (n & 1)) * T::kBufferBytes;
 #pragma unroll
     for (int x = 0; x < T::kPasses; ++x) {
       const int key = x * T::kRowsPerPass + load_row;
       u32x4 v = vreg[x];
-      if (st * kTileKeys + key >= q.ctx) v = u32x4{0u, 0u, 0u, 0u};  // what lies there may be NaN
+      if ((step + n) * kTileKeys + key >= q.ctx) v = u32x4{0u, 0u, 0u, 0u};  // what lies there may be NaN
       if constexpr (KV8) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          u32x4 kw, vw;
+          u32x4 w;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            kw[w] = fp8_adjacent_pair<KVF, F16>(kreg[x][2 * h + (w >> 1)], w & 1);
-            vw[w] = fp8_adjacent_pair<KVF, F16>(v[2 * h + (w >> 1)], w & 1);
-          }
-          *reinterpret_cast<u32x4 *>(kb + T::k_at(key, 2 * piece + h)) = kw;
-          *reinterpret_cast<u32x4 *>(vb + T::v_at(key, 2 * piece + h)) = vw;
+          for (int k = 0; k < 4; ++k) w[k] = fp8_adjacent_pair<KVF, F16>(v[2 * h + (k >> 1)], k & 1);
+          if (loads) *reinterpret_cast<u32x4 *>(vb + T::v_at(key, 2 * piece + h)) = w;
         }
       } else {
-        *reinterpret_cast<u32x4 *>(kb + T::k_at(key, piece)) = kreg[x];
-        *reinterpret_cast<u32x4 *>(vb + T::v_at(key, piece)) = v;
+        if (loads) *reinterpret_cast<u32x4 *>(vb + T::v_at(key, piece)) = v;
       }
     }
   };
-  // scales of a step's four groups of 16 keys (a group lies within a block); groups past the context take 1
-  auto fetch_scales = [&](int st, float (&sk)[4], float (&sv)[4]) {
+  // Scales of a step's four groups of 16 keys (a group lies within a block): lanes 0 to 3 fetch those of K, 4 to 7 those of V, the
+  // block ids two steps ahead, the scales one step ahead, both left as they come until they are used.  Groups past the context
+  // take 1.
+  // Byte pools without scales of blocks go the same way, with scales of 1 (log2: 0).
+  constexpr bool blocks = KV8;
+  const bool scaled = KV8 && p.k_scales != nullptr;
+  const int group_key = 16 * (lane & 3);
+  const float *lane_scales = (lane & 4) ? p.v_scales : p.k_scales;
+  int32_t scale_id = 0;
+  float scale_raw = 1.f;
+  float sk[4] = {1.f, 1.f, 1.f, 1.f}, lv[4] = {0.f, 0.f, 0.f, 0.f};  // K scales and log2 of V scales of the step at hand
+  auto fetch_scale_ids = [&](int n) {
+    if (scaled) scale_id = table[min(((step + n) * kTileKeys + group_key) >> p.b.block_shift, last_col)];
+  };
+  auto fetch_scales = [&]() {  // of the step that scale_id is of
+    if (scaled) scale_raw = lane_scales[(int64_t)((uint64_t)min((uint32_t)scale_id, (uint32_t)p.b.max_block_id) * (uint32_t)p.scale_pitch) + kvh];
+  };
+  auto take_scales = [&](int n) {
+    if (!scaled) return;
+    const float s = (step + n) * kTileKeys + group_key < q.ctx ? scale_raw : 1.f;
+    const float log = p.block_scales ? __builtin_amdgcn_logf(s) : 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int key = st * kTileKeys + 16 * x;
-      const int32_t id = (int32_t)min((uint32_t)load_uniform_i32(table + min(key >> p.b.block_shift, last_col)), (uint32_t)p.b.max_block_id);
-      const int64_t idx = (int64_t)id * p.scale_pitch + kvh;
-      const float a = load_uniform_f32(p.k_scales + idx), b = load_uniform_f32(p.v_scales + idx);
-      sk[x] = key < q.ctx ? a : 1.f;
-      sv[x] = key < q.ctx ? b : 1.f;
+      sk[x] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), x));
+      lv[x] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, log), 4 + x));
     }
   };
 
-  if (step < step_end) {
-    float sk[4] = {1.f, 1.f, 1.f, 1.f}, sv[4] = {1.f, 1.f, 1.f, 1.f}, nk[4], nv[4];
-    const bool scaled = KV8 && p.k_scales != nullptr;
-    const bool blocks = KV8 && p.block_scales;
-    fetch_ids(step);
-    issue(step);
-    if (scaled) fetch_scales(step, sk, sv);
-    fetch_ids(step + 1);
-    write(step, 0);
-    if (step + 1 < step_end) issue(step + 1);
-    fetch_ids(step + 2);
-    __syncthreads();
-    const float c_all = p.score_scale_log2 * q_mul * (KV8 && !scaled ? p.tensor_scale : 1.f);
-
-    for (int buf = 0; step < step_end; ++step, buf ^= 1) {
-      if (scaled) fetch_scales(step + 1, nk, nv);
-      const int t0 = step * kTileKeys;
-      const bool sees = wave_live && t0 <= wave_hi && t0 + kTileKeys > wave_lo - p.window;  // the same for the wavefront
-      if (sees) {
-        const char *kb = lds + buf * 2 * T::kBufferBytes, *vb = kb + T::kBufferBytes;
-        f32x16 x[2];
+  // ---- the two phases of a step ----
+  const float c_all = p.score_scale_log2 * q_mul * (KV8 && !scaled ? p.tensor_scale : 1.f);
+  f32x16 x[2];   // scores of the step that softmax comes to next
+  u32x4 pb[4];   // weights of the step before it, as the B operands of V^T P^T
+  // the steps of which this wavefront sees anything: see_lo .. see_hi - 1 (the same for all its lanes)
+  const int see_lo = wave_live ? max(0, (wave_lo - p.window) / kTileKeys - step) : steps;
+  const int see_hi = wave_live && wave_hi >= 0 ? min(steps, wave_hi / kTileKeys + 1 - step) : 0;
+  // Where this lane reads K (16-byte piece of key `col`) and V (8 bytes of key 4 half + i / 4) within a buffer; the swizzles are
+  // exclusive-ors, so a k-step or d-tile is one more of them and keys further on are an offset (see k_at, v_at).
+  const int i16 = lane & 15;
+  const int k_base = T::k_at(col, map * (D / MAPS / 8) + half);
+  const int v_base = T::v_at(4 * half + (i16 >> 2), ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1)) + (i16 & 1) * 8;
+  // The matrix phase as a line of products, each with one A operand from LDS: the scores of a step (k-steps of its two halves of 32
+  // keys in turn), then the values of the step before (d-tiles of its four groups of 16 keys).  kAhead operands are on
+  // their way at any time; the order is held with scheduling barriers, since left to itself the compiler reads an operand right
+  // in front of the product that waits for it.
+  constexpr int kScoreOps = 2 * KS, kValueOps = 4 * DT, kAhead = 6;
+  auto operand = [&](int op, const char *kb, const char *vb) {
+    if (op < kScoreOps) return *reinterpret_cast<const u32x4 *>(kb + (k_base ^ ((op >> 1) << 5)) + (op & 1) * 32 * 2 * D);
+    const int k = (op - kScoreOps) / DT, dt = (op - kScoreOps) % DT;
+    const char *at = vb + (v_base ^ (dt << 6)) + k * 16 * 2 * D;
+    const u32x2 a0 = lds_read_transposed(at), a1 = lds_read_transposed(at + 8 * 2 * D);
+    return u32x4{a0[0], a0[1], a1[0], a1[1]};
+  };
+  auto product = [&](int op, u32x4 a) {
+    if (op < kScoreOps) {
+      const int c = op >> 1, t = op & 1;
+      if (c == 0) {
+        f32x16 zero;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[t][e] = 0.f;
-#pragma unroll
-        for (int c = 0; c < KS; ++c)
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const u32x4 a = *reinterpret_cast<const u32x4 *>(kb + T::k_at(t * 32 + col, map * (D / MAPS / 8) + 2 * c + half));
-            x[t] = mfma_32x32x16<OT>(a, qv[c], x[t]);
-          }
-
-        // register (t, e) holds key t0 + 32 t + 8 (e / 4) + 4 half + e % 4; group 2 t + e / 8 of 16 keys
-        float cc[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) cc[k] = KV8 ? c_all * sk[k] : c_all;
-        if (p.mask_flags) {  // soft-capping, distance penalties: scores in base-2 units from here on
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float s = x[t][e] * cc[2 * t + (e >> 3)];
-              if (p.mask_flags & kMaskSoftcap) s = soft_capped(s, p.softcap);
-              s += slope * (float)(t0 + 32 * t + 8 * (e >> 2) + 4 * half + (e & 3) - pos);
-              x[t][e] = s;
-            }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) cc[k] = 1.f;
-        }
-        if (t0 + kTileKeys - 1 > wave_lo || t0 < wave_hi - p.window) {
-          const int hi = pos - t0 - 4 * half, lo = hi - p.window;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int key = 32 * t + 8 * (e >> 2) + (e & 3);
-              if (key > hi || key < lo) x[t][e] = -INFINITY;  // select: the pool may hold NaN there
-            }
-        }
-        float gm[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int t = k >> 1, e = (k & 1) * 8;
-          gm[k] = fmaxf(fmaxf(fmaxf(x[t][e], x[t][e + 1]), fmaxf(x[t][e + 2], x[t][e + 3])),
-                        fmaxf(fmaxf(x[t][e + 4], x[t][e + 5]), fmaxf(x[t][e + 6], x[t][e + 7]))) * cc[k];
-        }
-        mt = fmaxf(mt, halves_max(fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]))));
-        if (__any(mt - m > kRefresh)) {
-          const float to = mt - kHeadroom;
-          const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - to);
-          l *= alpha;
-          if (!blocks) {
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
-          }
-          m = to;
-        }
-        const float sub = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            x[t][e] = fast_exp2(__builtin_fmaf(x[t][e], cc[2 * t + (e >> 3)], -sub));
-            l += x[t][e];
-          }
-        float f[4];
-        if (blocks) {
-          float lv[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) lv[k] = __builtin_amdgcn_logf(sv[k]);
-          mvt = fmaxf(mvt, halves_max(fmaxf(fmaxf(gm[0] + lv[0], gm[1] + lv[1]), fmaxf(gm[2] + lv[2], gm[3] + lv[3]))));
-          if (__any(mvt - mv > kRefresh)) {
-            const float to = mvt - kHeadroom;
-            const float alpha = mv == -INFINITY ? 0.f : fast_exp2(mv - to);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
-            mv = to;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) f[k] = mv == -INFINITY ? 0.f : fast_exp2(fminf(sub + lv[k] - mv, 126.0f));
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int t = k >> 1, e = (k & 1) * 8;
-          u32x4 pb;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            float lo = x[t][e + 2 * w], hi = x[t][e + 2 * w + 1];
-            if (blocks) {
-              lo *= f[k];
-              hi *= f[k];
-            }
-            pb[w] = pack2<OT>(lo, hi);
-          }
-          const int i = lane & 15, key = 16 * k + 4 * half + (i >> 2);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const int c16 = dt * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);  // 16-byte piece; its upper 8 bytes for odd i
-            const u32x2 a0 = lds_read_transposed(vb + T::v_at(key, c16) + (i & 1) * 8);
-            const u32x2 a1 = lds_read_transposed(vb + T::v_at(key + 8, c16) + (i & 1) * 8);
-            acc[dt] = mfma_32x32x16<OT>(u32x4{a0[0], a0[1], a1[0], a1[1]}, pb, acc[dt]);
-          }
-        }
+        for (int e = 0; e < 16; ++e) zero[e] = 0.f;
+        x[t] = mfma_32x32x16<OT>(a, qv[c], zero);
+      } else {
+        x[t] = mfma_32x32x16<OT>(a, qv[c], x[t]);
       }
-      if (step + 1 < step_end) {
-        write(step + 1, buf ^ 1);
-        if (step + 2 < step_end) issue(step + 2);
-        fetch_ids(step + 3);
-      }
-      if (scaled) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          sk[k] = nk[k];
-          sv[k] = nv[k];
-        }
-      }
-      __syncthreads();
+    } else {
+      const int k = (op - kScoreOps) / DT, dt = (op - kScoreOps) % DT;
+      acc[dt] = mfma_32x32x16<OT>(a, pb[k], acc[dt]);
     }
+  };
+  // scores of step n + 1 and / or values of step n
+  auto matrix_phase = [&](int n, auto with_scores, auto with_values) {
+    constexpr int kFirst = decltype(with_scores)::value ? 0 : kScoreOps;
+    constexpr int kLast = decltype(with_values)::value ? kScoreOps + kValueOps : kScoreOps;
+    const char *kb = lds + ((n + 1) & 1) * T::kBufferBytes, *vb = lds + (2 + (n & 1)) * T::kBufferBytes;
+    u32x4 a[kAhead];
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int op = kFirst; op < kFirst + kAhead && op < kLast; ++op) a[(op - kFirst) % kAhead] = operand(op, kb, vb);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int op = kFirst; op < kLast; ++op) {
+      product(op, a[(op - kFirst) % kAhead]);
+      if (op + kAhead < kLast) a[(op - kFirst) % kAhead] = operand(op + kAhead, kb, vb);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto softmax = [&](int n) {
+    const int t0 = (step + n) * kTileKeys;
+    // register (t, e) holds key t0 + 32 t + 8 (e / 4) + 4 half + e % 4; group 2 t + e / 8 of 16 keys
+    float cc[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) cc[k] = KV8 ? c_all * sk[k] : c_all;
+    if constexpr (EXT) {  // soft-capping, distance penalties: scores in base-2 units from here on
+      const bool capped = p.mask_flags & kMaskSoftcap;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[t][e] *= cc[2 * t + (e >> 3)];
+      if (capped) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[t][e] = soft_capped(x[t][e], p.softcap);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[t][e] += slope * (float)(t0 + 32 * t + 8 * (e >> 2) + 4 * half + (e & 3) - pos);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) cc[k] = 1.f;
+    }
+    if (t0 + kTileKeys - 1 > wave_lo || t0 < wave_hi - p.window) {
+      const int hi = pos - t0 - 4 * half, lo = hi - p.window;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = 32 * t + 8 * (e >> 2) + (e & 3);
+          if (key > hi || key < lo) x[t][e] = -INFINITY;  // select: the pool may hold NaN there
+        }
+    }
+    float gm[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int t = k >> 1, e = (k & 1) * 8;
+      gm[k] = max3(max3(max3(x[t][e], x[t][e + 1], x[t][e + 2]), x[t][e + 3], x[t][e + 4]), x[t][e + 5], x[t][e + 6]);
+      gm[k] = max3(gm[k], x[t][e + 7], x[t][e + 7]);
+      if constexpr (KV8) gm[k] *= cc[k];
+    }
+    float top = halves_max(max3(max3(gm[0], gm[1], gm[2]), gm[3], gm[3]));
+    if constexpr (!KV8) top *= cc[0];
+    mt = fmaxf(mt, top);
+    if (__builtin_expect(__any(mt - m > kRefresh), 0)) {
+      const float to = mt - kHeadroom;
+      const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - to);
+      l *= alpha;
+      if constexpr (!blocks) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+      }
+      m = to;
+    }
+    const float sub = m == -INFINITY ? 0.f : m;
+    if constexpr (blocks) {
+      // weights 2^(score + log2(V scale) - mv); the sum takes each group's back to scores: times 2^(mv - log2(V scale) - m)
+      mvt = fmaxf(mvt, halves_max(fmaxf(fmaxf(gm[0] + lv[0], gm[1] + lv[1]), fmaxf(gm[2] + lv[2], gm[3] + lv[3]))));
+      if (__builtin_expect(__any(mvt - mv > kRefresh), 0)) {
+        const float to = mvt - kHeadroom;
+        const float alpha = mv == -INFINITY ? 0.f : fast_exp2(mv - to);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+        mv = to;
+      }
+      const float sub_v = mv == -INFINITY ? 0.f : mv;
+      const float least = fminf(fminf(lv[0], lv[1]), fminf(lv[2], lv[3]));
+      // A block whose V is smaller than others' by 2^80 and more (zeros, above all) would have its weights vanish, and its
+      // probabilities with them: those are summed for themselves then.
+      const bool apart = __any(sub_v - sub - least > 80.0f);
+      if (__builtin_expect(apart, 0)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) l += fast_exp2(__builtin_fmaf(x[k >> 1][(k & 1) * 8 + e], cc[k], -sub));
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float sum = 0.f;
+        const float from = lv[k] - sub_v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int at = (k & 1) * 8 + e;
+          x[k >> 1][at] = fast_exp2(__builtin_fmaf(x[k >> 1][at], cc[k], from));
+          sum += x[k >> 1][at];
+        }
+        if (!apart) l = __builtin_fmaf(sum, fast_exp2(-from - sub), l);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int at = (k & 1) * 8 + e;
+          x[k >> 1][at] = fast_exp2(__builtin_fmaf(x[k >> 1][at], cc[k], -sub));
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) pb[k][w] = pack2<OT>(x[k >> 1][(k & 1) * 8 + 2 * w], x[k >> 1][(k & 1) * 8 + 2 * w + 1]);
+    if constexpr (!blocks) {  // the sum of the weights as they are rounded: 16 instructions for 32 of them
+      float part[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) part[w & 1] = add_pair<OT>(pb[k][w], part[w & 1]);
+      l += part[0] + part[1];
+    }
+  };
+  // Everything this work-group wrote to LDS is there, and nobody goes on before everybody is here.
+  auto meet = [&]() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  };
+
+  // ---- steps ----
+  // Matrix phase of step n: scores of n + 1 and values of n.  Vector phase: softmax of n + 1, and the thread's share of K of
+  // n + 2 and V of n + 1 goes to LDS (what the next matrix phase reads), the loads of the step after that are sent out.
+  // With eight wavefronts every SIMD has two: the second four run one phase behind the first, so that one is in its matrix
+  // phase while the other is in its vector phase; their shares of K and V are due one step earlier.
+  if (steps > 0) {
+    const int late = NW == 8 ? wave >> 2 : 0;
+#pragma unroll
+    for (int x = 0; x < T::kPasses; ++x) kid[x] = fetch_id(0, x);
+    issue_k(0);
+    fetch_scale_ids(0);
+    fetch_scales();
+    fetch_scale_ids(1);
+    write_k(0);
+    issue_v(0);  // (V, then K, on every way into the loop: its waits count the loads behind the one that is waited for)
+    issue_k(1);
+    if (late) {
+      write_v(0);
+      write_k(1);
+      issue_v(1);
+      issue_k(2);
+    }
+    meet();
+    if (NW == 8 && late) meet();
+    // Between the matrix phase of step n and the next one.
+    auto vector_phase = [&](int n, auto with_softmax) {
+      if (NW == 8) meet();
+      take_scales(n + 1);
+      fetch_scales();
+      fetch_scale_ids(n + 3);
+      if constexpr (decltype(with_softmax)::value) softmax(n + 1);
+      write_v(n + 1 + late);
+      write_k(n + 2 + late);
+      issue_v(n + 2 + late);
+      issue_k(n + 3 + late);
+      meet();
+    };
+    // Loops of their own for the steps that the wavefront has no part in, so that accumulators stay where they are.
+    int n = -1;
+    const int from = min(see_lo, steps), to = see_hi;
+    for (; n + 1 < (from < to ? from : steps); ++n) vector_phase(n, std::false_type{});
+    if (from < to) {
+      matrix_phase(n, std::true_type{}, std::false_type{});
+      vector_phase(n, std::true_type{});
+      for (++n; n + 1 < to; ++n) {
+        matrix_phase(n, std::true_type{}, std::true_type{});
+        vector_phase(n, std::true_type{});
+      }
+      matrix_phase(n, std::false_type{}, std::true_type{});
+      for (; n + 1 < steps; ++n) vector_phase(n, std::false_type{});
+    }
+    if (NW == 8 && !late) meet();
   }
 
   // ---- results: element (dt, e) of a lane is d = 32 dt + 8 (e / 4) + 4 half + e % 4 of its row ----
   l = halves_sum(l);
   {
     const float to = mt == -INFINITY ? 0.f : mt;
-    const float from = KV8 && p.block_scales ? mv : m;
+    const float from = KV8 ? mv : m;
     const float v_mul = !KV8 || p.block_scales ? 1.f : p.v_scales ? load_uniform_f32(p.v_scales + kvh) : p.tensor_scale;
     const float f = (from == -INFINITY ? 0.f : fast_exp2(from - to)) * v_mul;
     l *= m == -INFINITY ? 0.f : fast_exp2(m - to);
@@ -399,10 +552,11 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
               u32x2{pack_out(p, acc[dt][4 * k] * inv, acc[dt][4 * k + 1] * inv), pack_out(p, acc[dt][4 * k + 2] * inv, acc[dt][4 * k + 3] * inv)};
     }
   } else {
-    // second maps -> first maps, through LDS (a lane's values at [value][lane] of its strip); the loop's last barrier is behind
+    // second maps -> first maps, through LDS (a lane's values at [value][lane] of its strip)
     constexpr int kValues = DT * 16;
     static_assert(kValues * 64 * 4 * (NW / 2) <= T::kLdsBytes, "the second maps' results fit the buffers");
     float *through = reinterpret_cast<float *>(lds) + strip * kValues * 64 + lane;
+    __syncthreads();  // nobody reads V any more
     if (map == 1) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
