@@ -76,12 +76,21 @@ inline RaggedPlan ragged_plan(const fa_ragged_shape &s, int maps, int cus) {
   if (r.tiles) {
     // 8 wavefronts halve what K and V cost per row; sequences that cannot fill them take 4
     r.wavefronts = most * G * maps <= 128 ? 4 : 8;
+#ifdef FORCE_NW
+    r.wavefronts = FORCE_NW;
+#endif
+#ifdef FORCE_SPLITS
+    const int fs = FORCE_SPLITS;
+#else
+    const int fs = 0;
+#endif
     r.tile_rows = r.wavefronts * 32 / maps;
     const int64_t each = (most * G + r.tile_rows - 1) / r.tile_rows;
     r.tile_bound = equal ? S * each : std::min(S * each, T * G / r.tile_rows + S);
     const int64_t resident = (int64_t)cus * (r.wavefronts == 4 ? 2 : 1);
     const int64_t steps = (keys + kTileKeys - 1) / kTileKeys;
     r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / std::max<int64_t>(1, r.tile_bound * Hk), steps / 8, 64}));
+    if (fs) r.splits = fs;
     if (r.splits > 1) {
       const int64_t slots = r.tile_bound * Hk * r.splits, rows = r.tile_rows * maps;
       r.tile_o = take(slots * rows * D * 4);

@@ -84,8 +84,8 @@ struct RaggedTile {
     else return key * 128 + ((c ^ ((key >> 1) & 7)) * 16);
   }
   static __device__ __forceinline__ int v_at(int key, int c) {
-    if constexpr (D == 128) return key * 256 + (((c >> 2) ^ (key & 3)) * 64) + (c & 3) * 16;
-    else return key * 128 + (((c >> 2) ^ ((key >> 1) & 1)) * 64) + (c & 3) * 16;
+    if constexpr (D == 128) return key * 256 + (((c >> 2) ^ (key & 3)) * 64) + (((c & 3) ^ (key & 1)) * 16);
+    else return key * 128 + (((c >> 2) ^ ((key >> 1) & 1)) * 64) + (((c & 3) ^ ((key >> 1) & 1)) * 16);
   }
 };
 
@@ -214,44 +214,39 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
     for (int x = 0; x < T::kPasses; ++x)
       vreg[x] = *reinterpret_cast<const u32x4 *>(v_row[x] + ((uint64_t)(uint32_t)vid[x] * block_bytes + more));
   };
-  auto write_k = [&](int n) {
-    char *kb = lds + (n & 1) * T::kBufferBytes;
+  // Piece `w` of what a thread has loaded of a step, into its buffer: a 16-byte piece of LDS each.
+  constexpr int kPieces = T::kPasses * (KV8 ? 2 : 1);
+  auto lds_piece = [&](const u32x4 &reg, int w) {
+    if constexpr (KV8) {
+      u32x4 o;
 #pragma unroll
-    for (int x = 0; x < T::kPasses; ++x) {
-      const int key = x * T::kRowsPerPass + load_row;
-      if constexpr (KV8) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          u32x4 w;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = fp8_adjacent_pair<KVF, F16>(kreg[x][2 * h + (k >> 1)], k & 1);
-          if (loads) *reinterpret_cast<u32x4 *>(kb + T::k_at(key, 2 * piece + h)) = w;
-        }
-      } else {
-        if (loads) *reinterpret_cast<u32x4 *>(kb + T::k_at(key, piece)) = kreg[x];
-      }
+      for (int k = 0; k < 4; ++k) o[k] = fp8_adjacent_pair<KVF, F16>(reg[2 * (w & 1) + (k >> 1)], k & 1);
+      return o;
+    } else {
+      return reg;
     }
   };
-  auto write_v = [&](int n) {
-    char *vb = lds + (2 + (n & 1)) * T::kBufferBytes;
-#pragma unroll
-    for (int x = 0; x < T::kPasses; ++x) {
-      const int key = x * T::kRowsPerPass + load_row;
-      u32x4 v = vreg[x];
-      if ((step + n) * kTileKeys + key >= q.ctx) v = u32x4{0u, 0u, 0u, 0u};  // what lies there may be NaN
-      if constexpr (KV8) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          u32x4 w;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = fp8_adjacent_pair<KVF, F16>(v[2 * h + (k >> 1)], k & 1);
-          if (loads) *reinterpret_cast<u32x4 *>(vb + T::v_at(key, 2 * piece + h)) = w;
-        }
-      } else {
-        if (loads) *reinterpret_cast<u32x4 *>(vb + T::v_at(key, piece)) = v;
-      }
-    }
+  auto write_k = [&](int n, int w) {
+    const int pass = KV8 ? w >> 1 : w, key = pass * T::kRowsPerPass + load_row;
+    const u32x4 o = lds_piece(kreg[pass], w);
+    if (loads) *reinterpret_cast<u32x4 *>(lds + (n & 1) * T::kBufferBytes + T::k_at(key, KV8 ? 2 * piece + (w & 1) : piece)) = o;
   };
+  auto write_v = [&](int n, int w) {
+    const int pass = KV8 ? w >> 1 : w, key = pass * T::kRowsPerPass + load_row;
+    if ((step + n) * kTileKeys + key >= q.ctx) vreg[pass] = u32x4{0u, 0u, 0u, 0u};  // what lies there may be NaN
+    const u32x4 o = lds_piece(vreg[pass], w);
+    if (loads) *reinterpret_cast<u32x4 *>(lds + (2 + (n & 1)) * T::kBufferBytes + T::v_at(key, KV8 ? 2 * piece + (w & 1) : piece)) = o;
+  };
+  // What a wavefront does for the coming steps during the matrix phase of step n, in small parts that lie between its products:
+  // V of step n + 1 and K of n + 2 go to LDS, the loads of the step after are sent out.
+  constexpr int kStageParts = 2 * kPieces + 2;
+  auto stage = [&](int n, int part) {
+    if (part < kPieces) write_v(n + 1, part);
+    else if (part < 2 * kPieces) write_k(n + 2, part - kPieces);
+    else if (part == 2 * kPieces) issue_v(n + 2);
+    else if (part == 2 * kPieces + 1) issue_k(n + 3);
+  };
+
   // Scales of a step's four groups of 16 keys (a group lies within a block): lanes 0 to 3 fetch those of K, 4 to 7 those of V, the
   // block ids two steps ahead, the scales one step ahead, both left as they come until they are used.  Groups past the context
   // take 1.
@@ -259,19 +254,20 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   constexpr bool blocks = KV8;
   const bool scaled = KV8 && p.k_scales != nullptr;
   const int group_key = 16 * (lane & 3);
-  const float *lane_scales = (lane & 4) ? p.v_scales : p.k_scales;
+  // (pools without scales: anything that can be read, not looked at, so that every step has the same loads in flight)
+  const float *lane_scales = !scaled ? reinterpret_cast<const float *>(table) - kvh : (lane & 4) ? p.v_scales : p.k_scales;
   int32_t scale_id = 0;
   float scale_raw = 1.f;
   float sk[4] = {1.f, 1.f, 1.f, 1.f}, lv[4] = {0.f, 0.f, 0.f, 0.f};  // K scales and log2 of V scales of the step at hand
   auto fetch_scale_ids = [&](int n) {
-    if (scaled) scale_id = table[min(((step + n) * kTileKeys + group_key) >> p.b.block_shift, last_col)];
+    if constexpr (KV8) scale_id = table[(uint32_t)min(((step + n) * kTileKeys + group_key) >> p.b.block_shift, last_col)];
   };
   auto fetch_scales = [&]() {  // of the step that scale_id is of
-    if (scaled) scale_raw = lane_scales[(int64_t)((uint64_t)min((uint32_t)scale_id, (uint32_t)p.b.max_block_id) * (uint32_t)p.scale_pitch) + kvh];
+    if constexpr (KV8) scale_raw = lane_scales[(int64_t)((uint64_t)min((uint32_t)scale_id, (uint32_t)p.b.max_block_id) * (uint32_t)p.scale_pitch) + kvh];
   };
   auto take_scales = [&](int n) {
-    if (!scaled) return;
-    const float s = (step + n) * kTileKeys + group_key < q.ctx ? scale_raw : 1.f;
+    if constexpr (!KV8) return;
+    const float s = scaled && (step + n) * kTileKeys + group_key < q.ctx ? scale_raw : 1.f;
     const float log = p.block_scales ? __builtin_amdgcn_logf(s) : 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -321,22 +317,27 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
     }
   };
   // scores of step n + 1 and / or values of step n
-  auto matrix_phase = [&](int n, auto with_scores, auto with_values) {
+  auto matrix_phase = [&](int n, auto with_scores, auto with_values, bool with_stage) {
     constexpr int kFirst = decltype(with_scores)::value ? 0 : kScoreOps;
     constexpr int kLast = decltype(with_values)::value ? kScoreOps + kValueOps : kScoreOps;
     const char *kb = lds + ((n + 1) & 1) * T::kBufferBytes, *vb = lds + (2 + (n & 1)) * T::kBufferBytes;
     u32x4 a[kAhead];
-    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int op = kFirst; op < kFirst + kAhead && op < kLast; ++op) a[(op - kFirst) % kAhead] = operand(op, kb, vb);
     __builtin_amdgcn_sched_barrier(0);
+    constexpr int kEvery = kLast - kFirst >= 2 * kStageParts + 2 ? 2 : 1;  // products from one part of the staging to the next
 #pragma unroll
     for (int op = kFirst; op < kLast; ++op) {
-      product(op, a[(op - kFirst) % kAhead]);
-      if (op + kAhead < kLast) a[(op - kFirst) % kAhead] = operand(op + kAhead, kb, vb);
+      const int at = op - kFirst;
+      product(op, a[at % kAhead]);
+      if (op + kAhead < kLast) a[at % kAhead] = operand(op + kAhead, kb, vb);
+      if (with_stage && at % kEvery == 0) stage(n, at / kEvery);
       __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_s_setprio(0);
+    if (with_stage) {
+#pragma unroll
+      for (int part = (kLast - kFirst + kEvery - 1) / kEvery; part < kStageParts; ++part) stage(n, part);
+    }
   };
   auto softmax = [&](int n) {
     const int t0 = (step + n) * kTileKeys;
@@ -416,17 +417,20 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
 #pragma unroll
           for (int e = 0; e < 8; ++e) l += fast_exp2(__builtin_fmaf(x[k >> 1][(k & 1) * 8 + e], cc[k], -sub));
       }
+      float part[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float sum = 0.f;
         const float from = lv[k] - sub_v;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int at = (k & 1) * 8 + e;
           x[k >> 1][at] = fast_exp2(__builtin_fmaf(x[k >> 1][at], cc[k], from));
-          sum += x[k >> 1][at];
+          part[k] = e == 0 ? x[k >> 1][at] : part[k] + x[k >> 1][at];
         }
-        if (!apart) l = __builtin_fmaf(sum, fast_exp2(-from - sub), l);
+      }
+      if (!apart) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) l = __builtin_fmaf(part[k], fast_exp2(sub_v - lv[k] - sub), l);
       }
     } else {
 #pragma unroll
@@ -458,57 +462,58 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   };
 
   // ---- steps ----
-  // Matrix phase of step n: scores of n + 1 and values of n.  Vector phase: softmax of n + 1, and the thread's share of K of
-  // n + 2 and V of n + 1 goes to LDS (what the next matrix phase reads), the loads of the step after that are sent out.
-  // With eight wavefronts every SIMD has two: the second four run one phase behind the first, so that one is in its matrix
-  // phase while the other is in its vector phase; their shares of K and V are due one step earlier.
+  // Matrix phase of step n: scores of n + 1 and values of n, and between the products the thread's share of V of n + 1 and K of
+  // n + 2 goes to LDS (what the next matrix phase reads) and the loads of the step after that are sent out.  Vector phase: softmax
+  // of n + 1.  With eight wavefronts every SIMD has two: the second four run one phase behind the first, so that one is in its
+  // matrix phase while the other is in its vector phase.
   if (steps > 0) {
-    const int late = NW == 8 ? wave >> 2 : 0;
+    constexpr bool kTurns = NW == 8;
+    const int late = kTurns ? wave >> 2 : 0;
 #pragma unroll
     for (int x = 0; x < T::kPasses; ++x) kid[x] = fetch_id(0, x);
     issue_k(0);
     fetch_scale_ids(0);
     fetch_scales();
     fetch_scale_ids(1);
-    write_k(0);
-    issue_v(0);  // (V, then K, on every way into the loop: its waits count the loads behind the one that is waited for)
+#pragma unroll
+    for (int w = 0; w < kPieces; ++w) write_k(0, w);
+    issue_v(0);
     issue_k(1);
-    if (late) {
-      write_v(0);
-      write_k(1);
-      issue_v(1);
-      issue_k(2);
-    }
     meet();
-    if (NW == 8 && late) meet();
-    // Between the matrix phase of step n and the next one.
+    if (kTurns && late) meet();
     auto vector_phase = [&](int n, auto with_softmax) {
-      if (NW == 8) meet();
+      if (kTurns) meet();
       take_scales(n + 1);
       fetch_scales();
       fetch_scale_ids(n + 3);
       if constexpr (decltype(with_softmax)::value) softmax(n + 1);
-      write_v(n + 1 + late);
-      write_k(n + 2 + late);
-      issue_v(n + 2 + late);
-      issue_k(n + 3 + late);
       meet();
+    };
+    auto idle_step = [&](int n) {
+#pragma unroll
+      for (int part = 0; part < kStageParts; ++part) stage(n, part);
+      vector_phase(n, std::false_type{});
     };
     // Loops of their own for the steps that the wavefront has no part in, so that accumulators stay where they are.
     int n = -1;
     const int from = min(see_lo, steps), to = see_hi;
-    for (; n + 1 < (from < to ? from : steps); ++n) vector_phase(n, std::false_type{});
+    for (; n + 1 < (from < to ? from : steps); ++n) idle_step(n);
     if (from < to) {
-      matrix_phase(n, std::true_type{}, std::false_type{});
+      matrix_phase(n, std::true_type{}, std::false_type{}, true);
       vector_phase(n, std::true_type{});
       for (++n; n + 1 < to; ++n) {
-        matrix_phase(n, std::true_type{}, std::true_type{});
+        matrix_phase(n, std::true_type{}, std::true_type{}, true);
         vector_phase(n, std::true_type{});
       }
-      matrix_phase(n, std::false_type{}, std::true_type{});
-      for (; n + 1 < steps; ++n) vector_phase(n, std::false_type{});
+      if (n + 1 < steps) {
+        matrix_phase(n, std::false_type{}, std::true_type{}, true);
+        vector_phase(n, std::false_type{});
+        for (++n; n + 1 < steps; ++n) idle_step(n);
+      } else {
+        matrix_phase(n, std::false_type{}, std::true_type{}, false);
+      }
     }
-    if (NW == 8 && !late) meet();
+    if (kTurns && !late) meet();
   }
 
   // ---- results: element (dt, e) of a lane is d = 32 dt + 8 (e / 4) + 4 half + e % 4 of its row ----
