@@ -16,7 +16,7 @@ struct RaggedPlan {
   int wavefronts;         // of a work-group of the tile form
   int tile_rows;          // rows of its tiles
   int64_t tile_bound;     // tiles per kv head, at most
-  int splits;
+  int tile_groups;        // work-groups that share all tiles; 0: a work-group for each tile
   int row_groups;
   int64_t row_o, row_ml, row_items, tile_o, tile_ml, bytes;  // offsets into the workspace, and its size
 };
@@ -46,6 +46,9 @@ inline fa_status check_ragged_shape(const fa_ragged_shape *s, int maps) {
   if ((int64_t)s->num_seqs * s->num_kv_heads * (keys / kRowUnit + 2) > 0x7fffffffLL ||
       ((int64_t)s->num_tokens + s->num_seqs) * s->num_heads > 0x7fffffffLL)
     return fail(FA_ERR_BAD_SHAPE, "num_seqs x num_kv_heads x keys or num_tokens x num_heads is too large");
+  // the line of tiles is as long as the sum of their keys, and cut at products with the work-groups' numbers
+  if (((int64_t)s->num_tokens * s->num_heads / 32 + s->num_seqs * (int64_t)s->num_kv_heads) * (keys + 1024) > (1LL << 41))
+    return fail(FA_ERR_BAD_SHAPE, "num_tokens x num_heads x keys is too large");
   return FA_OK;
 }
 
@@ -79,22 +82,17 @@ inline RaggedPlan ragged_plan(const fa_ragged_shape &s, int maps, int cus) {
 #ifdef FORCE_NW
     r.wavefronts = FORCE_NW;
 #endif
-#ifdef FORCE_SPLITS
-    const int fs = FORCE_SPLITS;
-#else
-    const int fs = 0;
-#endif
     r.tile_rows = r.wavefronts * 32 / maps;
     const int64_t each = (most * G + r.tile_rows - 1) / r.tile_rows;
     r.tile_bound = equal ? S * each : std::min(S * each, T * G / r.tile_rows + S);
     const int64_t resident = (int64_t)cus * (r.wavefronts == 4 ? 2 : 1);
-    const int64_t steps = (keys + kTileKeys - 1) / kTileKeys;
-    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / std::max<int64_t>(1, r.tile_bound * Hk), steps / 8, 64}));
-    if (fs) r.splits = fs;
-    if (r.splits > 1) {
-      const int64_t slots = r.tile_bound * Hk * r.splits, rows = r.tile_rows * maps;
-      r.tile_o = take(slots * rows * D * 4);
-      r.tile_ml = take(slots * rows * 2 * 4);
+#ifndef FORCE_LINE
+#define FORCE_LINE 2
+#endif
+    if (r.tile_bound * Hk < FORCE_LINE * resident) {
+      r.tile_groups = (int)std::max<int64_t>(8, resident / 8 * 8);  // (an eighth of the shares for each XCC)
+      r.tile_o = take(2 * (int64_t)r.tile_groups * r.wavefronts * D * 32 * 4);
+      r.tile_ml = take(2 * (int64_t)r.tile_groups * r.wavefronts * 128 * 4);
     }
   }
   r.bytes = at;
@@ -110,11 +108,14 @@ inline fa_status launch_ragged_kernels(const RaggedParams &p, const RaggedPlan &
   };
   fa_status st = FA_OK;
   if (plan.tiles) {
-    const dim3 grid((unsigned)(plan.tile_bound * Hk), (unsigned)plan.splits);
+    const dim3 grid((unsigned)(plan.tile_groups > 0 ? plan.tile_groups : plan.tile_bound * Hk));
+    const auto with_line = [&](auto ext, auto line) {
+      constexpr bool kExt = decltype(ext)::value, kLine = decltype(line)::value;
+      return plan.wavefronts == 8 ? timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 8, kExt, kLine>, grid, dim3(512), 0, p)
+                                  : timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 4, kExt, kLine>, grid, dim3(256), 0, p);
+    };
     const auto launch = [&](auto ext) {
-      constexpr bool kExt = decltype(ext)::value;
-      return plan.wavefronts == 8 ? timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 8, kExt>, grid, dim3(512), 0, p)
-                                  : timer.launch(ragged_tile_kernel<D, OT, KVF, MAPS, 4, kExt>, grid, dim3(256), 0, p);
+      return plan.tile_groups > 0 ? with_line(ext, std::true_type{}) : with_line(ext, std::false_type{});
     };
     if constexpr (MAPS == 1) {
       FA_HIP_CHECK(p.mask_flags ? launch(std::true_type{}) : launch(std::false_type{}));
@@ -122,12 +123,12 @@ inline fa_status launch_ragged_kernels(const RaggedParams &p, const RaggedPlan &
       FA_HIP_CHECK(launch(std::false_type{}));
     }
     if ((st = timed()) != FA_OK) return st;
-    if (plan.splits > 1) {
-      const dim3 merge((unsigned)(plan.tile_bound * Hk), (unsigned)(plan.tile_rows / 16));
+    if (plan.tile_groups > 1) {
+      const dim3 merge((unsigned)(plan.tile_groups - 1));
       if (plan.wavefronts == 8)
-        FA_HIP_CHECK(timer.launch(ragged_tile_merge_kernel<D, MAPS, 256 / MAPS>, merge, dim3(256), 0, p));
+        FA_HIP_CHECK(timer.launch(ragged_tile_merge_kernel<D, MAPS, 8>, merge, dim3(512), 0, p));
       else
-        FA_HIP_CHECK(timer.launch(ragged_tile_merge_kernel<D, MAPS, 128 / MAPS>, merge, dim3(256), 0, p));
+        FA_HIP_CHECK(timer.launch(ragged_tile_merge_kernel<D, MAPS, 4>, merge, dim3(256), 0, p));
       if ((st = timed()) != FA_OK) return st;
     }
   }
@@ -253,7 +254,7 @@ inline fa_status launch_ragged_attention(void *out, const void *query, const voi
   p.row_o = reinterpret_cast<float *>(space + plan.row_o);
   p.row_ml = reinterpret_cast<float *>(space + plan.row_ml);
   p.row_items = reinterpret_cast<int2 *>(space + plan.row_items);
-  p.splits = plan.splits;
+  p.tile_groups = plan.tile_groups;
   p.tile_o = reinterpret_cast<float *>(space + plan.tile_o);
   p.tile_ml = reinterpret_cast<float *>(space + plan.tile_ml);
 

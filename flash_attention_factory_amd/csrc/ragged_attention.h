@@ -43,9 +43,9 @@ struct RaggedParams {
   float *row_ml;                // [slot][2][16]: maxima (base-2 units), sums
   int2 *row_items;              // [seq * kv heads + kv head]: first and last work-group of the item
   // tile form
-  int32_t splits;               // pieces that the keys of a tile of rows are cut into
-  float *tile_o;                // [(tile * kv heads + kv head) * splits + piece][row][D]
-  float *tile_ml;               // [...][2][row]
+  int32_t tile_groups;          // > 0: work-groups that share the line of tiles; 0: a work-group for each tile
+  float *tile_o;                // [2 * work-group + (0: its first piece, 1: a later one)]: registers of its wavefronts
+  float *tile_ml;               // [...][wavefront][2][lane]: maxima, sums
 };
 
 constexpr int kRowColumns = 16;     // rows of the rows form: MFMA columns of a wavefront

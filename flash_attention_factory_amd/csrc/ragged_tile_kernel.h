@@ -89,7 +89,214 @@ struct RaggedTile {
   }
 };
 
-template <int D, typename OT, int KVF, int MAPS, int NW, bool EXT>
+// ---- the line of tiles ----
+// All tiles of the batch (sequence, kv head, tile of rows) laid end to end, each as long as it costs: about its keys, and
+// kTileStart for what a tile costs apart from them.  Within a sequence the cost grows by the same amount from tile to
+// tile (the causal rule), so sums and places have closed forms.  Work-group g takes the part from total * g / groups
+// to total * (g + 1) / groups: equal shares, whatever the lengths are.  A cut within a tile becomes a cut between two steps.
+// Measured against one work-group per tile, the longest of a sequence first (the card has 256 compute units): see the launcher.
+constexpr int kTileStart = 3 * kTileKeys;
+constexpr int kLeastShare = 4 * kTileKeys;  // no shares smaller than that
+
+struct TileCosts {
+  int tiles;      // of one kv head
+  int64_t first;  // cost of the first tile
+  int64_t more;   // by which each costs more than the one before it
+  __device__ __forceinline__ int64_t upto(int64_t t) const { return first * t + more * (t * (t - 1) / 2); }
+  __device__ __forceinline__ int64_t of_head() const { return upto(tiles); }
+};
+template <int MAPS, int ROWS>
+__device__ __forceinline__ TileCosts tile_costs(const RaggedParams &p, RaggedSeq q) {
+  TileCosts c;
+  c.tiles = row_tiles<MAPS, ROWS>(p, q);
+  q = ragged_seq_cut(p, q);
+  const int tokens = ROWS / p.group + 1, all = max(q.ctx - q.n, 0);
+  const int most = min(p.window, kNoWindow - tokens) + tokens;  // keys that a tile can see
+  const int a = min(all + tokens, most), b = min(all + c.tiles * tokens, most);
+  c.first = a + kTileStart;
+  c.more = c.tiles > 1 ? (b - a) / (c.tiles - 1) : 0;
+  return c;
+}
+
+__device__ __forceinline__ int64_t wave_inclusive_scan64(int64_t v, int lane) {
+#pragma unroll
+  for (int step = 1; step < 64; step <<= 1) {
+    const int64_t other = __shfl_up(v, step);
+    if (lane >= step) v += other;
+  }
+  return v;
+}
+__device__ __forceinline__ int64_t readlane64(int64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)v >> 32), lane);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// A place on the line: the tile that lies there, and how far into it.
+struct TilePlace {
+  int seq, kvh, tile;
+  int64_t off;  // cost units from the tile's start
+};
+// n / d for n < 2^53, without the 64-bit division's two hundred instructions.
+__device__ __forceinline__ int64_t divide(int64_t n, int d) {
+  int64_t q = (int64_t)((double)n / (double)d);
+  if (q * d > n) --q;
+  if ((q + 1) * d <= n) ++q;
+  return q;
+}
+template <int MAPS, int ROWS>
+struct TileLine {
+  int64_t total;
+  int groups;
+  int64_t mine, upto;  // of the first 64 sequences: this lane's, and the sum up to it
+  __device__ __forceinline__ TileLine(const RaggedParams &p, int lane) {
+    mine = costs(p, lane);
+    upto = wave_inclusive_scan64(mine, lane);
+    total = readlane64(upto, 63);
+    if (p.b.num_seqs > 64) {
+      int64_t more = 0;
+      for (int s = 64 + lane; s < p.b.num_seqs; s += 64) more += costs(p, s);
+      total += readlane64(wave_inclusive_scan64(more, lane), 63);
+    }
+    groups = (int)min((int64_t)p.tile_groups, total / kLeastShare + (total > 0));
+  }
+  static __device__ __forceinline__ int64_t costs(const RaggedParams &p, int s) {  // of all kv heads of sequence s
+    return s < p.b.num_seqs ? tile_costs<MAPS, ROWS>(p, ragged_seq_of_lane(p.b, s)).of_head() * p.num_kv_heads : 0;
+  }
+  __device__ __forceinline__ int64_t cut(int g) const { return divide(total * g, groups); }
+  // `at` < total
+  __device__ __forceinline__ TilePlace find(const RaggedParams &p, int64_t at, int lane) const {
+    TilePlace r;
+    int64_t before = 0, of_lane = mine, sum = upto;
+    for (int base = 0;; base += 64) {
+      if (base > 0) {
+        of_lane = costs(p, base + lane);
+        sum = wave_inclusive_scan64(of_lane, lane);
+      }
+      const unsigned long long beyond = __ballot(before + sum > at);
+      if (beyond || base + 64 >= p.b.num_seqs) {
+        const int k = __builtin_ctzll(beyond | (1ull << 63));
+        r.seq = __builtin_amdgcn_readfirstlane(base + k);
+        before += readlane64(sum - of_lane, k);
+        break;
+      }
+      before += readlane64(sum, 63);
+    }
+    const TileCosts c = tile_costs<MAPS, ROWS>(p, ragged_seq_uniform(p.b, r.seq));
+    int64_t in = at - before;
+    const int64_t head = c.of_head();
+    int kvh = min((int)((float)in / (float)head), p.num_kv_heads - 1);
+    while (kvh > 0 && in < head * kvh) --kvh;
+    while (kvh + 1 < p.num_kv_heads && in >= head * (kvh + 1)) ++kvh;
+    in -= head * kvh;
+    // in >= first t + more t (t - 1) / 2: the root, then the whole number by comparison
+    const float b = (float)c.first - 0.5f * (float)c.more;
+    int t = c.more > 0 ? (int)((sqrtf(b * b + 2.0f * (float)c.more * (float)in) - b) / (float)c.more) : (int)((float)in / (float)c.first);
+    t = min(max(t, 0), c.tiles - 1);
+    while (t > 0 && in < c.upto(t)) --t;
+    while (t + 1 < c.tiles && in >= c.upto(t + 1)) ++t;
+    r.kvh = __builtin_amdgcn_readfirstlane(kvh);
+    r.tile = __builtin_amdgcn_readfirstlane(t);
+    r.off = in - c.upto(t);
+    return r;
+  }
+};
+
+// The steps of a tile: the first one, and how many (64 keys each).
+struct TileSteps {
+  int first, count;
+};
+template <int ROWS>
+__device__ __forceinline__ TileSteps tile_steps(const RaggedParams &p, const RaggedSeq &q, int tile) {
+  const int row0 = tile * ROWS, pos0 = q.ctx - q.n;
+  const int pos_lo = pos0 + row0 / p.group, pos_hi = pos0 + (min(row0 + ROWS, q.n * p.group) - 1) / p.group;
+  TileSteps s;
+  s.first = max(0, pos_lo - p.window) / kTileKeys;
+  s.count = pos_hi < 0 ? 0 : pos_hi / kTileKeys + 1 - s.first;
+  return s;
+}
+// Where a cut `off` into a tile of cost `cost` falls between its steps.
+__device__ __forceinline__ int cut_step(int64_t off, int64_t cost, int steps) {
+  return min((int)((float)off * (float)steps / (float)cost), steps);
+}
+
+// What the wavefronts of a work-group have of a tile's rows: lane (half, col) holds elements d = 32 dt + 8 k + 4 half + e of row
+// `strip * 32 + col` in acc[dt][4 k + e], against the maximum m with the sum l.  Normalises them, joins the maps, and stores the
+// rows by way of LDS, 16 bytes per lane and whole rows at a time: eight bytes at a time into 32 rows cost more than four steps do.
+// All wavefronts call it; LDS holds nothing else any more.
+template <int D, int MAPS, int NW>
+__device__ __forceinline__ void tile_finish(const RaggedParams &p, const RaggedSeq &q, int kvh, int row0, f32x16 (&acc)[D / 32], float l,
+                                            char *lds) {
+  constexpr int DT = D / 32, kRows = NW * 32 / MAPS;
+  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int map = MAPS == 2 ? wave / (NW / 2) : 0, strip = MAPS == 2 ? wave % (NW / 2) : wave;
+  const int all_rows = q.n * p.group, row = min(row0 + strip * 32 + col, all_rows - 1);
+  const int j = row / p.group, head = kvh * p.group + (row - j * p.group);
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] *= inv;
+  if constexpr (MAPS == 2) {  // second maps -> first maps (a lane's values at [value][lane] of its strip)
+    float *through = reinterpret_cast<float *>(lds) + strip * DT * 16 * 64 + lane;
+    if (map == 1) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) through[(dt * 16 + e) * 64] = acc[dt][e];
+    }
+    __syncthreads();
+    if (map == 1) return;
+    const float lambda = p.lambdas[head];
+    float square = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        acc[dt][e] -= lambda * through[(dt * 16 + e) * 64];
+        square += acc[dt][e] * acc[dt][e];
+      }
+    if (p.norm_weight) {
+      f32x4 w[DT * 4];  // all asked for before the first is used
+#pragma unroll
+      for (int k = 0; k < DT * 4; ++k) w[k] = *reinterpret_cast<const f32x4 *>(p.norm_weight + 8 * k + 4 * half);
+      const float mul = p.out_scale / sqrtf(halves_sum(square) / D + p.norm_eps);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] *= mul * w[dt * 4 + (e >> 2)][e & 3];
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= p.out_scale;
+    }
+  }
+  // rows of D 16-bit values in the wavefront's own part of LDS, their 16-byte pieces swizzled by the row
+  constexpr int kPer = D / 8;  // 16-byte pieces, and lanes, per row
+  char *mine = lds + strip * 32 * D * 2 * MAPS;
+  const auto put = [&](auto type) {
+    using OutT = decltype(type);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<u32x2 *>(mine + col * (D * 2) + (((4 * dt + k) ^ (col & (kPer - 1))) * 16) + half * 8) =
+            u32x2{pack2<OutT>(acc[dt][4 * k], acc[dt][4 * k + 1]), pack2<OutT>(acc[dt][4 * k + 2], acc[dt][4 * k + 3])};
+  };
+  if (p.q_bf16) put(BF16{});  // (asked once, not for every pair)
+  else put(F16{});
+  const int32_t out_row = (q.first + j) * p.num_heads + head;  // (num_tokens x num_heads fits 31 bits)
+  const int left = all_rows - row0 - strip * 32;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 64 / kPer) {
+    const int r = r0 + lane / kPer, c = lane & (kPer - 1);
+    const int32_t to = __shfl(out_row, r);
+    const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + r * (D * 2) + ((c ^ (r & (kPer - 1))) * 16));
+    if (r < left) *reinterpret_cast<u32x4 *>(p.out + (int64_t)to * (D * 2) + c * 16) = v;
+  }
+  static_assert(kRows * D * 2 * MAPS <= 4 * kTileKeys * D * 2 && (MAPS == 1 || kRows * D * 4 <= 4 * kTileKeys * D * 2), "it fits the buffers");
+}
+
+template <int D, typename OT, int KVF, int MAPS, int NW, bool EXT, bool LINE>
 __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) ragged_tile_kernel(const RaggedParams p) {
   using T = RaggedTile<D, KVF, MAPS, NW>;
   constexpr bool KV8 = T::KV8;
@@ -104,25 +311,72 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const int strip = MAPS == 2 ? wave % (NW / 2) : wave;
   const int Hk = p.num_kv_heads, G = p.group;
 
-  // which tile of rows: the last tiles of a sequence, which see the most keys, come first
-  const int tile = blockIdx.x / Hk, kvh = blockIdx.x - tile * Hk;
-  const RaggedPlace at = ragged_find(p.b.num_seqs, tile, lane,
-                                     [&](int s) { return row_tiles<MAPS, T::kRows>(p, ragged_seq_of_lane(p.b, s)); });
-  const int seq = __builtin_amdgcn_readfirstlane(at.seq);
-  if (seq >= p.b.num_seqs) return;
-  const RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq));
-  const int all_rows = q.n * G;
-  const int row0 = (row_tiles<MAPS, T::kRows>(p, q) - 1 - (tile - __builtin_amdgcn_readfirstlane(at.before))) * T::kRows;
-
-  // the keys that the work-group goes through, in steps of 64
-  const int pos0 = q.ctx - q.n;  // position of the sequence's first new token
-  const int pos_lo = pos0 + row0 / G, pos_hi = pos0 + (min(row0 + T::kRows, all_rows) - 1) / G;
-  int step = max(0, pos_lo - p.window) / kTileKeys, step_end = pos_hi < 0 ? 0 : pos_hi / kTileKeys + 1;
-  if (p.splits > 1) {
-    const int share = (max(0, step_end - step) + p.splits - 1) / p.splits;
-    step += (int)blockIdx.y * share;
-    step_end = min(step_end, step + share);
+  // This work-group's tiles: one, the last ones of a sequence first, since they see the most keys; or a share of the line.
+  // Work-groups are handed to the eight XCCs in turn: each gets an eighth of the line, so that tiles of one kv head meet in
+  // few L2 caches.
+  int seq, kvh, tile, from = 0, g = 0, end_seq = 0, end_kvh = 0, end_tile = 0, end_cut = 0;
+  bool first_piece = true;
+  if constexpr (LINE) {
+    const TileLine<MAPS, T::kRows> line(p, lane);
+    const int per = (line.groups + 7) >> 3;
+    g = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+    if (((int)blockIdx.x >> 3) >= per || g >= line.groups) return;
+    const TilePlace at = line.find(p, line.cut(g), lane), to = line.find(p, line.cut(g + 1) - 1, lane);
+    seq = at.seq, kvh = at.kvh, tile = at.tile;
+    end_seq = to.seq, end_kvh = to.kvh, end_tile = to.tile;
+    const RaggedSeq q0 = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq)), q1 = ragged_seq_cut(p, ragged_seq_uniform(p.b, end_seq));
+    const TileCosts c0 = tile_costs<MAPS, T::kRows>(p, q0), c1 = tile_costs<MAPS, T::kRows>(p, q1);
+    from = cut_step(at.off, c0.first + c0.more * tile, tile_steps<T::kRows>(p, q0, tile).count);
+    const int64_t end_cost = c1.first + c1.more * end_tile;
+    const int end_count = tile_steps<T::kRows>(p, q1, end_tile).count;
+    end_cut = to.off + 1 == end_cost ? end_count : cut_step(to.off + 1, end_cost, end_count);
+    from = __builtin_amdgcn_readfirstlane(from), end_cut = __builtin_amdgcn_readfirstlane(end_cut);
+  } else {
+    const int t = blockIdx.x / Hk;
+    kvh = blockIdx.x - t * Hk;
+    int before;
+    if (p.b.num_seqs <= 64) {
+      // Sequences with more keys first.  Each lane has one; its rank is the number of those before it, and what lies before it the
+      // sum of their tiles.
+      const RaggedSeq mine = lane < p.b.num_seqs ? ragged_seq_of_lane(p.b, lane) : RaggedSeq{0, 0, 0};
+      const int tiles = lane < p.b.num_seqs ? row_tiles<MAPS, T::kRows>(p, mine) : 0;
+      before = 0;
+      for (int s = 0; s < p.b.num_seqs; ++s) {
+        const int ctx = __builtin_amdgcn_readlane(mine.ctx, s), n = __builtin_amdgcn_readlane(tiles, s);
+        before += ctx > mine.ctx || (ctx == mine.ctx && s < lane) ? n : 0;
+      }
+      const unsigned long long here = __ballot(t >= before && t < before + tiles);
+      if (here == 0) return;
+      seq = __builtin_ctzll(here);
+      before = __builtin_amdgcn_readlane(before, seq);
+    } else {
+      const RaggedPlace at = ragged_find(p.b.num_seqs, t, lane,
+                                         [&](int s) { return row_tiles<MAPS, T::kRows>(p, ragged_seq_of_lane(p.b, s)); });
+      seq = __builtin_amdgcn_readfirstlane(at.seq);
+      if (seq >= p.b.num_seqs) return;
+      before = __builtin_amdgcn_readfirstlane(at.before);
+    }
+    tile = row_tiles<MAPS, T::kRows>(p, ragged_seq_uniform(p.b, seq)) - 1 - (t - before);
+    end_seq = seq, end_kvh = kvh, end_tile = tile, end_cut = 0x7fffffff;
   }
+
+  // Everything this work-group wrote to LDS is there, and nobody goes on before everybody is here.
+  auto meet = [&]() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  };
+
+  for (;; first_piece = false) {
+  const RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq));
+  const bool last_tile = !LINE || (seq == end_seq && kvh == end_kvh && tile == end_tile);
+  const TileSteps of_tile = tile_steps<T::kRows>(p, q, tile);
+  const int until = LINE && last_tile ? min(end_cut, of_tile.count) : of_tile.count;
+  const bool whole = !LINE || (from == 0 && until == of_tile.count);
+  if (whole || from < until) {  // (a tile that sees no keys is whole: its rows get zeros)
+  const int all_rows = q.n * G, row0 = tile * T::kRows;
+  const int pos0 = q.ctx - q.n;  // position of the sequence's first new token
+  const int step = of_tile.first + from, step_end = of_tile.first + until;
 
   // this lane's row (rows past the end repeat the last one and are not stored)
   const int my_row = row0 + strip * 32 + col;
@@ -158,7 +412,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const float slope = EXT && (p.mask_flags & kMaskAlibi) ? p.alibi_slopes[head] * kLog2e : 0.f;
 
   float m = -INFINITY, mt = -INFINITY, l = 0.f, mv = -INFINITY, mvt = -INFINITY;
-  if (p.sinks != nullptr && blockIdx.y == 0) {
+  if (p.sinks != nullptr && from == 0) {
     m = mt = sink_log2(p, head);
     l = half == 0 ? 1.f : 0.f;
   }
@@ -173,7 +427,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const int piece = tid % T::kPerRow, load_row = tid / T::kPerRow;
   const bool loads = T::kRowsPerPass <= kTileKeys || load_row < kTileKeys;
   const int last_col = p.b.max_blocks_per_seq - 1, in_block = (1 << p.b.block_shift) - 1;
-  const int steps = max(0, step_end - step);
+  const int steps = step_end - step;
   // Blocks of this thread's rows: of the next step of K as the table has them (cut to the pool where they are used, since
   // arithmetic here would wait for the load, and for every load before it), and of the next step of V, one step behind.
   int32_t kid[T::kPasses], vid[T::kPasses];
@@ -292,7 +546,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   // keys in turn), then the values of the step before (d-tiles of its four groups of 16 keys).  kAhead operands are on
   // their way at any time; the order is held with scheduling barriers, since left to itself the compiler reads an operand right
   // in front of the product that waits for it.
-  constexpr int kScoreOps = 2 * KS, kValueOps = 4 * DT, kAhead = 6;
+  constexpr int kScoreOps = 2 * KS, kValueOps = 4 * DT, kAhead = 4;
   auto operand = [&](int op, const char *kb, const char *vb) {
     if (op < kScoreOps) return *reinterpret_cast<const u32x4 *>(kb + (k_base ^ ((op >> 1) << 5)) + (op & 1) * 32 * 2 * D);
     const int k = (op - kScoreOps) / DT, dt = (op - kScoreOps) % DT;
@@ -454,18 +708,12 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
       l += part[0] + part[1];
     }
   };
-  // Everything this work-group wrote to LDS is there, and nobody goes on before everybody is here.
-  auto meet = [&]() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-  };
-
   // ---- steps ----
   // Matrix phase of step n: scores of n + 1 and values of n, and between the products the thread's share of V of n + 1 and K of
   // n + 2 goes to LDS (what the next matrix phase reads) and the loads of the step after that are sent out.  Vector phase: softmax
   // of n + 1.  With eight wavefronts every SIMD has two: the second four run one phase behind the first, so that one is in its
   // matrix phase while the other is in its vector phase.
+  if (LINE && !first_piece) meet();  // LDS of the piece before has been read
   if (steps > 0) {
     constexpr bool kTurns = NW == 8;
     const int late = kTurns ? wave >> 2 : 0;
@@ -527,116 +775,90 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
   }
-  if (p.splits > 1) {
-    const int64_t slot = (int64_t)blockIdx.x * p.splits + blockIdx.y;
-    const int r = map * T::kRows + strip * 32 + col;
-    constexpr int kAll = T::kRows * MAPS;
-    if (valid) {
-      float *dst = p.tile_o + (slot * kAll + r) * D + 4 * half;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<f32x4 *>(dst + 32 * dt + 8 * k) = f32x4{acc[dt][4 * k], acc[dt][4 * k + 1], acc[dt][4 * k + 2], acc[dt][4 * k + 3]};
-      if (half == 0) {
-        p.tile_ml[slot * 2 * kAll + r] = mt;
-        p.tile_ml[slot * 2 * kAll + kAll + r] = l;
-      }
-    }
-    return;
-  }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  char *dst = p.out + ((int64_t)(q.first + j) * p.num_heads + head) * (D * 2) + 8 * half;
-  if constexpr (MAPS == 1) {
-    if (valid) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<u32x2 *>(dst + 64 * dt + 16 * k) =
-              u32x2{pack_out(p, acc[dt][4 * k] * inv, acc[dt][4 * k + 1] * inv), pack_out(p, acc[dt][4 * k + 2] * inv, acc[dt][4 * k + 3] * inv)};
-    }
+  if (whole) {
+    meet();  // nobody reads V any more
+    tile_finish<D, MAPS, NW>(p, q, kvh, row0, acc, l, lds);
   } else {
-    // second maps -> first maps, through LDS (a lane's values at [value][lane] of its strip)
-    constexpr int kValues = DT * 16;
-    static_assert(kValues * 64 * 4 * (NW / 2) <= T::kLdsBytes, "the second maps' results fit the buffers");
-    float *through = reinterpret_cast<float *>(lds) + strip * kValues * 64 + lane;
-    __syncthreads();  // nobody reads V any more
-    if (map == 1) {
+    // a piece of a tile: as it lies in the registers, 1 KiB at a time (slots: see ragged_tile_merge_kernel)
+    const int64_t slot = 2 * (int64_t)g + (first_piece ? 0 : 1);
+    float *dst = p.tile_o + ((slot * NW + wave) * (DT * 4) * 64 + lane) * 4;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) through[(dt * 16 + e) * 64] = acc[dt][e] * inv;
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<f32x4 *>(dst + (dt * 4 + k) * 256) = f32x4{acc[dt][4 * k], acc[dt][4 * k + 1], acc[dt][4 * k + 2], acc[dt][4 * k + 3]};
+    float *ml = p.tile_ml + (slot * NW + wave) * 128 + lane;
+    ml[0] = mt;
+    ml[64] = l;
+  }
+  }
+  if (!LINE || last_tile) return;
+  from = 0;
+  if (++tile == row_tiles<MAPS, T::kRows>(p, q)) {
+    tile = 0;
+    if (++kvh == Hk) {
+      kvh = 0;
+      do ++seq;
+      while (row_tiles<MAPS, T::kRows>(p, ragged_seq_uniform(p.b, seq)) == 0);
     }
-    __syncthreads();
-    if (map == 0) {
-      const float lambda = p.lambdas[head];
-      float square = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          acc[dt][e] = acc[dt][e] * inv - lambda * through[(dt * 16 + e) * 64];
-          square += acc[dt][e] * acc[dt][e];
-        }
-      float mul = p.out_scale;
-      if (p.norm_weight) mul /= sqrtf(halves_sum(square) / D + p.norm_eps);
-      if (valid) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            f32x4 w = {mul, mul, mul, mul};
-            if (p.norm_weight) w *= *reinterpret_cast<const f32x4 *>(p.norm_weight + 32 * dt + 8 * k + 4 * half);
-            *reinterpret_cast<u32x2 *>(dst + 64 * dt + 16 * k) = u32x2{pack_out(p, acc[dt][4 * k] * w[0], acc[dt][4 * k + 1] * w[1]),
-                                                                      pack_out(p, acc[dt][4 * k + 2] * w[2], acc[dt][4 * k + 3] * w[3])};
-          }
-      }
-    }
+  }
   }
 }
 
-// Joins the pieces of a tile's rows: work-group (tile and kv head, 16 rows), a wavefront per row.
-template <int D, int MAPS, int ROWS>
-__global__ void __launch_bounds__(256) ragged_tile_merge_kernel(const RaggedParams p) {
-  constexpr int N = D / 64, kAll = ROWS * MAPS;
+// Joins the pieces of a cut tile.  Work-group g looks at the cut between the shares of g and g + 1: if it is the first one within
+// its tile, the pieces are those of g (its first, if its share begins with the tile, else its second one) and of the work-groups
+// after it, whose first pieces they are.
+template <int D, int MAPS, int NW>
+__global__ void __launch_bounds__(NW * 64) ragged_tile_merge_kernel(const RaggedParams p) {
+  constexpr int DT = D / 32, ROWS = NW * 32 / MAPS;
+  __shared__ __attribute__((aligned(16))) char lds[4 * kTileKeys * D * 2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int Hk = p.num_kv_heads, G = p.group;
-  const int tile = blockIdx.x / Hk, kvh = blockIdx.x - tile * Hk;
-  const RaggedPlace at = ragged_find(p.b.num_seqs, tile, lane,
-                                     [&](int s) { return row_tiles<MAPS, ROWS>(p, ragged_seq_of_lane(p.b, s)); });
-  const int seq = __builtin_amdgcn_readfirstlane(at.seq);
-  if (seq >= p.b.num_seqs) return;
-  const RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq));
-  const int all_rows = q.n * G;
-  const int row0 = (row_tiles<MAPS, ROWS>(p, q) - 1 - (tile - __builtin_amdgcn_readfirstlane(at.before))) * ROWS;
-  for (int r = (int)blockIdx.y * 16 + wave; r < (int)blockIdx.y * 16 + 16; r += 4) {
-    const int row = row0 + r;
-    if (row >= all_rows) return;
-    const int j = row / G, head = kvh * G + (row - j * G);
-    RowMerge<N> of[MAPS];
+  const TileLine<MAPS, ROWS> line(p, lane);
+  const int g = blockIdx.x;
+  if (g + 1 >= line.groups) return;
+  const int64_t at = line.cut(g + 1);
+  const TilePlace place = line.find(p, at, lane);
+  const int64_t start = at - place.off, before = line.cut(g);  // of the tile; of the share of g
+  if (place.off == 0 || before > start) return;  // a cut between two tiles, or not the first one within its tile
+  const RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, place.seq));
+  const TileCosts c = tile_costs<MAPS, ROWS>(p, q);
+  const int64_t cost = c.first + c.more * place.tile;
+  const int steps = tile_steps<ROWS>(p, q, place.tile).count;
+
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[DT];
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m) {
-#pragma unroll 4
-      for (int x = 0; x < p.splits; ++x) {
-        const int64_t slot = (int64_t)blockIdx.x * p.splits + x;
-        const float *src = p.tile_o + (slot * kAll + m * ROWS + r) * D + lane * N;
-        float po[N];
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int k = 0; k < N; ++k) po[k] = src[k];
-        of[m].add(p.tile_ml[slot * 2 * kAll + m * ROWS + r], p.tile_ml[slot * 2 * kAll + kAll + m * ROWS + r], po);
-      }
-      of[m].normalise();
+    for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
+  int from = 0;
+  for (int h = g;; ++h) {
+    const int64_t share_end = h + 1 < line.groups ? line.cut(h + 1) : line.total;
+    const bool last = share_end >= start + cost;
+    const int until = __builtin_amdgcn_readfirstlane(last ? steps : cut_step(share_end - start, cost, steps));
+    if (from == 0 && until == steps) return;  // one piece has it all: its work-group has stored the rows
+    if (from < until) {
+      const int64_t slot = 2 * (int64_t)h + (h == g && before < start ? 1 : 0);
+      const float *ml = p.tile_ml + (slot * NW + wave) * 128 + lane;
+      const float *src = p.tile_o + ((slot * NW + wave) * (DT * 4) * 64 + lane) * 4;
+      const float pm = ml[0], to = fmaxf(m, pm), sub = to == -INFINITY ? 0.f : to;
+      const float mine = fast_exp2(m - sub), its = fast_exp2(pm - sub);
+      l = l * mine + ml[64] * its;
+      m = to;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const f32x4 o = *reinterpret_cast<const f32x4 *>(src + (dt * 4 + k) * 256);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[dt][4 * k + e] = acc[dt][4 * k + e] * mine + o[e] * its;
+        }
     }
-    if constexpr (MAPS == 2) {
-      float x[N];
-      differential_row<N>(p, head, lane, of[0].o, of[1].o, x);
-      store_row<N>(p, q.first + j, head, lane, x);
-    } else {
-      store_row<N>(p, q.first + j, head, lane, of[0].o);
-    }
+    from = until;
+    if (last) break;
   }
+  tile_finish<D, MAPS, NW>(p, q, place.kvh, place.tile * ROWS, acc, l, lds);
 }
 
 }  // namespace fa
