@@ -18,6 +18,7 @@ struct RaggedPlan {
   int64_t tile_bound;     // tiles per kv head, at most
   int tile_groups;        // work-groups that share all tiles; 0: a work-group for each tile
   int row_groups;
+  bool row_aligned;       // rows form: a work-group for each item, and no second kernel
   int64_t row_o, row_ml, row_items, tile_o, tile_ml, bytes;  // offsets into the workspace, and its size
 };
 
@@ -70,11 +71,17 @@ inline RaggedPlan ragged_plan(const fa_ragged_shape &s, int maps, int cus) {
     return here;
   };
   if (r.rows) {
-    r.row_groups = (int)std::min<int64_t>(2 * (int64_t)cus, S * Hk * (keys / kRowUnit + 2));
-    const int64_t slots = S * Hk + r.row_groups;
-    r.row_o = take(slots * kRowColumns * D * 4);
-    r.row_ml = take(slots * 2 * kRowColumns * 4);
-    r.row_items = take(S * Hk * 8);
+#ifndef FORCE_ALIGNED
+#define FORCE_ALIGNED 512
+#endif
+    r.row_aligned = keys <= FORCE_ALIGNED;
+    r.row_groups = (int)std::min<int64_t>({2 * (int64_t)cus, kMaxRowGroups, S * Hk * (keys / kRowUnit + 2)});
+    if (!r.row_aligned) {
+      const int64_t slots = S * Hk + r.row_groups;
+      r.row_o = take(slots * kRowColumns * D * 4);
+      r.row_ml = take(slots * 2 * kRowColumns * 4);
+      r.row_items = take(S * Hk * 8);
+    }
   }
   if (r.tiles) {
     // 8 wavefronts halve what K and V cost per row; sequences that cannot fill them take 4
@@ -133,10 +140,11 @@ inline fa_status launch_ragged_kernels(const RaggedParams &p, const RaggedPlan &
     }
   }
   if (plan.rows) {
-    FA_HIP_CHECK(timer.launch(ragged_rows_kernel<D, OT, KVF, MAPS>, dim3((unsigned)plan.row_groups), dim3(256), 0, p));
-    if ((st = timed()) != FA_OK) return st;
+    const unsigned groups = plan.row_aligned ? (unsigned)(p.b.num_seqs * Hk) : (unsigned)plan.row_groups;
+    FA_HIP_CHECK(timer.launch(ragged_rows_kernel<D, OT, KVF, MAPS>, dim3(groups), dim3(256), 0, p));
+    if ((st = timed()) != FA_OK || plan.row_aligned) return st;
     const int rows = std::min<int64_t>(kRowColumns / MAPS, (int64_t)p.max_query_len * p.group);
-    FA_HIP_CHECK(timer.launch(ragged_rows_merge_kernel<D, MAPS>, dim3((unsigned)(p.b.num_seqs * Hk), (unsigned)rows), dim3(256), 0, p));
+    FA_HIP_CHECK(timer.launch(ragged_rows_merge_kernel<D, MAPS>, dim3((unsigned)(p.b.num_seqs * Hk), (unsigned)rows), dim3(512), 0, p));
     if ((st = timed()) != FA_OK) return st;
   }
   return FA_OK;
@@ -251,6 +259,7 @@ inline fa_status launch_ragged_attention(void *out, const void *query, const voi
   }
   char *space = reinterpret_cast<char *>(workspace);
   p.row_groups = plan.row_groups;
+  p.row_aligned = plan.row_aligned;
   p.row_o = reinterpret_cast<float *>(space + plan.row_o);
   p.row_ml = reinterpret_cast<float *>(space + plan.row_ml);
   p.row_items = reinterpret_cast<int2 *>(space + plan.row_items);

@@ -38,7 +38,8 @@ struct RaggedParams {
   const float *norm_weight;
   float norm_eps, out_scale;
   // rows form: work-groups, and their partial results
-  int32_t row_groups;
+  int32_t row_groups;           // at most kMaxRowGroups
+  int32_t row_aligned;          // a work-group for each item instead: nothing is cut, nothing merged
   float *row_o;                 // [slot][16][D]
   float *row_ml;                // [slot][2][16]: maxima (base-2 units), sums
   int2 *row_items;              // [seq * kv heads + kv head]: first and last work-group of the item
@@ -49,6 +50,7 @@ struct RaggedParams {
 };
 
 constexpr int kRowColumns = 16;     // rows of the rows form: MFMA columns of a wavefront
+constexpr int kMaxRowGroups = 512;  // work-groups that share the line of units
 constexpr int kRowUnit = 128;       // keys that a work-group of the rows form takes at a time
 constexpr int kTileKeys = 64;       // keys per step of the tile form
 constexpr int kNoWindow = 0x3fffffff;
@@ -155,25 +157,5 @@ __device__ __forceinline__ void store_row(const RaggedParams &p, int token, int 
     *reinterpret_cast<uint16_t *>(dst) = (uint16_t)pack_out(p, x[0], 0.f);
   }
 }
-
-// Partial results of one row: running maximum, sum and weighted values, merged in the order of the pieces.
-template <int N>
-struct RowMerge {
-  float m = -INFINITY, l = 0.f, o[N] = {};
-  __device__ __forceinline__ void add(float pm, float pl, const float (&po)[N]) {
-    const float to = fmaxf(m, pm);
-    const float sub = to == -INFINITY ? 0.f : to;
-    const float mine = fast_exp2(m - sub), its = fast_exp2(pm - sub);
-    l = l * mine + pl * its;
-#pragma unroll
-    for (int k = 0; k < N; ++k) o[k] = o[k] * mine + po[k] * its;
-    m = to;
-  }
-  __device__ __forceinline__ void normalise() {
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-    for (int k = 0; k < N; ++k) o[k] *= inv;
-  }
-};
 
 }  // namespace fa

@@ -126,31 +126,73 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int Hk = p.num_kv_heads, G = p.group;
 
-  // this work-group's share of the line of units
-  int32_t mine = 0;
-  for (int s = lane; s < p.b.num_seqs; s += 64) mine += row_units<MAPS>(p, ragged_seq_of_lane(p.b, s));
-  const int32_t total = __builtin_amdgcn_readlane(wave_inclusive_scan(mine, lane), 63) * Hk;
-  const int groups = min(p.row_groups, total);
+  // This work-group's share of the line of units.  The first 64 sequences' lengths are asked for once; whose turn it is
+  // among them is read from the lanes.
+  RaggedSeq of_lane = {0, 0, 0};
+  int32_t units_of_lane = 0;
+  if (lane < p.b.num_seqs) {
+    of_lane = ragged_seq_of_lane(p.b, lane);
+    units_of_lane = row_units<MAPS>(p, of_lane);
+  }
+  const auto seq_at = [&](int s) {
+    return s < 64 ? RaggedSeq{__builtin_amdgcn_readlane(of_lane.first, s), __builtin_amdgcn_readlane(of_lane.n, s),
+                              __builtin_amdgcn_readlane(of_lane.ctx, s)}
+                  : ragged_seq_uniform(p.b, s);
+  };
   const int g = blockIdx.x;
-  if (g >= groups) return;
-  int32_t u = (int32_t)((int64_t)total * g / groups);
-  const int32_t u_end = (int32_t)((int64_t)total * (g + 1) / groups);
-  const RaggedPlace at = ragged_find(p.b.num_seqs, u, lane,
-                                     [&](int s) { return row_units<MAPS>(p, ragged_seq_of_lane(p.b, s)) * Hk; });
-  int seq = __builtin_amdgcn_readfirstlane(at.seq);
-  int32_t before = __builtin_amdgcn_readfirstlane(at.before);
+  int32_t total = 0, u, u_end, before = 0;
+  int groups = 0, seq;
+  if (p.row_aligned) {  // one work-group per item
+    seq = g / Hk;
+    const int units = row_units<MAPS>(p, seq_at(seq));
+    u = (g - seq * Hk) * units;
+    u_end = u + units;
+    const RaggedSeq q = ragged_seq_cut(p, seq_at(seq));
+    if (units == 0) {  // no keys: zeros
+      if (q.n > 0 && in_rows_form<MAPS>(p, q))
+        for (int k = threadIdx.x; k < q.n * G * (D / 8); k += 256) {
+          const int row = k / (D / 8), j = row / G;
+          *reinterpret_cast<u32x4 *>(p.out + (((int64_t)(q.first + j) * p.num_heads + (g - seq * Hk) * G + (row - j * G)) * D + (k % (D / 8)) * 8) * 2) =
+              u32x4{0u, 0u, 0u, 0u};
+        }
+      return;
+    }
+  } else {
+    const int32_t upto = wave_inclusive_scan(units_of_lane, lane);
+    total = __builtin_amdgcn_readlane(upto, 63);
+    if (p.b.num_seqs > 64) {
+      int32_t more = 0;
+      for (int s = 64 + lane; s < p.b.num_seqs; s += 64) more += row_units<MAPS>(p, ragged_seq_of_lane(p.b, s));
+      total += __builtin_amdgcn_readlane(wave_inclusive_scan(more, lane), 63);
+    }
+    total *= Hk;
+    groups = min(p.row_groups, total);
+    if (g >= groups) return;
+    u = (int32_t)((int64_t)total * g / groups);
+    u_end = (int32_t)((int64_t)total * (g + 1) / groups);
+    const unsigned long long beyond = __ballot(upto * Hk > u);
+    if (beyond) {
+      seq = __builtin_ctzll(beyond);
+      before = (__builtin_amdgcn_readlane(upto, seq) - __builtin_amdgcn_readlane(units_of_lane, seq)) * Hk;
+    } else {
+      const RaggedPlace at = ragged_find(p.b.num_seqs, u, lane,
+                                         [&](int s) { return row_units<MAPS>(p, ragged_seq_of_lane(p.b, s)) * Hk; });
+      seq = __builtin_amdgcn_readfirstlane(at.seq);
+      before = __builtin_amdgcn_readfirstlane(at.before);
+    }
+  }
 
   W wa(p.a, lane);
   const int r = wa.r, i = wa.i;
   while (u < u_end) {
-    RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq));
+    RaggedSeq q = ragged_seq_cut(p, seq_at(seq));
     const int units = row_units<MAPS>(p, q);
     if (u >= before + units * Hk) {
       before += units * Hk;
       ++seq;
       continue;
     }
-    const int kvh = (u - before) / units;
+    const int kvh = p.row_aligned ? g - seq * Hk : (u - before) / units;
     const int first = (u - before) - kvh * units;
     const int last = min(units, first + (u_end - u));
     const int item = seq * Hk + kvh;
@@ -291,6 +333,33 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
 #pragma unroll
           for (int k = 0; k < SL; k += 2) *reinterpret_cast<uint32_t *>(dst + 2 * k) = pack_out(p, o[k] * inv, o[k + 1] * inv);
         }
+      } else if (MAPS == 2 && whole) {
+        // the maps of a row lie in neighbouring columns
+        const float inv = L == 0.f ? 0.f : v_mul / L;
+        const float lambda = p.lambdas[valid ? head : 0];
+        float square = 0.f;
+#pragma unroll
+        for (int k = 0; k < SL; ++k) {
+          const float mine = o[k] * inv;
+          const float other = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, mine), 0xB1, 0xF, 0xF, true));
+          o[k] = mine - lambda * other;  // (of use in the columns of the first map)
+          square += o[k] * o[k];
+        }
+        float mul = p.out_scale;
+        if (p.norm_weight) {
+          __syncthreads();  // the maxima have been read
+          sm_m[wave][i] = rows_sum(square);
+        }
+        __syncthreads();
+        if (p.norm_weight) mul /= sqrtf((sm_m[0][i] + sm_m[1][i] + sm_m[2][i] + sm_m[3][i]) / D + p.norm_eps);
+        if (valid && map == 0) {
+          char *dst = p.out + (((int64_t)(q.first + j) * p.num_heads + head) * D + d0) * 2;
+          float w[SL];
+#pragma unroll
+          for (int k = 0; k < SL; ++k) w[k] = p.norm_weight ? mul * p.norm_weight[d0 + k] : mul;
+#pragma unroll
+          for (int k = 0; k < SL; k += 2) *reinterpret_cast<uint32_t *>(dst + 2 * k) = pack_out(p, o[k] * w[k], o[k + 1] * w[k + 1]);
+        }
       } else {
         const int64_t slot = (int64_t)item + g;
         if (valid) {
@@ -304,7 +373,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
           p.row_ml[slot * 2 * kRowColumns + kRowColumns + i] = L;
         }
       }
-      if (first == 0 && threadIdx.x == 0) {  // the work-groups that hold the item's pieces
+      if (first == 0 && threadIdx.x == 0 && !p.row_aligned) {  // the work-groups that hold the item's pieces
         const int64_t end = (int64_t)before + (int64_t)kvh * units + units;
         p.row_items[item] = int2{g, (int)((end * groups - 1) / total)};
       }
@@ -312,68 +381,113 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   }
 }
 
-// Joins the pieces of an item's rows.  Work-group (item, row); its four wavefronts take every fourth piece each.
+// Joins the pieces of an item's rows.  Work-group (item, row): the pieces' maxima first, in LDS as factors; then the eight wavefronts
+// sum every eighth piece each, with no load waiting for another.
 template <int D, int MAPS>
-__global__ void __launch_bounds__(256) ragged_rows_merge_kernel(const RaggedParams p) {
-  constexpr int N = D / 64;
-  __shared__ float sm[MAPS][4][N + 2][64];
+__global__ void __launch_bounds__(512) ragged_rows_merge_kernel(const RaggedParams p) {
+  constexpr int N = D / 64, NW = 8, kAhead = 4;
+  __shared__ float factor[MAPS][kMaxRowGroups];
+  __shared__ float sm[MAPS][NW][N][64], tops[MAPS][NW], sums[MAPS][NW];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int item = blockIdx.x, row = blockIdx.y;
   const int seq = item / p.num_kv_heads, kvh = item - seq * p.num_kv_heads;
+  // (not set where the item has no keys; asked for with the lengths)
+  const int first = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_items + item));
+  const int last = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_items + item) + 1);
   const RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq));
   if (row >= q.n * p.group || !in_rows_form<MAPS>(p, q)) return;
   const int j = row / p.group, head = kvh * p.group + (row - j * p.group);
-  int2 span = {0, -1};  // (no keys: no pieces)
-  if (row_units<MAPS>(p, q) > 0) {
-    span.x = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_items + item));
-    span.y = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_items + item) + 1);
-    if (MAPS == 1 && span.x == span.y) return;  // the rows kernel has stored the result
-  }
-  RowMerge<N> of[MAPS];
-#pragma unroll
-  for (int m = 0; m < MAPS; ++m) {
-    const int c = MAPS == 2 ? row * 2 + m : row;
-#pragma unroll 4
-    for (int g = span.x + wave; g <= span.y; g += 4) {
-      const int64_t slot = (int64_t)item + g;
-      const float pm = p.row_ml[slot * 2 * kRowColumns + c], pl = p.row_ml[slot * 2 * kRowColumns + kRowColumns + c];
-      const float *src = p.row_o + (slot * kRowColumns + c) * D + lane * N;
-      float po[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k) po[k] = src[k];
-      of[m].add(pm, pl, po);
-    }
-  }
-  if (span.y - span.x >= 1) {
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) {
-      sm[m][wave][0][lane] = of[m].m;
-      sm[m][wave][1][lane] = of[m].l;
-#pragma unroll
-      for (int k = 0; k < N; ++k) sm[m][wave][2 + k][lane] = of[m].o[k];
-    }
-    __syncthreads();
-    if (wave != 0) return;
+  const int pieces = row_units<MAPS>(p, q) > 0 ? last - first + 1 : 0;
+  if (pieces == 1) return;  // the rows kernel has stored the result
+  const int64_t slot0 = (int64_t)item + first;
+  float o[MAPS][N] = {};
+  if (pieces > 0) {
+    float early[MAPS][kAhead][N];  // the first pieces' values, asked for before the factors are known
 #pragma unroll
     for (int m = 0; m < MAPS; ++m)
 #pragma unroll
-      for (int w = 1; w < 4; ++w) {
-        float po[N];
+      for (int u = 0; u < kAhead; ++u) {
+        const int x = min(wave + u * NW, pieces - 1);
+        const float *src = p.row_o + ((slot0 + x) * kRowColumns + row * MAPS + m) * D + lane * N;
 #pragma unroll
-        for (int k = 0; k < N; ++k) po[k] = sm[m][w][2 + k][lane];
-        of[m].add(sm[m][w][0][lane], sm[m][w][1][lane], po);
+        for (int k = 0; k < N; ++k) early[m][u][k] = src[k];
       }
+    float l_of[MAPS];
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      float top = -INFINITY;
+      l_of[m] = 0.f;
+      for (int x = threadIdx.x; x < pieces; x += 512) {  // (no more than 512 pieces: once)
+        const float *ml = p.row_ml + (slot0 + x) * 2 * kRowColumns + row * MAPS + m;
+        top = ml[0];
+        l_of[m] = ml[kRowColumns];
+        factor[m][x] = top;
+      }
+      top = wave_max(top);
+      if (lane == 0) tops[m][wave] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      float top = tops[m][0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) top = fmaxf(top, tops[m][w]);
+      const float sub = top == -INFINITY ? 0.f : top;
+      float l = 0.f;
+      for (int x = threadIdx.x; x < pieces; x += 512) {
+        const float f = fast_exp2(factor[m][x] - sub);
+        factor[m][x] = f;
+        l = f * l_of[m];
+      }
+      l = wave_sum(l);
+      if (lane == 0) sums[m][wave] = l;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float f = wave + u * NW < pieces ? factor[m][wave + u * NW] : 0.f;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[m][k] += f == 0.f ? 0.f : f * early[m][u][k];
+      }
+#pragma unroll 8
+      for (int x = wave + kAhead * NW; x < pieces; x += NW) {
+        const float f = factor[m][x];
+        const float *src = p.row_o + ((slot0 + x) * kRowColumns + row * MAPS + m) * D + lane * N;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[m][k] += f * src[k];
+      }
+#pragma unroll
+      for (int k = 0; k < N; ++k) sm[m][wave][k][lane] = o[m][k];
+    }
+    __syncthreads();
   }
   if (wave != 0) return;
 #pragma unroll
-  for (int m = 0; m < MAPS; ++m) of[m].normalise();
+  for (int m = 0; m < MAPS; ++m) {
+    float l = 0.f;
+    if (pieces > 0) {
+#pragma unroll
+      for (int w = 0; w < NW; ++w) l += sums[m][w];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        o[m][k] = sm[m][0][k][lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) o[m][k] += sm[m][w][k][lane];
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int k = 0; k < N; ++k) o[m][k] *= inv;
+  }
   if constexpr (MAPS == 2) {
     float x[N];
-    differential_row<N>(p, head, lane, of[0].o, of[1].o, x);
+    differential_row<N>(p, head, lane, o[0], o[1], x);
     store_row<N>(p, q.first + j, head, lane, x);
   } else {
-    store_row<N>(p, q.first + j, head, lane, of[0].o);
+    store_row<N>(p, q.first + j, head, lane, o[0]);
   }
 }
 
