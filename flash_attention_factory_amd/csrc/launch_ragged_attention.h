@@ -17,9 +17,9 @@ struct RaggedPlan {
   int tile_rows;          // rows of its tiles
   int64_t tile_bound;     // tiles per kv head, at most
   int tile_groups;        // work-groups that share all tiles; 0: a work-group for each tile
-  int row_groups;
+  int row_groups, row_shares;
   bool row_aligned;       // rows form: a work-group for each item, and no second kernel
-  int64_t row_o, row_ml, row_items, tile_o, tile_ml, bytes;  // offsets into the workspace, and its size
+  int64_t row_o, row_ml, row_seqs, tile_o, tile_ml, bytes;  // offsets into the workspace, and its size
 };
 
 inline fa_status check_ragged_shape(const fa_ragged_shape *s, int maps) {
@@ -42,7 +42,7 @@ inline fa_status check_ragged_shape(const fa_ragged_shape *s, int maps) {
                 s->num_heads, s->num_kv_heads, kMaxGroup);
   if ((int64_t)s->max_blocks_per_seq * s->block_size > 0x3fffffffLL)
     return fail(FA_ERR_BAD_SHAPE, "a block table of 2^30 tokens or more is not supported");
-  // the rows form numbers 128-key units of the whole batch, the tile form 16-row pieces of its grid
+  // the rows form numbers 128-key units, the tile form 16-row pieces of its grid
   const int64_t keys = (int64_t)s->max_blocks_per_seq * s->block_size;
   if ((int64_t)s->num_seqs * s->num_kv_heads * (keys / kRowUnit + 2) > 0x7fffffffLL ||
       ((int64_t)s->num_tokens + s->num_seqs) * s->num_heads > 0x7fffffffLL)
@@ -71,32 +71,24 @@ inline RaggedPlan ragged_plan(const fa_ragged_shape &s, int maps, int cus) {
     return here;
   };
   if (r.rows) {
-#ifndef FORCE_ALIGNED
-#define FORCE_ALIGNED 512
-#endif
-    r.row_aligned = keys <= FORCE_ALIGNED;
-    r.row_groups = (int)std::min<int64_t>({2 * (int64_t)cus, kMaxRowGroups, S * Hk * (keys / kRowUnit + 2)});
+    r.row_aligned = keys <= 512;
+    r.row_groups = (int)std::min<int64_t>(2 * (int64_t)cus, kMaxRowGroups);
     if (!r.row_aligned) {
-      const int64_t slots = S * Hk + r.row_groups;
+      r.row_shares = std::max<int>(1, r.row_groups / (int)Hk);
+      const int64_t slots = (S + r.row_shares) * Hk;
       r.row_o = take(slots * kRowColumns * D * 4);
       r.row_ml = take(slots * 2 * kRowColumns * 4);
-      r.row_items = take(S * Hk * 8);
+      r.row_seqs = take(S * 8);
     }
   }
   if (r.tiles) {
     // 8 wavefronts halve what K and V cost per row; sequences that cannot fill them take 4
     r.wavefronts = most * G * maps <= 128 ? 4 : 8;
-#ifdef FORCE_NW
-    r.wavefronts = FORCE_NW;
-#endif
     r.tile_rows = r.wavefronts * 32 / maps;
     const int64_t each = (most * G + r.tile_rows - 1) / r.tile_rows;
     r.tile_bound = equal ? S * each : std::min(S * each, T * G / r.tile_rows + S);
     const int64_t resident = (int64_t)cus * (r.wavefronts == 4 ? 2 : 1);
-#ifndef FORCE_LINE
-#define FORCE_LINE 2
-#endif
-    if (r.tile_bound * Hk < FORCE_LINE * resident) {
+    if (r.tile_bound * Hk < 2 * resident) {
       r.tile_groups = (int)std::max<int64_t>(8, resident / 8 * 8);  // (an eighth of the shares for each XCC)
       r.tile_o = take(2 * (int64_t)r.tile_groups * r.wavefronts * D * 32 * 4);
       r.tile_ml = take(2 * (int64_t)r.tile_groups * r.wavefronts * 128 * 4);
@@ -140,7 +132,7 @@ inline fa_status launch_ragged_kernels(const RaggedParams &p, const RaggedPlan &
     }
   }
   if (plan.rows) {
-    const unsigned groups = plan.row_aligned ? (unsigned)(p.b.num_seqs * Hk) : (unsigned)plan.row_groups;
+    const unsigned groups = plan.row_aligned ? (unsigned)(p.b.num_seqs * Hk) : (unsigned)(plan.row_shares * Hk);
     FA_HIP_CHECK(timer.launch(ragged_rows_kernel<D, OT, KVF, MAPS>, dim3(groups), dim3(256), 0, p));
     if ((st = timed()) != FA_OK || plan.row_aligned) return st;
     const int rows = std::min<int64_t>(kRowColumns / MAPS, (int64_t)p.max_query_len * p.group);
@@ -262,7 +254,8 @@ inline fa_status launch_ragged_attention(void *out, const void *query, const voi
   p.row_aligned = plan.row_aligned;
   p.row_o = reinterpret_cast<float *>(space + plan.row_o);
   p.row_ml = reinterpret_cast<float *>(space + plan.row_ml);
-  p.row_items = reinterpret_cast<int2 *>(space + plan.row_items);
+  p.row_seqs = reinterpret_cast<int2 *>(space + plan.row_seqs);
+  p.row_shares = plan.row_shares;
   p.tile_groups = plan.tile_groups;
   p.tile_o = reinterpret_cast<float *>(space + plan.tile_o);
   p.tile_ml = reinterpret_cast<float *>(space + plan.tile_ml);

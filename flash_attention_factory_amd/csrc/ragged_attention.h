@@ -38,11 +38,12 @@ struct RaggedParams {
   const float *norm_weight;
   float norm_eps, out_scale;
   // rows form: work-groups, and their partial results
-  int32_t row_groups;           // at most kMaxRowGroups
+  int32_t row_groups;           // work-groups that the chip holds, at most kMaxRowGroups
+  int32_t row_shares;           // shares of the line at most, each for the work-groups of all kv heads
   int32_t row_aligned;          // a work-group for each item instead: nothing is cut, nothing merged
   float *row_o;                 // [slot][16][D]
   float *row_ml;                // [slot][2][16]: maxima (base-2 units), sums
-  int2 *row_items;              // [seq * kv heads + kv head]: first and last work-group of the item
+  int2 *row_seqs;               // first and last share of a sequence
   // tile form
   int32_t tile_groups;          // > 0: work-groups that share the line of tiles; 0: a work-group for each tile
   float *tile_o;                // [2 * work-group + (0: its first piece, 1: a later one)]: registers of its wavefronts

@@ -1,11 +1,17 @@
 // Ragged paged attention, rows form: at most 16 rows (new token, query head, map) per (sequence, kv head), the 16 columns of an
-// MFMA tile; bound by the bytes of K and V.
+// MFMA tile; bound by the bytes of K and V.  Measured on an MI355X: 2.0 GB of integer K and V (500 000 keys of 48 sequences, 8 kv
+// heads) 350 us, 5.8 TB/s; 0.37 GB of 16-bit ones (48 sequences, 8 kv heads, two maps) 65 us, 5.7 TB/s; a single sequence of
+// 30 000 keys and 4 kv heads (62 MB) 20 us, of which 5 are the two launches and 3 the second kernel.
 //
-// Split of the work: the keys of every (sequence, kv head) are cut into units of 128 and all units of the batch are laid end to end;
-// the resident work-groups take equal shares of that line, whatever the lengths of the sequences are.  A share may end within an item
-// (sequence, kv head); its piece of the item goes to the workspace as an unnormalised sum with its maximum, in slot
-// item + work-group (both only grow along the line, so no two pieces meet), and ragged_rows_merge_kernel joins the pieces in their
-// order.  No atomics: results do not vary from run to run.
+// Split of the work: the keys of every sequence are cut into units of 128 and the units of all sequences are laid end to end; that
+// line is cut into equal shares, whatever the lengths of the sequences are, and the work-groups of all kv heads take the same
+// shares.  Those lie next to each other and go through the same blocks at the same time, whose K, V and scales lie side by side
+// in the pool: shares that end at other keys from head to head took 361 us instead of 350 (and 68 instead of 65) above, and heads
+// one after the other, all sequences each, up to 1.5 times as long.  A share may end within a sequence; its piece goes
+// to the workspace as an unnormalised sum with its maximum (row_slot), and ragged_rows_merge_kernel joins the pieces in
+// their order.  No atomics: results do not vary from run to run.
+// Calls with at most 512 keys take a work-group for each (sequence, kv head) instead, without a second kernel: one sequence of 200
+// keys 7.4 us and 10.7 with shares, 400 keys 9.7 and 10.7, 700 keys 12.4 and 10.5.
 //
 // Within a unit each of the four wavefronts takes 32 keys (WaveAttn: operands straight from the pool, no LDS) and keeps a softmax
 // state of its own; the states merge through LDS at the end of a piece.
@@ -25,10 +31,11 @@ struct RowState {
   float m, mt, l, mv, mvt;
 };
 
-// Multipliers of a chunk's two 16-key tiles.
+// Multipliers of a chunk's 16-key tiles.
+template <int TILES>
 struct RowScales {
-  float k[2];   // raw score -> base-2 units, without the column's own factor
-  float lv[2];  // log2 of the V scale
+  float k[TILES];   // raw score -> base-2 units, without the column's own factor
+  float lv[TILES];  // log2 of the V scale
 };
 
 template <typename W>
@@ -39,11 +46,11 @@ struct RowColumns {
   int vis_lo, vis_hi;  // keys that every column sees
 };
 
-template <bool KV8, typename W>
+template <bool KV8, typename W, int TILES>
 __device__ __forceinline__ typename W::Probs row_soft(W &wa, RowState &st, const RowColumns<W> &col, typename W::Chunk &R,
-                                                      const typename W::Scores &s, const RowScales &sc, int ci, int ctx,
+                                                      const typename W::Scores &s, const RowScales<TILES> &sc, int ci, int ctx,
                                                       const RaggedParams &p) {
-  constexpr int NT = 8;
+  constexpr int NT = 4 * TILES;
   float t[NT];
 #pragma unroll
   for (int e = 0; e < NT; ++e) t[e] = s.v[e >> 2][e & 3] * (sc.k[e >> 2] * col.mul);
@@ -67,10 +74,13 @@ __device__ __forceinline__ typename W::Probs row_soft(W &wa, RowState &st, const
       }
     }
   }
-  float mx[2];
+  float mx[TILES];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) mx[h] = fmaxf(fmaxf(t[4 * h], t[4 * h + 1]), fmaxf(t[4 * h + 2], t[4 * h + 3]));
-  st.mt = fmaxf(st.mt, rows_max(fmaxf(mx[0], mx[1])));
+  for (int h = 0; h < TILES; ++h) mx[h] = fmaxf(fmaxf(t[4 * h], t[4 * h + 1]), fmaxf(t[4 * h + 2], t[4 * h + 3]));
+  float top = mx[0];
+#pragma unroll
+  for (int h = 1; h < TILES; ++h) top = fmaxf(top, mx[h]);
+  st.mt = fmaxf(st.mt, rows_max(top));
   const bool blocks = KV8 && p.block_scales;
   if (__builtin_expect(__any(st.mt - st.m > kRefresh), 0)) {
     const float to = st.mt - kHeadroom;
@@ -91,7 +101,10 @@ __device__ __forceinline__ typename W::Probs row_soft(W &wa, RowState &st, const
   }
   st.l += sum;
   if (blocks) {
-    st.mvt = fmaxf(st.mvt, rows_max(fmaxf(mx[0] + sc.lv[0], mx[1] + sc.lv[1])));
+    float top_v = mx[0] + sc.lv[0];
+#pragma unroll
+    for (int h = 1; h < TILES; ++h) top_v = fmaxf(top_v, mx[h] + sc.lv[h]);
+    st.mvt = fmaxf(st.mvt, rows_max(top_v));
     if (__builtin_expect(__any(st.mvt - st.mv > kRefresh), 0)) {
       const float to = st.mvt - kHeadroom;
       const float alpha = st.mv == -INFINITY ? 0.f : fast_exp2(st.mv - to);
@@ -100,7 +113,7 @@ __device__ __forceinline__ typename W::Probs row_soft(W &wa, RowState &st, const
       st.mv = to;
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < TILES; ++h) {
       // (cut so that a weight of 0 stays 0 where the factor would overflow)
       const float f = st.mv == -INFINITY ? 0.f : fast_exp2(fminf(sub + sc.lv[h] - st.mv, 126.0f));
 #pragma unroll
@@ -109,15 +122,32 @@ __device__ __forceinline__ typename W::Probs row_soft(W &wa, RowState &st, const
   }
   typename W::Probs pb;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) pb.v[0][c] = pack2<typename W::Operand>(t[2 * c], t[2 * c + 1]);
+  for (int c = 0; c < 2 * TILES; ++c) pb.v[c >> 2][c & 3] = pack2<typename W::Operand>(t[2 * c], t[2 * c + 1]);
   return pb;
+}
+
+// Shares that the line of `total` units is cut into.  Up to 3/2 of the compute units' number, a unit each: 320 units of integers
+// 11.2 us, and 13.3 with a work-group for each compute unit.  Then one for each compute unit, since pieces cost more than a second
+// work-group brings, until there are 6 units for each (12 of 16-bit pools), and two from there on: 1008 units of integers 14.5 us
+// with one and 15.0 with two, 1536 16.9 and 15.4, 4032 29.4 and 27.7; of 16-bit pools 940 units 19.5 and 21.3, 5800 70.8 and 68.2.
+template <bool KV8>
+__device__ __forceinline__ int row_shares(const RaggedParams &p, int32_t total) {
+  const int64_t all = (int64_t)total * p.num_kv_heads;
+  const int most = p.row_groups, half = (most + 1) >> 1;
+  const int groups = all <= half + (half >> 1) || all >= (KV8 ? 6 : 12) * half ? most : half;
+  return min(total, max(1, groups / p.num_kv_heads));
+}
+// Where a share's piece of an item lies: both sequences and shares only grow along the line, so no two pieces meet.
+__device__ __forceinline__ int64_t row_slot(const RaggedParams &p, int kvh, int seq, int share) {
+  return (int64_t)kvh * (p.b.num_seqs + p.row_shares) + seq + share;
 }
 
 template <int D, typename OT, int KVF, int MAPS>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ragged_rows_kernel(const RaggedParams p) {
   constexpr bool KV8 = KVF != kKv16;
   constexpr int NW = 4;
-  using W = WaveAttn<D, OT, KVF, 2, Pipeline<KV8>::stream_loads_loop, false, true>;
+  constexpr int TILES = 2;
+  using W = WaveAttn<D, OT, KVF, TILES, Pipeline<KV8>::stream_loads_loop, false, true>;
   constexpr int NR = W::NR, NDT = W::NDT, SL = NR / NW;
   static_assert(W::CT * NW == kRowUnit, "a unit is one chunk per wavefront");
   __shared__ float lds[NW * (NR * 64 + 32)];
@@ -139,20 +169,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
                               __builtin_amdgcn_readlane(of_lane.ctx, s)}
                   : ragged_seq_uniform(p.b, s);
   };
-  const int g = blockIdx.x;
-  int32_t total = 0, u, u_end, before = 0;
-  int groups = 0, seq;
+  int32_t total = 0, u, u_end, before = 0;  // units of the line, this share of it, units before the sequence's own
+  int shares = 0, share = 0, seq, kvh;
   if (p.row_aligned) {  // one work-group per item
-    seq = g / Hk;
-    const int units = row_units<MAPS>(p, seq_at(seq));
-    u = (g - seq * Hk) * units;
-    u_end = u + units;
+    seq = blockIdx.x / Hk;
+    kvh = blockIdx.x - seq * Hk;
+    u = 0;
+    u_end = row_units<MAPS>(p, seq_at(seq));
     const RaggedSeq q = ragged_seq_cut(p, seq_at(seq));
-    if (units == 0) {  // no keys: zeros
+    if (u_end == 0) {  // no keys: zeros
       if (q.n > 0 && in_rows_form<MAPS>(p, q))
         for (int k = threadIdx.x; k < q.n * G * (D / 8); k += 256) {
           const int row = k / (D / 8), j = row / G;
-          *reinterpret_cast<u32x4 *>(p.out + (((int64_t)(q.first + j) * p.num_heads + (g - seq * Hk) * G + (row - j * G)) * D + (k % (D / 8)) * 8) * 2) =
+          *reinterpret_cast<u32x4 *>(p.out + (((int64_t)(q.first + j) * p.num_heads + kvh * G + (row - j * G)) * D + (k % (D / 8)) * 8) * 2) =
               u32x4{0u, 0u, 0u, 0u};
         }
       return;
@@ -165,18 +194,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
       for (int s = 64 + lane; s < p.b.num_seqs; s += 64) more += row_units<MAPS>(p, ragged_seq_of_lane(p.b, s));
       total += __builtin_amdgcn_readlane(wave_inclusive_scan(more, lane), 63);
     }
-    total *= Hk;
-    groups = min(p.row_groups, total);
-    if (g >= groups) return;
-    u = (int32_t)((int64_t)total * g / groups);
-    u_end = (int32_t)((int64_t)total * (g + 1) / groups);
-    const unsigned long long beyond = __ballot(upto * Hk > u);
+    shares = row_shares<KV8>(p, total);
+    share = blockIdx.x / Hk;
+    kvh = blockIdx.x - share * Hk;
+    if (share >= shares) return;
+    u = (int32_t)((int64_t)total * share / shares);
+    u_end = (int32_t)((int64_t)total * (share + 1) / shares);
+    const unsigned long long beyond = __ballot(upto > u);
     if (beyond) {
       seq = __builtin_ctzll(beyond);
-      before = (__builtin_amdgcn_readlane(upto, seq) - __builtin_amdgcn_readlane(units_of_lane, seq)) * Hk;
+      before = __builtin_amdgcn_readlane(upto, seq) - __builtin_amdgcn_readlane(units_of_lane, seq);
     } else {
-      const RaggedPlace at = ragged_find(p.b.num_seqs, u, lane,
-                                         [&](int s) { return row_units<MAPS>(p, ragged_seq_of_lane(p.b, s)) * Hk; });
+      const RaggedPlace at = ragged_find(p.b.num_seqs, u, lane, [&](int s) { return row_units<MAPS>(p, ragged_seq_of_lane(p.b, s)); });
       seq = __builtin_amdgcn_readfirstlane(at.seq);
       before = __builtin_amdgcn_readfirstlane(at.before);
     }
@@ -184,19 +213,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
 
   W wa(p.a, lane);
   const int r = wa.r, i = wa.i;
-  while (u < u_end) {
+  do {
+    // (a loop of its own, so that no way to the end of this one joins a branch on lanes: `seq` stays known to be the same for
+    // the wavefront.  Where it is not, block ids and scales come with vector loads, and every one of those waits for all of K and V)
     RaggedSeq q = ragged_seq_cut(p, seq_at(seq));
-    const int units = row_units<MAPS>(p, q);
-    if (u >= before + units * Hk) {
-      before += units * Hk;
+    int units = row_units<MAPS>(p, q);
+    while (u >= before + units && seq + 1 < p.b.num_seqs) {
+      before += units;
       ++seq;
-      continue;
+      q = ragged_seq_cut(p, seq_at(seq));
+      units = row_units<MAPS>(p, q);
     }
-    const int kvh = p.row_aligned ? g - seq * Hk : (u - before) / units;
-    const int first = (u - before) - kvh * units;
+    const int first = min(u - before, units);
     const int last = min(units, first + (u_end - u));
-    const int item = seq * Hk + kvh;
-    u += last - first;
+    u += max(last - first, 1);
     const int base_unit = first_key(p, q) / kRowUnit;
     const int tok_begin = (base_unit + first) * kRowUnit, tok_end = min(q.ctx, (base_unit + last) * kRowUnit);
     const int32_t *table = p.b.block_tables + (int64_t)seq * p.b.max_blocks_per_seq;
@@ -206,9 +236,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
 
     // block scales of a chunk; tiles past the context take 1, whatever the block that their id names holds
     auto fetch_scales = [&](const typename W::Ids &ids, int c) {
-      RowScales x;
+      RowScales<TILES> x;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < TILES; ++t) {
         x.k[t] = p.score_scale_log2;
         x.lv[t] = 0.f;
         if constexpr (KV8) {
@@ -261,7 +291,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
       typename W::Ids ids = wa.fetch_ids(table, ci, last_col);
       wa.issue_k(R, kvh, ci, ids);
       wa.issue_v(R, kvh, ci, ids);
-      RowScales sc = fetch_scales(ids, ci), nsc = sc;
+      RowScales<TILES> sc = fetch_scales(ids, ci), nsc = sc;
       ids = wa.fetch_ids(table, ci + NW, last_col);
       if (KV8 && p.q_bf16) {
         float most = 0.f;
@@ -361,7 +391,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
           for (int k = 0; k < SL; k += 2) *reinterpret_cast<uint32_t *>(dst + 2 * k) = pack_out(p, o[k] * w[k], o[k + 1] * w[k + 1]);
         }
       } else {
-        const int64_t slot = (int64_t)item + g;
+        const int64_t slot = row_slot(p, kvh, seq, share);
         if (valid) {
           float *dst = p.row_o + (slot * kRowColumns + i) * D + d0;
 #pragma unroll
@@ -373,12 +403,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
           p.row_ml[slot * 2 * kRowColumns + kRowColumns + i] = L;
         }
       }
-      if (first == 0 && threadIdx.x == 0 && !p.row_aligned) {  // the work-groups that hold the item's pieces
-        const int64_t end = (int64_t)before + (int64_t)kvh * units + units;
-        p.row_items[item] = int2{g, (int)((end * groups - 1) / total)};
-      }
+      if (first == 0 && kvh == 0 && threadIdx.x == 0 && !p.row_aligned)  // the shares that hold the sequence's pieces
+        p.row_seqs[seq] = int2{share, (int)((((int64_t)before + units) * shares - 1) / total)};
     }
-  }
+  } while (u < u_end);
 }
 
 // Joins the pieces of an item's rows.  Work-group (item, row): the pieces' maxima first, in LDS as factors; then the eight wavefronts
@@ -386,21 +414,21 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
 template <int D, int MAPS>
 __global__ void __launch_bounds__(512) ragged_rows_merge_kernel(const RaggedParams p) {
   constexpr int N = D / 64, NW = 8, kAhead = 4;
-  __shared__ float factor[MAPS][kMaxRowGroups];
+  __shared__ float factor[MAPS][kMaxRowGroups], ls[MAPS][kMaxRowGroups];
   __shared__ float sm[MAPS][NW][N][64], tops[MAPS][NW], sums[MAPS][NW];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int item = blockIdx.x, row = blockIdx.y;
   const int seq = item / p.num_kv_heads, kvh = item - seq * p.num_kv_heads;
   // (not set where the item has no keys; asked for with the lengths)
-  const int first = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_items + item));
-  const int last = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_items + item) + 1);
+  const int first = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_seqs + seq));
+  const int last = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_seqs + seq) + 1);
   const RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq));
   if (row >= q.n * p.group || !in_rows_form<MAPS>(p, q)) return;
   const int j = row / p.group, head = kvh * p.group + (row - j * p.group);
   const int pieces = row_units<MAPS>(p, q) > 0 ? last - first + 1 : 0;
   if (pieces == 1) return;  // the rows kernel has stored the result
-  const int64_t slot0 = (int64_t)item + first;
+  const int64_t slot0 = row_slot(p, kvh, seq, first);
   float o[MAPS][N] = {};
   if (pieces > 0) {
     float early[MAPS][kAhead][N];  // the first pieces' values, asked for before the factors are known
@@ -413,16 +441,15 @@ __global__ void __launch_bounds__(512) ragged_rows_merge_kernel(const RaggedPara
 #pragma unroll
         for (int k = 0; k < N; ++k) early[m][u][k] = src[k];
       }
-    float l_of[MAPS];
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
       float top = -INFINITY;
-      l_of[m] = 0.f;
-      for (int x = threadIdx.x; x < pieces; x += 512) {  // (no more than 512 pieces: once)
+      for (int x = threadIdx.x; x < pieces; x += 512) {
         const float *ml = p.row_ml + (slot0 + x) * 2 * kRowColumns + row * MAPS + m;
-        top = ml[0];
-        l_of[m] = ml[kRowColumns];
-        factor[m][x] = top;
+        const float pm = ml[0];
+        factor[m][x] = pm;
+        ls[m][x] = ml[kRowColumns];
+        top = fmaxf(top, pm);
       }
       top = wave_max(top);
       if (lane == 0) tops[m][wave] = top;
@@ -438,7 +465,7 @@ __global__ void __launch_bounds__(512) ragged_rows_merge_kernel(const RaggedPara
       for (int x = threadIdx.x; x < pieces; x += 512) {
         const float f = fast_exp2(factor[m][x] - sub);
         factor[m][x] = f;
-        l = f * l_of[m];
+        l += f * ls[m][x];
       }
       l = wave_sum(l);
       if (lane == 0) sums[m][wave] = l;
