@@ -44,6 +44,7 @@ struct RowColumns {
   float slope_log2;
   int pos;           // position of the column's token
   int vis_lo, vis_hi;  // keys that every column sees
+  int first;         // before it: keys that no column sees
 };
 
 template <bool KV8, typename W, int TILES>
@@ -68,7 +69,7 @@ __device__ __forceinline__ typename W::Probs row_soft(W &wa, RowState &st, const
     for (int e = 0; e < NT; ++e) {
       const int tok = t0 + (e >> 2) * 16 + 4 * wa.r + (e & 3);
       if (tok > col.pos || tok < col.pos - p.window) t[e] = -INFINITY;  // select: the pool may hold NaN there
-      if (tok >= ctx) {
+      if (tok >= ctx || tok < col.first) {
 #pragma unroll
         for (int w = 0; w < W::VW; ++w) R.v[e][w] = 0u;
       }
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
     int ci = tok_begin / W::CT + wave;
     const int c_end = (tok_end + W::CT - 1) / W::CT;
 
-    // block scales of a chunk; tiles past the context take 1, whatever the block that their id names holds
+    // block scales of a chunk; tiles that no column sees take 1, whatever the block that their id names holds
     auto fetch_scales = [&](const typename W::Ids &ids, int c) {
       RowScales<TILES> x;
 #pragma unroll
@@ -246,7 +247,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
             x.k[t] *= p.tensor_scale;
           } else {
             const int64_t idx = (int64_t)ids.v[t] * p.scale_pitch + kvh;
-            const bool there = c * W::CT + t * 16 < q.ctx;
+            const int tok = c * W::CT + t * 16;
+            const bool there = tok < q.ctx && tok + 15 >= first_key(p, q);
             const float ks = load_uniform_f32(p.k_scales + idx), vs = load_uniform_f32(p.v_scales + idx);
             x.k[t] = there ? x.k[t] * ks : x.k[t];
             x.lv[t] = there && p.block_scales ? __builtin_amdgcn_logf(vs) : 0.f;
@@ -266,6 +268,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
     col.pos = q.ctx - q.n + j;
     col.vis_hi = q.ctx - q.n;
     col.vis_lo = q.ctx - 1 - p.window;
+    col.first = first_key(p, q);
     col.slope_log2 = (p.mask_flags & kMaskAlibi) && valid ? p.alibi_slopes[head] * kLog2e : 0.f;
     const char *qrow = p.query + (int64_t)(q.first + (valid ? j : 0)) * p.q_token_bytes + (valid ? head : 0) * p.q_head_bytes;
     u32x4 qv[W::KSTEPS];

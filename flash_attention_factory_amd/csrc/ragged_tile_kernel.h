@@ -428,6 +428,8 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const bool loads = T::kRowsPerPass <= kTileKeys || load_row < kTileKeys;
   const int last_col = p.b.max_blocks_per_seq - 1, in_block = (1 << p.b.block_shift) - 1;
   const int steps = step_end - step;
+  const int seen_lo = max(0, pos0 + row0 / G - p.window);  // keys that some row of the tile sees
+  const int seen_keys = pos0 + (min(row0 + T::kRows, all_rows) - 1) / G + 1 - seen_lo;
   // Blocks of this thread's rows: of the next step of K as the table has them (cut to the pool where they are used, since
   // arithmetic here would wait for the load, and for every load before it), and of the next step of V, one step behind.
   int32_t kid[T::kPasses], vid[T::kPasses];
@@ -487,7 +489,8 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   };
   auto write_v = [&](int n, int w) {
     const int pass = KV8 ? w >> 1 : w, key = pass * T::kRowsPerPass + load_row;
-    if ((step + n) * kTileKeys + key >= q.ctx) vreg[pass] = u32x4{0u, 0u, 0u, 0u};  // what lies there may be NaN
+    // what no row of the tile sees may be NaN
+    if ((uint32_t)((step + n) * kTileKeys + key - seen_lo) >= (uint32_t)seen_keys) vreg[pass] = u32x4{0u, 0u, 0u, 0u};
     const u32x4 o = lds_piece(vreg[pass], w);
     if (loads) *reinterpret_cast<u32x4 *>(lds + (2 + (n & 1)) * T::kBufferBytes + T::v_at(key, KV8 ? 2 * piece + (w & 1) : piece)) = o;
   };
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   };
 
   // Scales of a step's four groups of 16 keys (a group lies within a block): lanes 0 to 3 fetch those of K, 4 to 7 those of V, the
-  // block ids two steps ahead, the scales one step ahead, both left as they come until they are used.  Groups past the context
+  // block ids two steps ahead, the scales one step ahead, both left as they come until they are used.  Groups that no row sees
   // take 1.
   // Byte pools without scales of blocks go the same way, with scales of 1 (log2: 0).
   constexpr bool blocks = KV8;
@@ -521,7 +524,8 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   };
   auto take_scales = [&](int n) {
     if constexpr (!KV8) return;
-    const float s = scaled && (step + n) * kTileKeys + group_key < q.ctx ? scale_raw : 1.f;
+    const int key = (step + n) * kTileKeys + group_key;
+    const float s = scaled && key < seen_lo + seen_keys && key + 15 >= seen_lo ? scale_raw : 1.f;
     const float log = p.block_scales ? __builtin_amdgcn_logf(s) : 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -798,8 +802,9 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
     tile = 0;
     if (++kvh == Hk) {
       kvh = 0;
-      do ++seq;
-      while (row_tiles<MAPS, T::kRows>(p, ragged_seq_uniform(p.b, seq)) == 0);
+      do {
+        if (++seq >= p.b.num_seqs) return;  // (not while the arrays stay as they are)
+      } while (row_tiles<MAPS, T::kRows>(p, ragged_seq_uniform(p.b, seq)) == 0);
     }
   }
   }

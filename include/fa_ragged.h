@@ -19,6 +19,10 @@
  * A context beyond what the table row holds is cut to that; block ids outside the pool are never
  * read from or written to (reads take a block of the pool instead, writes are left out); a token
  * at a negative position (context_lens[s] < n) is not stored and its result is zero.
+ * Pool rows that none of the call's tokens sees -- past the context, before every token's window,
+ * unused blocks -- and scales of such blocks may hold anything.  Keys that a token does not see
+ * have no weight whatever they are; values of one token that are infinite or NaN can reach earlier new
+ * tokens of the same call, whose weight for them is zero, as products of zero.
  *
  * Pools are addressed as in fa_paged_attention.h.  Nothing but kernel launches is put on
  * options->stream unless options->elapsed_us is given.  No exception crosses this boundary.
