@@ -82,13 +82,23 @@ inline RaggedPlan ragged_plan(const fa_ragged_shape &s, int maps, int cus) {
     }
   }
   if (r.tiles) {
-    // 8 wavefronts halve what K and V cost per row; sequences that cannot fill them take 4
-    r.wavefronts = most * G * maps <= 128 ? 4 : 8;
+    // 8 wavefronts halve what K and V cost per row, and take turns in the matrix phase; 4 start and end a tile sooner, and two
+    // such work-groups share a compute unit.  4 where rows do not fill more or keys are few: one prompt of 1000 tokens (8 kv heads, 4
+    // query heads each, integers) 33 us with 4, 40 with 8; 16 such 230 and 239; 64 new tokens of 16 sequences of 1000 keys
+    // 37 and 45; 8 prompts of 2000 tokens 371 and 357; of 3000 763 and 725; 300 new tokens of 64 sequences of 2300 keys 927 and 864.
+    r.wavefronts = most * G * maps <= 128 || keys <= 1536 ? 4 : 8;
     r.tile_rows = r.wavefronts * 32 / maps;
     const int64_t each = (most * G + r.tile_rows - 1) / r.tile_rows;
     r.tile_bound = equal ? S * each : std::min(S * each, T * G / r.tile_rows + S);
-    const int64_t resident = (int64_t)cus * (r.wavefronts == 4 ? 2 : 1);
-    if (r.tile_bound * Hk < 2 * resident) {
+    // Tiles for each compute unit: from two on, a work-group each, longest first, keeps them all busy.  With fewer, the longest
+    // tile (or two one after the other) leaves compute units idle for so many keys; shares of a line do not, but cost a second
+    // kernel and their bookkeeping, about what 20 steps take: 20 new tokens of one sequence of 8000 keys 65 us as shares, 196 as
+    // tiles, of 2000 keys 36 and 56, of 4 sequences of 1000 keys 37 and 31; 64 of 8 sequences of 4000 keys 76 and 133; two prompts
+    // of 2000 tokens 123 and 94.
+    const double x = (double)(r.tile_bound * Hk) / cus, mean = std::max<double>(keys - most / 2, 0);
+    const bool line = x < 2 && std::max<double>(keys, x > 1 ? 2 * mean : mean) - x * mean > 20 * kTileKeys;
+    if (line) {
+      const int64_t resident = (int64_t)cus * (r.wavefronts == 4 ? 2 : 1);
       r.tile_groups = (int)std::max<int64_t>(8, resident / 8 * 8);  // (an eighth of the shares for each XCC)
       r.tile_o = take(2 * (int64_t)r.tile_groups * r.wavefronts * D * 32 * 4);
       r.tile_ml = take(2 * (int64_t)r.tile_groups * r.wavefronts * 128 * 4);

@@ -94,7 +94,7 @@ struct RaggedTile {
 // kTileStart for what a tile costs apart from them.  Within a sequence the cost grows by the same amount from tile to
 // tile (the causal rule), so sums and places have closed forms.  Work-group g takes the part from total * g / groups
 // to total * (g + 1) / groups: equal shares, whatever the lengths are.  A cut within a tile becomes a cut between two steps.
-// Measured against one work-group per tile, the longest of a sequence first (the card has 256 compute units): see the launcher.
+// When this is done rather than one work-group per tile, longest first: ragged_plan, with both sides measured.
 constexpr int kTileStart = 3 * kTileKeys;
 constexpr int kLeastShare = 4 * kTileKeys;  // no shares smaller than that
 

@@ -12,12 +12,12 @@ from test_gpu_ragged_attention import _close, _differential, _pools, _query, _ra
 
 pytestmark = pytest.mark.gpu
 
-# Sequences and heads whose tiles are more than twice what 256 compute units hold: a work-group for each tile.
+# Sequences and heads with two tiles and more for each of 256 compute units: a work-group for each tile.
 GRIDS = {
     "four_wavefronts_many_sequences": (R.Batch([20] * 130 + [0, 3], [(k * 29) % 150 for k in range(132)], B=16), 16, 8),
     "four_wavefronts": (R.Batch([30 - k % 3 for k in range(64)], [(k * 29) % 150 for k in range(64)], B=16), 64, 16),
-    "eight_wavefronts": (R.Batch([33, 0, 40] + [37] * 40, [(k * 29) % 150 for k in range(43)], B=16), 64, 8),
-    "eight_wavefronts_many_sequences": (R.Batch([65] * 66, [(k * 29) % 150 for k in range(66)], B=16), 32, 8),
+    "eight_wavefronts": (R.Batch([33, 0, 40] + [37] * 40, [1600] + [(k * 29) % 150 for k in range(42)], B=16), 64, 8),
+    "eight_wavefronts_many_sequences": (R.Batch([65] * 66, [(k * 29) % 150 for k in range(65)] + [1700], B=16), 32, 8),
 }
 
 
