@@ -146,7 +146,11 @@ inline fa_status launch_ragged_kernels(const RaggedParams &p, const RaggedPlan &
     FA_HIP_CHECK(timer.launch(ragged_rows_kernel<D, OT, KVF, MAPS>, dim3(groups), dim3(256), 0, p));
     if ((st = timed()) != FA_OK || plan.row_aligned) return st;
     const int rows = std::min<int64_t>(kRowColumns / MAPS, (int64_t)p.max_query_len * p.group);
-    FA_HIP_CHECK(timer.launch(ragged_rows_merge_kernel<D, MAPS>, dim3((unsigned)(p.b.num_seqs * Hk), (unsigned)rows), dim3(512), 0, p));
+    const int64_t items = (int64_t)p.b.num_seqs * Hk;
+    if (items * rows > 8 * (int64_t)plan.row_groups)  // four times what the chip holds at a time: see the second kernel
+      FA_HIP_CHECK(timer.launch(ragged_rows_join_kernel<D, MAPS>, dim3((unsigned)items), dim3(512), 0, p));
+    else
+      FA_HIP_CHECK(timer.launch(ragged_rows_merge_kernel<D, MAPS>, dim3((unsigned)items, (unsigned)rows), dim3(512), 0, p));
     if ((st = timed()) != FA_OK) return st;
   }
   return FA_OK;

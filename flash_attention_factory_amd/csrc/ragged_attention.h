@@ -62,6 +62,18 @@ constexpr int kNoWindow = 0x3fffffff;
 // instead of 2^-14.  Sums and accumulators are 32 bits wide.
 constexpr float kHeadroom = 6.0f, kRefresh = 14.0f;
 
+// Two maps over 16-bit values: weights go to the matrix cores in two parts, the rounded ones and what the rounding left.  The
+// difference of the maps, normalised, is smaller than either, and the rounding of the weights showed in it: with bf16 the
+// result's error was 0.0024 of its norm, with fp16 0.00030, where rounding the result alone makes 0.0016 and 0.0002.
+template <int KVF, int MAPS>
+constexpr bool two_parts() {
+  return MAPS == 2 && KVF == kKv16;
+}
+template <typename OT>
+__device__ __forceinline__ uint32_t rest_of_pair(uint32_t rounded, float lo, float hi) {
+  return pack2<OT>(lo - f32_from_half_of<OT>(rounded, 0), hi - f32_from_half_of<OT>(rounded, 1));
+}
+
 __device__ __forceinline__ RaggedSeq ragged_seq_cut(const RaggedParams &p, RaggedSeq q) {
   q.n = min(q.n, p.max_query_len);
   return q;

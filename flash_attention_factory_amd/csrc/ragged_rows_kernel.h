@@ -1,6 +1,6 @@
 // Ragged paged attention, rows form: at most 16 rows (new token, query head, map) per (sequence, kv head), the 16 columns of an
-// MFMA tile; bound by the bytes of K and V.  Measured on an MI355X: 2.0 GB of integer K and V (500 000 keys of 48 sequences, 8 kv
-// heads) 350 us, 5.8 TB/s; 0.37 GB of 16-bit ones (48 sequences, 8 kv heads, two maps) 65 us, 5.7 TB/s; a single sequence of
+// MFMA tile; bound by the bytes of K and V.  Measured on an MI355X: 2.0 GB of integer K and V (990 000 keys of 128 sequences, 8 kv
+// heads) 344 us, 5.9 TB/s; 0.37 GB of 16-bit ones (32 sequences, 8 kv heads, two maps) 65 us, 5.7 TB/s; a single sequence of
 // 30 000 keys and 4 kv heads (62 MB) 20 us, of which 5 are the two launches and 3 the second kernel.
 //
 // Split of the work: the keys of every sequence are cut into units of 128 and the units of all sequences are laid end to end; that
@@ -47,8 +47,14 @@ struct RowColumns {
   int first;         // before it: keys that no column sees
 };
 
-template <bool KV8, typename W, int TILES>
-__device__ __forceinline__ typename W::Probs row_soft(W &wa, RowState &st, const RowColumns<W> &col, typename W::Chunk &R,
+// Weights as operands of the matrix cores, and what their rounding left (of use with two parts, see two_parts).
+template <typename W>
+struct RowWeights {
+  typename W::Probs top, rest;
+};
+
+template <bool KV8, bool TWO, typename W, int TILES>
+__device__ __forceinline__ RowWeights<W> row_soft(W &wa, RowState &st, const RowColumns<W> &col, typename W::Chunk &R,
                                                       const typename W::Scores &s, const RowScales<TILES> &sc, int ci, int ctx,
                                                       const RaggedParams &p) {
   constexpr int NT = 4 * TILES;
@@ -121,9 +127,13 @@ __device__ __forceinline__ typename W::Probs row_soft(W &wa, RowState &st, const
       for (int e = 0; e < 4; ++e) t[4 * h + e] *= f;
     }
   }
-  typename W::Probs pb;
+  RowWeights<W> pb;
 #pragma unroll
-  for (int c = 0; c < 2 * TILES; ++c) pb.v[c >> 2][c & 3] = pack2<typename W::Operand>(t[2 * c], t[2 * c + 1]);
+  for (int c = 0; c < 2 * TILES; ++c) {
+    const uint32_t w = pack2<typename W::Operand>(t[2 * c], t[2 * c + 1]);
+    pb.top.v[c >> 2][c & 3] = w;
+    if constexpr (TWO) pb.rest.v[c >> 2][c & 3] = rest_of_pair<typename W::Operand>(w, t[2 * c], t[2 * c + 1]);
+  }
   return pb;
 }
 
@@ -146,6 +156,7 @@ __device__ __forceinline__ int64_t row_slot(const RaggedParams &p, int kvh, int 
 template <int D, typename OT, int KVF, int MAPS>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) ragged_rows_kernel(const RaggedParams p) {
   constexpr bool KV8 = KVF != kKv16;
+  constexpr bool kTwo = two_parts<KVF, MAPS>();
   constexpr int NW = 4;
   constexpr int TILES = 2;
   using W = WaveAttn<D, OT, KVF, TILES, Pipeline<KV8>::stream_loads_loop, false, true>;
@@ -314,15 +325,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
         const auto s = wa.qk(R);
         wa.issue_k(R, kvh, cn, ids);
         nsc = fetch_scales(ids, cn);
-        const auto pb = row_soft<KV8>(wa, st, col, R, s, sc, ci, q.ctx, p);
-        wa.pv(R, pb);
+        const auto pb = row_soft<KV8, kTwo>(wa, st, col, R, s, sc, ci, q.ctx, p);
+        wa.pv(R, pb.top);
+        if constexpr (kTwo) wa.pv(R, pb.rest);
         wa.issue_v(R, kvh, cn, ids);
         ids = wa.fetch_ids(table, cn + NW, last_col);
         sc = nsc;
         ci = cn;
       }
       const auto s = wa.qk(R);
-      wa.pv(R, row_soft<KV8>(wa, st, col, R, s, sc, ci, q.ctx, p));
+      const auto pb = row_soft<KV8, kTwo>(wa, st, col, R, s, sc, ci, q.ctx, p);
+      wa.pv(R, pb.top);
+      if constexpr (kTwo) wa.pv(R, pb.rest);
     }
 
     // Merge: sums and weights against the true maximum, then the wavefronts' states through LDS.  Wavefront w keeps the
@@ -518,6 +532,65 @@ __global__ void __launch_bounds__(512) ragged_rows_merge_kernel(const RaggedPara
     store_row<N>(p, q.first + j, head, lane, x);
   } else {
     store_row<N>(p, q.first + j, head, lane, o[0]);
+  }
+}
+
+// The same for many items, of which few are in more than two or three pieces: a work-group for all rows of one, a wavefront
+// for each row.  1024 items of 8 rows: 344 us with this kernel, 353 with the one above, whose 8192 work-groups find in the main that
+// there is nothing to join; 152 items of up to 16 rows 133 and 130, a sequence in 64 pieces 44 and 20.
+template <int D, int MAPS>
+__global__ void __launch_bounds__(512) ragged_rows_join_kernel(const RaggedParams p) {
+  constexpr int N = D / 64, NW = 8;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int seq = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x - seq * p.num_kv_heads;
+  // (not set where the sequence has no keys; asked for with the lengths)
+  const int first = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_seqs + seq));
+  const int last = load_uniform_i32(reinterpret_cast<const int32_t *>(p.row_seqs + seq) + 1);
+  const RaggedSeq q = ragged_seq_cut(p, ragged_seq_uniform(p.b, seq));
+  if (!in_rows_form<MAPS>(p, q)) return;
+  const int pieces = row_units<MAPS>(p, q) > 0 ? last - first + 1 : 0;
+  if (pieces == 1) return;  // the rows kernel has stored the result
+  const int64_t slot0 = row_slot(p, kvh, seq, first);
+  for (int row = wave; row < q.n * p.group; row += NW) {
+    const int j = row / p.group, head = kvh * p.group + (row - j * p.group);
+    float o[MAPS][N] = {};
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      const float *ml = p.row_ml + slot0 * 2 * kRowColumns + row * MAPS + m;
+      float top = -INFINITY;
+      for (int x0 = 0; x0 < pieces; x0 += 64)
+        top = fmaxf(top, wave_max(x0 + lane < pieces ? ml[(int64_t)(x0 + lane) * 2 * kRowColumns] : -INFINITY));
+      const float sub = top == -INFINITY ? 0.f : top;
+      float l = 0.f;
+      for (int x0 = 0; x0 < pieces; x0 += 64) {
+        const int here = min(64, pieces - x0);
+        float f = 0.f;
+        if (lane < here) {
+          const float *at = ml + (int64_t)(x0 + lane) * 2 * kRowColumns;
+          f = fast_exp2(at[0] - sub);
+          l += f * at[kRowColumns];
+        }
+#pragma unroll 4
+        for (int x = 0; x < here; ++x) {
+          const float fx = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), x));
+          const float *src = p.row_o + ((slot0 + x0 + x) * kRowColumns + row * MAPS + m) * D + lane * N;
+#pragma unroll
+          for (int k = 0; k < N; ++k) o[m][k] += fx * src[k];
+        }
+      }
+      l = wave_sum(l);
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+      for (int k = 0; k < N; ++k) o[m][k] *= inv;
+    }
+    if constexpr (MAPS == 2) {
+      float x[N];
+      differential_row<N>(p, head, lane, o[0], o[1], x);
+      store_row<N>(p, q.first + j, head, lane, x);
+    } else {
+      store_row<N>(p, q.first + j, head, lane, o[0]);
+    }
   }
 }
 
