@@ -249,7 +249,7 @@ inline fa_status launch_ragged_attention(void *out, const void *query, const voi
   p.softcap = o ? o->softcap : 0.f;
   p.window = (flags & FA_MASK_WINDOW) ? std::min<int32_t>(o->window_left, kNoWindow) : kNoWindow;
   p.mask_flags = flags & (FA_MASK_ALIBI | FA_MASK_SOFTCAP);
-  p.score_scale_log2 = std::max(std::abs(scale) * kLog2e, 1e-30f);  // (0 would turn masked scores into NaN)
+  p.score_scale_log2 = std::abs(scale) * kLog2e;
   p.query_flip = scale < 0.f ? 0x80008000u : 0u;
   p.q_bf16 = s->q_dtype == FA_DTYPE_BF16;
   p.num_heads = s->num_heads;

@@ -27,7 +27,7 @@ struct RaggedParams {
   float softcap;
   int32_t window;               // keys before a token's own that it sees; INT32_MAX / 2 without a window
   int32_t mask_flags;           // kMaskAlibi | kMaskSoftcap (the window is in `window`)
-  float score_scale_log2;       // |scale| * log2(e), > 0
+  float score_scale_log2;       // |scale| * log2(e)
   uint32_t query_flip;          // 0x80008000 for a negative scale: the queries change their sign instead
   int32_t q_bf16;               // type of query and out: bf16, or fp16
   int32_t num_heads, num_kv_heads, group;

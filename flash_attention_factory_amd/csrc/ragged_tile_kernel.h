@@ -637,8 +637,12 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int key = 32 * t + 8 * (e >> 2) + (e & 3);
-          if (key > hi || key < lo) x[t][e] = -INFINITY;  // select: the pool may hold NaN there
+          // multiplied first: a factor may be 0 (keys of zeros have the least scale, queries of zeros the least exponent), and
+          // -inf times 0 is NaN.  A select, since the pool may hold NaN there.
+          x[t][e] = key > hi || key < lo ? -INFINITY : x[t][e] * cc[2 * t + (e >> 3)];
         }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) cc[k] = 1.f;
     }
     float gm[4];
 #pragma unroll

@@ -6,7 +6,7 @@ a sequence's n new ones sits at position ``context_lens[s] - n + j`` and sees th
 already (``kv_cache_append`` puts them there).  ``max_query_len`` bounds the new tokens of a sequence, ``max_context_len`` its keys (0:
 what the block table holds).
 
-Pools: 16-bit of the queries' type; FP8 with ``fp8_scale``; or bytes (FP8 or int8) with ``k_scales`` / ``v_scales``, positive, of
+Pools: 16-bit of the queries' type; FP8 with ``fp8_scale``; or bytes (FP8 or int8) with ``k_scales`` / ``v_scales``, not negative, of
 ``[kv_heads]`` or ``[blocks, kv_heads]``.  ``sinks``, ``alibi_slopes``, ``softcap`` (> 0) and ``window_left`` (>= 0) act when they are
 passed.  The reference has the single-token case only (paged_attention_loop.cpp:21-84); its ``attention_ref`` (test_paged.py:40-168)
 says what the modifiers mean.

@@ -120,8 +120,8 @@ int64_t fa_paged_attention_ragged_workspace_bytes(const fa_ragged_shape *shape, 
 /*
  * out [num_tokens, num_heads, head_size], contiguous, q_dtype.  Of options: sinks, alibi_slopes,
  * softcap, mask_flags and window_left as in fa_paged_attention.h; fp8_scale, kv_scale_mode,
- * k_scales and v_scales of byte pools (integers take FA_KV_SCALE_BLOCK or _HEAD); stream, elapsed_us (1 float)
- * and validate_only.  A token that sees no key gets zeros.  Tokens beyond max_query_len of their
+ * k_scales and v_scales of byte pools (integers take FA_KV_SCALE_BLOCK or _HEAD; scales are not negative, and 0
+ * stands for rows of zeros); stream, elapsed_us (1 float) and validate_only.  A token that sees no key gets zeros.  Tokens beyond max_query_len of their
  * sequence are left out.
  */
 int32_t fa_paged_attention_ragged(void *out, const void *query, const void *key_cache, const void *value_cache,

@@ -1,0 +1,84 @@
+"""Ragged append and attention at the edges of what a call may hold: rows and scales of zeros, lengths that the table or the caller's
+bounds do not cover, sinks far above the scores, blocks longer than a step."""
+import math
+
+import pytest
+import torch
+
+from flash_attention_factory_amd import torch_ops  # noqa: F401
+
+import _ragged as R
+from test_gpu_ragged_attention import _close, _pools, _query, _strided
+
+pytestmark = pytest.mark.gpu
+
+LEAST = 2.0 ** -126  # the scale that the append gives to a block of zeros
+
+
+def _attend(batch, query, pools, scale, *, maps=1, most=None, longest=0, window=-1, sinks=None, slopes=None, lambdas=None, weight=None,
+            eps=1e-5, out_scale=1.0, fp8_scale=1.0):
+    """The operator's result; rows that it leaves alone are NaN."""
+    (kp, _, ks), (vp, _, vs) = pools
+    dev = "cuda"
+    tables, start, lens = batch.on(dev)
+    out = torch.full(query.shape, float("nan"), dtype=query.dtype, device=dev)
+    args = (out, _strided(query), kp, vp, tables.contiguous(), start, lens, scale)
+    most = most or max(1, max(batch.new))
+    if maps == 1:
+        torch.ops.fa_amd.paged_attention_ragged(*args, most, longest, fp8_scale=fp8_scale, k_scales=ks, v_scales=vs,
+                                                sinks=None if sinks is None else sinks.to(dev),
+                                                alibi_slopes=None if slopes is None else slopes.to(dev), window_left=window)
+    else:
+        torch.ops.fa_amd.paged_attention_differential(*args, lambdas.to(dev), None if weight is None else weight.to(dev), most, longest,
+                                                      norm_eps=eps, out_scale=out_scale, k_scales=ks, v_scales=vs, window_left=window)
+    torch.cuda.synchronize()
+    return out
+
+
+# ---- factors of zero ----
+
+@pytest.mark.parametrize("new,old", [([40, 1], [0, 30]), ([40], [100]), ([1, 3], [20, 47])])
+@pytest.mark.parametrize("maps", [1, 2])
+def test_rows_of_zeros_from_the_append(new, old, maps):
+    """Padding: keys, values and queries of zeros, put into integer pools by the append itself."""
+    batch = R.Batch(new, [0] * len(old), B=16, lens=[n + o for n, o in zip(new, old)])
+    fill = R.Batch([n + o for n, o in zip(new, old)], [0] * len(old), B=16)
+    fill.tables = batch.tables
+    H, Hk, D, dtype, dev = 4, 2, 64, torch.bfloat16, "cuda"
+    pools = [torch.full((batch.blocks, 16, Hk, D), 55, dtype=torch.int8, device=dev) for _ in range(2)]
+    scales = [torch.full((batch.blocks, Hk), float("nan"), device=dev) for _ in range(2)]
+    tables, start, lens = fill.on(dev)
+    rows = torch.zeros(fill.T, Hk, D, dtype=dtype, device=dev)
+    values = torch.ones(fill.T, Hk, D, dtype=dtype, device=dev)
+    torch.ops.fa_amd.kv_cache_append(rows, values, *pools, tables, start, lens, None, None, None, *scales)
+    for size in (0.0, 1e-6, 1.0):
+        query = torch.full((batch.T, H, D), size, dtype=dtype)
+        out = _attend(batch, query, [(pools[0], None, scales[0]), (pools[1], None, scales[1])], 0.125, maps=maps,
+                      lambdas=torch.full((H,), 0.25))
+        # every key counts the same, and every value is 1: 127 steps of 1 / 127 in 32 bits
+        want = 1.0 if maps == 1 else 0.75
+        assert bool(((out.float() - want).abs() < 2.0 ** -8).all())
+
+
+@pytest.mark.parametrize("name", ["mixed", "decode"])
+@pytest.mark.parametrize("k_scale", [LEAST, 0.0])
+@pytest.mark.parametrize("scale", [0.0, 1e-33, 0.125, -0.125])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_key_scales_down_to_zero(name, k_scale, scale, dtype):
+    """Some blocks' keys count for nothing (scores of 0 with them), whatever the scale of the scores and the queries' size."""
+    batch = R.Batch(*{"mixed": ([1, 70, 0, 3, 1, 150], [300, 10, 20, 129, 0, 77]), "decode": ([1] * 6, [0, 1, 62, 127, 128, 515])}[name], B=16)
+    H, Hk, D = 4, 2, 64
+    (kp, k, ks), (vp, v, vs) = _pools(batch, Hk, D, "i8", dtype, "head", 3)
+    some = torch.arange(batch.blocks) % 3 == 0
+    there = some & batch.used.any(1)
+    ks[there.cuda()] = k_scale
+    k = k.masked_fill(some[:, None, None, None], 0.0)
+    query = _query(batch, H, D, dtype, 3)
+    query[::5] = 0
+    out = _attend(batch, query, [(kp, k, ks), (vp, v, vs)], scale)
+    maps = R.attention(batch, query, k, v, scale)
+    _close(out, maps[0][0], R.attention_bound(maps, dtype, torch.float16))
+    lambdas = torch.full((H,), 0.3)
+    out = _attend(batch, query, [(kp, k, ks), (vp, v, vs)], scale, maps=2, lambdas=lambdas)
+    maps = R.attention(batch, query, k, v, scale, maps=2)
+    _close(out, R.differential(maps, lambdas, None, 0.0, 1.0), R.attention_bound(maps, dtype, torch.float16, lambdas))
