@@ -81,6 +81,10 @@ struct RaggedTile {
   static constexpr int kPerRow = kRowBytes / 16;             // threads that load a row
   static constexpr int kRowsPerPass = kThreads / kPerRow;
   static constexpr int kPasses = kRowsPerPass >= kTileKeys ? 1 : kTileKeys / kRowsPerPass;
+  // Key of a step that thread row `load_row` loads in a pass.  Where there are more thread rows than keys the surplus ones repeat the
+  // others' (what they have loaded is not stored): a key beyond the step's 64 would lie, with blocks of more than 64, as
+  // far beyond the end of its block.
+  static __host__ __device__ constexpr int load_key(int pass, int load_row) { return (pass * kRowsPerPass + load_row) & (kTileKeys - 1); }
 
   // where 16-byte piece c of row `key` of a step lies in its buffer
   static __device__ __forceinline__ int k_at(int key, int c) {
@@ -384,7 +388,6 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
 
   // this lane's row (rows past the end repeat the last one and are not stored)
   const int my_row = row0 + strip * 32 + col;
-  const bool valid = my_row < all_rows;
   const int row = min(my_row, all_rows - 1);
   const int j = row / G, head = kvh * G + (row - j * G);
   const int pos = pos0 + j;
@@ -444,7 +447,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   int32_t row_col[T::kPasses];  // the thread's row in block-table columns from the step's first
 #pragma unroll
   for (int x = 0; x < T::kPasses; ++x) {
-    const int key = x * T::kRowsPerPass + load_row;
+    const int key = T::load_key(x, load_row);
     const int64_t off = (int64_t)kvh * p.a.kv_head_bytes + piece * 16 + (int64_t)((uint64_t)(uint32_t)(key & in_block) * token_bytes);
     k_row[x] = p.a.key_cache + off;
     v_row[x] = p.a.value_cache + off;
@@ -487,12 +490,12 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
     }
   };
   auto write_k = [&](int n, int w) {
-    const int pass = KV8 ? w >> 1 : w, key = pass * T::kRowsPerPass + load_row;
+    const int pass = KV8 ? w >> 1 : w, key = T::load_key(pass, load_row);
     const u32x4 o = lds_piece(kreg[pass], w);
     if (loads) *reinterpret_cast<u32x4 *>(lds + (n & 1) * T::kBufferBytes + T::k_at(key, KV8 ? 2 * piece + (w & 1) : piece)) = o;
   };
   auto write_v = [&](int n, int w) {
-    const int pass = KV8 ? w >> 1 : w, key = pass * T::kRowsPerPass + load_row;
+    const int pass = KV8 ? w >> 1 : w, key = T::load_key(pass, load_row);
     // what no row of the tile sees may be NaN
     if ((uint32_t)((step + n) * kTileKeys + key - seen_lo) >= (uint32_t)seen_keys) vreg[pass] = u32x4{0u, 0u, 0u, 0u};
     const u32x4 o = lds_piece(vreg[pass], w);

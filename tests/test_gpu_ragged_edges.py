@@ -82,3 +82,25 @@ def test_key_scales_down_to_zero(name, k_scale, scale, dtype):
     out = _attend(batch, query, [(kp, k, ks), (vp, v, vs)], scale, maps=2, lambdas=lambdas)
     maps = R.attention(batch, query, k, v, scale, maps=2)
     _close(out, R.differential(maps, lambdas, None, 0.0, 1.0), R.attention_bound(maps, dtype, torch.float16, lambdas))
+
+
+# ---- blocks longer than a step of 64 keys, with a pool that ends with them ----
+
+@pytest.mark.parametrize("B", [128, 256])
+@pytest.mark.parametrize("layout", ["head", "token"])
+@pytest.mark.parametrize("kv", ["i8", "e4m3"])
+def test_long_blocks_with_more_loading_threads_than_keys(B, layout, kv):
+    """Rows of 64 bytes and eight wavefronts: twice as many threads as a step has keys to load."""
+    batch = R.Batch([70, 1, 45], [1700, 300, 3], B=B, spare=0)
+    H, Hk, D, dtype = 16, 2, 64, torch.float16
+    query = _query(batch, H, D, dtype, 4)
+    pools = _pools(batch, Hk, D, kv, dtype, layout, 4)
+    (_, k, _), (_, v, _) = pools
+    out = _attend(batch, query, pools, 0.125)
+    maps = R.attention(batch, query, k, v, 0.125)
+    _close(out, maps[0][0], R.attention_bound(maps, dtype, torch.float16))
+    if kv == "i8":
+        lambdas = torch.full((H,), 0.4)
+        out = _attend(batch, query, pools, 0.125, maps=2, lambdas=lambdas)
+        maps = R.attention(batch, query, k, v, 0.125, maps=2)
+        _close(out, R.differential(maps, lambdas, None, 0.0, 1.0), R.attention_bound(maps, dtype, torch.float16, lambdas))
