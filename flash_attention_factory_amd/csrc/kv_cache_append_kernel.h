@@ -135,7 +135,7 @@ __device__ __forceinline__ void place_tokens(const RaggedBatch &b, int t0, int c
     const int from = max(q.first, t0), to = min(q.first + q.n, t0 + count);
     for (int t = from; t < to; ++t) {
       seq[t - t0] = s;
-      pos[t - t0] = q.ctx - q.n + (t - q.first);
+      pos[t - t0] = q.pos0 + (t - q.first);
     }
   }
   __syncthreads();

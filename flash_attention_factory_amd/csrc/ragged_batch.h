@@ -18,16 +18,19 @@ struct RaggedBatch {
   int32_t max_block_id;
 };
 
-// New tokens of a sequence: first row, how many, and the keys with them.  A length that the block table cannot hold is cut to
-// what it holds, rows that the token arrays do not have are not asked for.
+// New tokens of a sequence: first row, how many, keys up to the last one's own, and the position of the first.  Rows that the token
+// arrays do not have are not asked for, and keys that the block table cannot hold are not there; positions are those of
+// the lengths as they are given, whatever has been cut.
 struct RaggedSeq {
-  int32_t first, n, ctx;
+  int32_t first, n, ctx, pos0;
 };
 __device__ __forceinline__ RaggedSeq ragged_seq(const RaggedBatch &b, int s, int32_t start, int32_t end, int32_t len) {
   RaggedSeq q;
   q.first = min(max(start, 0), b.num_tokens);
-  q.n = min(max(end, q.first), b.num_tokens) - q.first;
-  q.ctx = max(0, min(len, b.max_blocks_per_seq << b.block_shift));
+  const int32_t all = max(end, q.first) - q.first;
+  q.n = min(all, b.num_tokens - q.first);
+  q.pos0 = max(len, 0) - all;
+  q.ctx = max(0, min(q.pos0 + q.n, b.max_blocks_per_seq << b.block_shift));
   return q;
 }
 // for a sequence number that all lanes share (scalar loads) ...

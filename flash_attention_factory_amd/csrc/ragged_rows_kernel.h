@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
 
   // This work-group's share of the line of units.  The first 64 sequences' lengths are asked for once; whose turn it is
   // among them is read from the lanes.
-  RaggedSeq of_lane = {0, 0, 0};
+  RaggedSeq of_lane = {0, 0, 0, 0};
   int32_t units_of_lane = 0;
   if (lane < p.b.num_seqs) {
     of_lane = ragged_seq_of_lane(p.b, lane);
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
   }
   const auto seq_at = [&](int s) {
     return s < 64 ? RaggedSeq{__builtin_amdgcn_readlane(of_lane.first, s), __builtin_amdgcn_readlane(of_lane.n, s),
-                              __builtin_amdgcn_readlane(of_lane.ctx, s)}
+                              __builtin_amdgcn_readlane(of_lane.ctx, s), __builtin_amdgcn_readlane(of_lane.pos0, s)}
                   : ragged_seq_uniform(p.b, s);
   };
   int32_t total = 0, u, u_end, before = 0;  // units of the line, this share of it, units before the sequence's own

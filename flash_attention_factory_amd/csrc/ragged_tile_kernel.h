@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
     if (p.b.num_seqs <= 64) {
       // Sequences with more keys first.  Each lane has one; its rank is the number of those before it, and what lies before it the
       // sum of their tiles.
-      const RaggedSeq mine = lane < p.b.num_seqs ? ragged_seq_of_lane(p.b, lane) : RaggedSeq{0, 0, 0};
+      const RaggedSeq mine = lane < p.b.num_seqs ? ragged_seq_of_lane(p.b, lane) : RaggedSeq{0, 0, 0, 0};
       const int tiles = lane < p.b.num_seqs ? row_tiles<MAPS, T::kRows>(p, mine) : 0;
       before = 0;
       for (int s = 0; s < p.b.num_seqs; ++s) {

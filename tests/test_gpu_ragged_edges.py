@@ -104,3 +104,65 @@ def test_long_blocks_with_more_loading_threads_than_keys(B, layout, kv):
         out = _attend(batch, query, pools, 0.125, maps=2, lambdas=lambdas)
         maps = R.attention(batch, query, k, v, 0.125, maps=2)
         _close(out, R.differential(maps, lambdas, None, 0.0, 1.0), R.attention_bound(maps, dtype, torch.float16, lambdas))
+
+
+# ---- tokens beyond the block table ----
+
+def _narrow(batch, columns):
+    batch.tables = batch.tables[:, :columns].contiguous()
+    return batch
+
+
+@pytest.mark.parametrize("kv", ["16", "i8"])
+@pytest.mark.parametrize("new,lens,columns", [([1], [33], 2), ([1, 40, 5], [40, 45, 31], 2), ([70, 2], [100, 65], 4), ([3], [80], 2)])
+def test_append_beyond_the_table_is_left_out(kv, new, lens, columns):
+    """Tokens at positions past the table's columns are not stored; those before are, at their own positions."""
+    H, Hk, D, dtype, dev = 2, 2, 64, torch.float16, "cuda"
+    batch = R.Batch(new, [0] * len(new), B=16, lens=lens)
+    whole = batch.tables.clone()
+    _narrow(batch, columns)
+    g = torch.Generator().manual_seed(6)
+    fused = torch.randn(batch.T, H + 2 * Hk, D, generator=g).to(dtype)
+    shape = (batch.blocks, 16, Hk, D)
+    if kv == "i8":
+        pools = [torch.randint(-127, 128, shape, generator=g, dtype=torch.int8) for _ in range(2)]
+        scales = [0.002 + 0.03 * torch.rand(batch.blocks, Hk, generator=g) for _ in range(2)]
+    else:
+        pools, scales = [torch.randn(shape, generator=g).to(dtype) for _ in range(2)], []
+    table = R.angle_table(max(lens), D)
+    d_fused, d_pools, d_scales = fused.to(dev), [p.to(dev) for p in pools], [s.to(dev) for s in scales]
+    d_out = torch.zeros(batch.T, H, D, dtype=dtype, device=dev)
+    torch.ops.fa_amd.kv_cache_append(d_fused[:, H:H + Hk], d_fused[:, H + Hk:], *d_pools, *batch.on(dev), table.to(dev), d_fused[:, :H],
+                                     d_out, *(d_scales or (None, None)))
+    # the plain form on the wide table, with ids of no block beyond the narrow one
+    batch.tables = torch.where(torch.arange(whole.size(1))[None] < columns, whole, torch.full_like(whole, 1 << 30))
+    want = R.append(batch, fused[:, H:H + Hk], fused[:, H + Hk:], *pools, table, False, *(scales or (None, None)), query=fused[:, :H])
+    for got, ref in zip(d_pools + d_scales, pools + scales):
+        assert torch.equal(got.cpu(), ref)
+    assert torch.equal(d_out.cpu(), want)
+
+
+@pytest.mark.parametrize("new,old", [([3, 50], [20, 40]), ([1, 4], [0, 300])])
+@pytest.mark.parametrize("kv", ["16", "i8"])
+def test_append_of_more_tokens_in_query_start_than_rows(new, old, kv):
+    """Arrays with fewer rows than query_start counts: the rows that are there keep their positions."""
+    Hk, D, dtype, dev = 2, 64, torch.float16, "cuda"
+    batch = R.Batch(new, old, B=16)
+    rows = batch.T - 2
+    fewer = R.Batch(new[:-1] + [new[-1] - 2], old, B=16)
+    fewer.tables = batch.tables
+    g = torch.Generator().manual_seed(11)
+    fused = torch.randn(rows, 2 * Hk, D, generator=g).to(dtype)
+    shape = (batch.blocks, 16, Hk, D)
+    if kv == "i8":
+        pools = [torch.randint(-127, 128, shape, generator=g, dtype=torch.int8) for _ in range(2)]
+        scales = [0.002 + 0.03 * torch.rand(batch.blocks, Hk, generator=g) for _ in range(2)]
+    else:
+        pools, scales = [torch.randn(shape, generator=g).to(dtype) for _ in range(2)], []
+    table = R.angle_table(max(batch.lens), D)
+    d_rows, d_pools, d_scales = fused.to(dev), [p.to(dev) for p in pools], [x.to(dev) for x in scales]
+    torch.ops.fa_amd.kv_cache_append(d_rows[:, :Hk], d_rows[:, Hk:], *d_pools, *batch.on(dev), table.to(dev), None, None,
+                                     *(d_scales or (None, None)))
+    R.append(fewer, fused[:, :Hk], fused[:, Hk:], *pools, table, False, *(scales or (None, None)))
+    for got, ref in zip(d_pools + d_scales, pools + scales):
+        assert torch.equal(got.cpu(), ref)
