@@ -74,8 +74,10 @@ __device__ __forceinline__ uint32_t rest_of_pair(uint32_t rounded, float lo, flo
   return pack2<OT>(lo - f32_from_half_of<OT>(rounded, 0), hi - f32_from_half_of<OT>(rounded, 1));
 }
 
+// The tokens that the call has bounds for: the first max_query_len ones, and the keys that those see.
 __device__ __forceinline__ RaggedSeq ragged_seq_cut(const RaggedParams &p, RaggedSeq q) {
   q.n = min(q.n, p.max_query_len);
+  q.ctx = max(0, min(q.ctx, q.pos0 + q.n));
   return q;
 }
 template <int MAPS>
@@ -83,14 +85,14 @@ __device__ __forceinline__ bool in_rows_form(const RaggedParams &p, const Ragged
   return q.n * p.group * MAPS <= p.row_limit;
 }
 // First key that some new token of the sequence sees.
-__device__ __forceinline__ int first_key(const RaggedParams &p, const RaggedSeq &q) { return max(0, q.ctx - q.n - p.window); }
+__device__ __forceinline__ int first_key(const RaggedParams &p, const RaggedSeq &q) { return max(0, q.pos0 - p.window); }
 
 // Units of keys that the rows form has to go through for one kv head of a sequence.
 template <int MAPS>
 __device__ __forceinline__ int row_units(const RaggedParams &p, RaggedSeq q) {
   q = ragged_seq_cut(p, q);
   if (q.n <= 0 || !in_rows_form<MAPS>(p, q)) return 0;
-  return (q.ctx + kRowUnit - 1) / kRowUnit - first_key(p, q) / kRowUnit;
+  return max(0, (q.ctx + kRowUnit - 1) / kRowUnit - first_key(p, q) / kRowUnit);
 }
 // Tiles of `rows` rows that the tile form has to go through for one kv head of a sequence.
 template <int MAPS, int ROWS>

@@ -118,7 +118,7 @@ __device__ __forceinline__ TileCosts tile_costs(const RaggedParams &p, RaggedSeq
   TileCosts c;
   c.tiles = row_tiles<MAPS, ROWS>(p, q);
   q = ragged_seq_cut(p, q);
-  const int tokens = ROWS / p.group + 1, all = max(q.ctx - q.n, 0);
+  const int tokens = ROWS / p.group + 1, all = min(max(q.pos0, 0), q.ctx);
   const int most = min(p.window, kNoWindow - tokens) + tokens;  // keys that a tile can see
   const int a = min(all + tokens, most), b = min(all + c.tiles * tokens, most);
   c.first = a + kTileStart;
@@ -216,11 +216,12 @@ struct TileSteps {
 };
 template <int ROWS>
 __device__ __forceinline__ TileSteps tile_steps(const RaggedParams &p, const RaggedSeq &q, int tile) {
-  const int row0 = tile * ROWS, pos0 = q.ctx - q.n;
-  const int pos_lo = pos0 + row0 / p.group, pos_hi = pos0 + (min(row0 + ROWS, q.n * p.group) - 1) / p.group;
+  const int row0 = tile * ROWS;
+  const int pos_lo = q.pos0 + row0 / p.group, pos_hi = q.pos0 + (min(row0 + ROWS, q.n * p.group) - 1) / p.group;
+  const int last = min(pos_hi, q.ctx - 1);  // (tokens past the block table see what it holds)
   TileSteps s;
   s.first = max(0, pos_lo - p.window) / kTileKeys;
-  s.count = pos_hi < 0 ? 0 : pos_hi / kTileKeys + 1 - s.first;
+  s.count = last < 0 ? 0 : max(0, last / kTileKeys + 1 - s.first);
   return s;
 }
 // Where a cut `off` into a tile of cost `cost` falls between its steps.
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const bool whole = !LINE || (from == 0 && until == of_tile.count);
   if (whole || from < until) {  // (a tile that sees no keys is whole: its rows get zeros)
   const int all_rows = q.n * G, row0 = tile * T::kRows;
-  const int pos0 = q.ctx - q.n;  // position of the sequence's first new token
+  const int pos0 = q.pos0, last_key = q.ctx - 1;
   const int step = of_tile.first + from, step_end = of_tile.first + until;
 
   // this lane's row (rows past the end repeat the last one and are not stored)
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const int last_col = p.b.max_blocks_per_seq - 1, in_block = (1 << p.b.block_shift) - 1;
   const int steps = step_end - step;
   const int seen_lo = max(0, pos0 + row0 / G - p.window);  // keys that some row of the tile sees
-  const int seen_keys = pos0 + (min(row0 + T::kRows, all_rows) - 1) / G + 1 - seen_lo;
+  const int seen_keys = max(0, min(pos0 + (min(row0 + T::kRows, all_rows) - 1) / G, last_key) + 1 - seen_lo);
   // Blocks of this thread's rows: of the next step of K as the table has them (cut to the pool where they are used, since
   // arithmetic here would wait for the load, and for every load before it), and of the next step of V, one step behind.
   int32_t kid[T::kPasses], vid[T::kPasses];
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   u32x4 rest[kTwo ? 4 : 1];  // what their rounding left
   // the steps of which this wavefront sees anything: see_lo .. see_hi - 1 (the same for all its lanes)
   const int see_lo = wave_live ? max(0, (wave_lo - p.window) / kTileKeys - step) : steps;
-  const int see_hi = wave_live && wave_hi >= 0 ? min(steps, wave_hi / kTileKeys + 1 - step) : 0;
+  const int see_hi = wave_live && wave_hi >= 0 ? min(steps, min(wave_hi, last_key) / kTileKeys + 1 - step) : 0;
   // Where this lane reads K (16-byte piece of key `col`) and V (8 bytes of key 4 half + i / 4) within a buffer; the swizzles are
   // exclusive-ors, so a k-step or d-tile is one more of them and keys further on are an offset (see k_at, v_at).
   const int i16 = lane & 15;
@@ -633,8 +634,8 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
 #pragma unroll
       for (int k = 0; k < 4; ++k) cc[k] = 1.f;
     }
-    if (t0 + kTileKeys - 1 > wave_lo || t0 < wave_hi - p.window) {
-      const int hi = pos - t0 - 4 * half, lo = hi - p.window;
+    if (t0 + kTileKeys - 1 > min(wave_lo, last_key) || t0 < wave_hi - p.window) {
+      const int hi = min(pos, last_key) - t0 - 4 * half, lo = pos - p.window - t0 - 4 * half;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll

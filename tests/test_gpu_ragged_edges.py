@@ -166,3 +166,92 @@ def test_append_of_more_tokens_in_query_start_than_rows(new, old, kv):
     R.append(fewer, fused[:, :Hk], fused[:, Hk:], *pools, table, False, *(scales or (None, None)))
     for got, ref in zip(d_pools + d_scales, pools + scales):
         assert torch.equal(got.cpu(), ref)
+
+
+def _beyond(batch, query, k, v, scale, columns, maps=1, window=-1, slopes=None):
+    """64-bit form for tables of `columns` columns: positions are the lengths', keys are those of the table."""
+    T, H, D = query.shape
+    Hk, B, d = k.size(2), batch.B, D // maps
+    got = [(torch.zeros(T, H, D, dtype=torch.float64), torch.zeros(T, H, D, dtype=torch.float64)) for _ in range(maps)]
+    for s, (n, ctx) in enumerate(zip(batch.new, batch.lens)):
+        a, keys = int(batch.start[s]), min(ctx, columns * B)
+        t, pos = torch.arange(keys), torch.arange(ctx - n, ctx)
+        ids = batch.tables[s, t // B].long()
+        sees = t[None] <= pos[:, None]
+        if window >= 0:
+            sees &= t[None] >= pos[:, None] - window
+        for h in range(H):
+            rows, vals = k[ids, t % B, h // (H // Hk)], v[ids, t % B, h // (H // Hk)]
+            for m in range(maps):
+                x = query[a:a + n, h, m * d:(m + 1) * d].double() @ rows[:, m * d:(m + 1) * d].T * scale
+                if slopes is not None:
+                    x = x + float(slopes[h]) * (t[None] - pos[:, None])
+                x = x.masked_fill(~sees, -math.inf)
+                p = torch.softmax(x, -1).masked_fill(~sees, 0.0)
+                got[m][0][a:a + n, h] = p @ vals
+                got[m][1][a:a + n, h] = p @ vals.abs()
+    return got
+
+
+@pytest.mark.parametrize("kv", ["16", "i8"])
+@pytest.mark.parametrize("new,lens,columns", [([1, 1], [40, 33], 2), ([1, 2], [1300, 1290], 80), ([40, 7], [47, 20], 2),
+                                              ([300], [1500], 80), ([90, 30], [100, 60], 2)])
+@pytest.mark.parametrize("window", [-1, 12])
+def test_attention_beyond_the_table_sees_what_is_there(kv, new, lens, columns, window):
+    H, Hk, D, dtype = 4, 2, 64, torch.float16
+    batch = R.Batch(new, [0] * len(new), B=16, lens=lens)
+    query = _query(batch, H, D, dtype, 8)
+    # rows past the narrow table's are not to be read
+    wide = batch.tables.clone()
+    for s in range(len(new)):
+        for block in wide[s, columns:].tolist():
+            if 0 <= block < batch.blocks:
+                batch.used[block] = False
+    pools = _pools(batch, Hk, D, kv, dtype, "head", 8)
+    (_, k, _), (_, v, _) = pools
+    _narrow(batch, columns)
+    slopes = torch.tensor([0.5, 0.1, 0.02, 0.0])
+    for more in ({}, {"slopes": slopes}):
+        out = _attend(batch, query, pools, 0.125, window=window, **more)
+        maps = _beyond(batch, query, k, v, 0.125, columns, window=window, **more)
+        _close(out, maps[0][0], R.attention_bound(maps, dtype, dtype))
+    lambdas = torch.full((H,), 0.4)
+    out = _attend(batch, query, pools, 0.17, maps=2, lambdas=lambdas, window=window)
+    maps = _beyond(batch, query, k, v, 0.17, columns, maps=2, window=window)
+    _close(out, R.differential(maps, lambdas, None, 0.0, 1.0), R.attention_bound(maps, dtype, dtype, lambdas))
+
+
+# ---- more new tokens than the call's bounds allow ----
+
+@pytest.mark.parametrize("kv", ["16", "i8"])
+@pytest.mark.parametrize("most", [1, 3, 30, 200])
+@pytest.mark.parametrize("maps", [1, 2])
+def test_tokens_beyond_max_query_len_are_left_out(kv, most, maps):
+    """The first `most` tokens of a sequence are right, the rest of `out` stays as it was."""
+    H, Hk, D, dtype = 4, 2, 64, torch.float16
+    batch = R.Batch([40, 1, 300, 5], [7, 100, 650, 0], B=16)
+    query = _query(batch, H, D, dtype, 9)
+    pools = _pools(batch, Hk, D, kv, dtype, "head", 9)
+    (_, k, _), (_, v, _) = pools
+    lambdas = torch.full((H,), 0.4)
+    out = _attend(batch, query, pools, 0.125, maps=maps, most=most, lambdas=lambdas, window=70 if most == 30 else -1)
+    refs = R.attention(batch, query, k, v, 0.125, maps=maps, window=70 if most == 30 else -1)
+    want = refs[0][0] if maps == 1 else R.differential(refs, lambdas, None, 0.0, 1.0)
+    bound = R.attention_bound(refs, dtype, dtype, None if maps == 1 else lambdas)
+    kept = torch.cat([torch.arange(n) < most for n in batch.new])
+    assert bool(torch.isnan(out.cpu()[~kept]).all())
+    _close(out.cpu()[kept], want[kept], bound[kept])
+
+
+@pytest.mark.parametrize("new,old", [([3, 50], [20, 40]), ([1, 4], [0, 300])])
+def test_more_tokens_in_query_start_than_rows(new, old):
+    """Arrays with fewer rows than query_start counts: the rows that are there keep their positions."""
+    H, Hk, D, dtype, dev = 4, 2, 64, torch.float16, "cuda"
+    batch = R.Batch(new, old, B=16)
+    rows = batch.T - 2
+    query = _query(batch, H, D, dtype, 10)
+    pools = _pools(batch, Hk, D, "16", dtype, "head", 10)
+    (kp, k, _), (vp, v, _) = pools
+    out = _attend(batch, query[:rows], pools, 0.125, most=max(new))
+    refs = R.attention(batch, query, k, v, 0.125)
+    _close(out, refs[0][0][:rows], R.attention_bound(refs, dtype, dtype)[:rows])
