@@ -141,6 +141,13 @@ __device__ __forceinline__ float sink_log2(const RaggedParams &p, int head) {
                    : load_scalar16<F16>(reinterpret_cast<const char *>(p.sinks) + head * 2)) * kLog2e;
 }
 
+// What a differential row with this mean square is multiplied with.  A row of zeros (a token that sees nothing) stays one without
+// an epsilon, too.
+__device__ __forceinline__ float norm_factor(const RaggedParams &p, float mean_square) {
+  const float x = mean_square + p.norm_eps;
+  return x == 0.f ? 0.f : p.out_scale / sqrtf(x);
+}
+
 // The differential result of one row from its two maps: lane l of a wavefront holds the N elements from l * N on.
 template <int N>
 __device__ __forceinline__ void differential_row(const RaggedParams &p, int head, int lane, const float (&o1)[N], const float (&o2)[N],
@@ -157,7 +164,7 @@ __device__ __forceinline__ void differential_row(const RaggedParams &p, int head
     for (int k = 0; k < N; ++k) x[k] *= p.out_scale;
     return;
   }
-  const float mul = p.out_scale / sqrtf(wave_sum(square) / (64.0f * N) + p.norm_eps);
+  const float mul = norm_factor(p, wave_sum(square) / (64.0f * N));
 #pragma unroll
   for (int k = 0; k < N; ++k) x[k] *= mul * p.norm_weight[lane * N + k];
 }

@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
           sm_m[wave][i] = rows_sum(square);
         }
         __syncthreads();
-        if (p.norm_weight) mul /= sqrtf((sm_m[0][i] + sm_m[1][i] + sm_m[2][i] + sm_m[3][i]) / D + p.norm_eps);
+        if (p.norm_weight) mul = norm_factor(p, (sm_m[0][i] + sm_m[1][i] + sm_m[2][i] + sm_m[3][i]) / D);
         if (valid && map == 0) {
           char *dst = p.out + (((int64_t)(q.first + j) * p.num_heads + head) * D + d0) * 2;
           float w[SL];

@@ -268,7 +268,7 @@ __device__ __forceinline__ void tile_finish(const RaggedParams &p, const RaggedS
       f32x4 w[DT * 4];  // all asked for before the first is used
 #pragma unroll
       for (int k = 0; k < DT * 4; ++k) w[k] = *reinterpret_cast<const f32x4 *>(p.norm_weight + 8 * k + 4 * half);
-      const float mul = p.out_scale / sqrtf(halves_sum(square) / D + p.norm_eps);
+      const float mul = norm_factor(p, halves_sum(square) / D);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll

@@ -135,7 +135,7 @@ int32_t fa_paged_attention_ragged(void *out, const void *query, const void *key_
  *   o   = softmax(scale q1 k1^T) V - lambdas[head] softmax(scale q2 k2^T) V      (in 32 bits)
  *   out = out_scale * norm_weight * o / sqrt(mean(o^2) + norm_eps)
  * lambdas [num_heads], norm_weight [head_size] fp32 device memory; without norm_weight
- * out = out_scale * o.  16-bit and integer pools; of mask_flags only FA_MASK_WINDOW; no sinks.
+ * out = out_scale * o.  Rows of zeros stay zeros, also with norm_eps 0.  16-bit and integer pools; of mask_flags only FA_MASK_WINDOW; no sinks.
  */
 int32_t fa_paged_attention_differential(void *out, const void *query, const void *key_cache, const void *value_cache,
                                         const int32_t *block_tables, const int32_t *query_start,

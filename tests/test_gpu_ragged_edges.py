@@ -255,3 +255,25 @@ def test_more_tokens_in_query_start_than_rows(new, old):
     out = _attend(batch, query[:rows], pools, 0.125, most=max(new))
     refs = R.attention(batch, query, k, v, 0.125)
     _close(out, refs[0][0][:rows], R.attention_bound(refs, dtype, dtype)[:rows])
+
+
+# ---- nothing to normalise ----
+
+@pytest.mark.parametrize("new,old,lens", [([5, 3], [0, 0], [2, 0]), ([5, 40, 1], [0, 0, 0], [2, 25, 0]), ([2, 1], [0, 700], [1, 701]),
+                                          ([2, 1], [0, 700], [0, 701])])
+@pytest.mark.parametrize("longest", [0, 10000])
+def test_differential_without_epsilon_and_without_keys(new, old, lens, longest):
+    """norm_eps may be 0: tokens that see nothing are zeros, the others are normalised."""
+    H, Hk, D, dtype = 4, 2, 64, torch.float16
+    batch = R.Batch(new, old, B=16, lens=lens)
+    query = _query(batch, H, D, dtype, 12)
+    pools = _pools(batch, Hk, D, "16", dtype, "head", 12)
+    (_, k, _), (_, v, _) = pools
+    lambdas, weight = torch.full((H,), 0.3), 1.0 + 0.1 * torch.randn(D, generator=torch.Generator().manual_seed(1))
+    out = _attend(batch, query, pools, 0.17, maps=2, lambdas=lambdas, weight=weight, eps=0.0, out_scale=0.8, longest=longest)
+    refs = R.attention(batch, query, k, v, 0.17, maps=2)
+    blind = (refs[0][1] == 0).all(-1).all(-1)
+    assert bool(blind.any()) and bool((out.cpu()[blind] == 0).all())
+    want = R.differential(refs, lambdas, weight, 0.0, 0.8)
+    bound = R.attention_bound(refs, dtype, dtype, lambdas, weight, 0.0, 0.8)
+    _close(out.cpu()[~blind], want[~blind], bound[~blind])
