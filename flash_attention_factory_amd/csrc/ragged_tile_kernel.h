@@ -543,6 +543,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   };
 
   // ---- the two phases of a step ----
+  // (always inlined: a call would have everything that they work on, accumulators and all, go through memory)
   const float c_all = p.score_scale_log2 * q_mul * (KV8 && !scaled ? p.tensor_scale : 1.f);
   f32x16 x[2];   // scores of the step that softmax comes to next
   u32x4 pb[4];   // weights of the step before it, as the B operands of V^T P^T
@@ -587,7 +588,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
     }
   };
   // scores of step n + 1 and / or values of step n
-  auto matrix_phase = [&](int n, auto with_scores, auto with_values, bool with_stage) {
+  auto matrix_phase = [&](int n, auto with_scores, auto with_values, bool with_stage) __attribute__((always_inline)) {
     constexpr int kFirst = decltype(with_scores)::value ? 0 : kScoreOps;
     constexpr int kLast = decltype(with_values)::value ? kScoreOps + kValueOps : kScoreOps;
     const char *kb = lds + ((n + 1) & 1) * T::kBufferBytes, *vb = lds + (2 + (n & 1)) * T::kBufferBytes;
@@ -609,7 +610,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
       for (int part = (kLast - kFirst + kEvery - 1) / kEvery; part < kStageParts; ++part) stage(n, part);
     }
   };
-  auto softmax = [&](int n) {
+  auto softmax = [&](int n) __attribute__((always_inline)) {
     const int t0 = (step + n) * kTileKeys;
     // register (t, e) holds key t0 + 32 t + 8 (e / 4) + 4 half + e % 4; group 2 t + e / 8 of 16 keys
     float cc[4];
@@ -756,7 +757,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
     issue_k(1);
     meet();
     if (kTurns && late) meet();
-    auto vector_phase = [&](int n, auto with_softmax) {
+    auto vector_phase = [&](int n, auto with_softmax) __attribute__((always_inline)) {
       if (kTurns) meet();
       take_scales(n + 1);
       fetch_scales();
