@@ -6,6 +6,7 @@
 // matrix cores.  Both forms may run for one call; each takes the sequences that are its own.
 #pragma once
 
+#include "kv_cache_write_kernel.h"
 #include "paged_attention_wave.h"
 #include "ragged_batch.h"
 
@@ -84,15 +85,17 @@ template <int MAPS>
 __device__ __forceinline__ bool in_rows_form(const RaggedParams &p, const RaggedSeq &q) {
   return q.n * p.group * MAPS <= p.row_limit;
 }
+// Position that the j-th new token attends from: its own, or the last one that the block table has.
+__device__ __forceinline__ int attends_from(const RaggedSeq &q, int j) { return min(q.pos0 + j, q.ctx - 1); }
 // First key that some new token of the sequence sees.
-__device__ __forceinline__ int first_key(const RaggedParams &p, const RaggedSeq &q) { return max(0, q.pos0 - p.window); }
+__device__ __forceinline__ int first_key(const RaggedParams &p, const RaggedSeq &q) { return max(0, attends_from(q, 0) - p.window); }
 
 // Units of keys that the rows form has to go through for one kv head of a sequence.
 template <int MAPS>
 __device__ __forceinline__ int row_units(const RaggedParams &p, RaggedSeq q) {
   q = ragged_seq_cut(p, q);
   if (q.n <= 0 || !in_rows_form<MAPS>(p, q)) return 0;
-  return max(0, (q.ctx + kRowUnit - 1) / kRowUnit - first_key(p, q) / kRowUnit);
+  return (q.ctx + kRowUnit - 1) / kRowUnit - first_key(p, q) / kRowUnit;
 }
 // Tiles of `rows` rows that the tile form has to go through for one kv head of a sequence.
 template <int MAPS, int ROWS>

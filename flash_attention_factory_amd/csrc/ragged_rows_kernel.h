@@ -42,7 +42,7 @@ template <typename W>
 struct RowColumns {
   float mul;         // what the column's raw scores are multiplied with (fp16 queries: 1)
   float slope_log2;
-  int pos, hi;       // position of the column's token, and the last key that it sees (its own, if the table has that)
+  int pos;           // position that the column's token attends from
   int vis_lo, vis_hi;  // keys that every column sees
   int first;         // before it: keys that no column sees
 };
@@ -74,7 +74,7 @@ __device__ __forceinline__ RowWeights<W> row_soft(W &wa, RowState &st, const Row
 #pragma unroll
     for (int e = 0; e < NT; ++e) {
       const int tok = t0 + (e >> 2) * 16 + 4 * wa.r + (e & 3);
-      if (tok > col.hi || tok < col.pos - p.window) t[e] = -INFINITY;  // select: the pool may hold NaN there
+      if (tok > col.pos || tok < col.pos - p.window) t[e] = -INFINITY;  // select: the pool may hold NaN there
       if (tok >= ctx || tok < col.first) {
 #pragma unroll
         for (int w = 0; w < W::VW; ++w) R.v[e][w] = 0u;
@@ -276,10 +276,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
     const int head = kvh * G + (row - j * G);
     RowColumns<W> col;
     col.mul = 1.f;
-    col.pos = q.pos0 + j;
-    col.hi = min(col.pos, q.ctx - 1);
-    col.vis_hi = min(q.pos0, q.ctx - 1);
-    col.vis_lo = q.pos0 + q.n - 1 - p.window;
+    col.pos = attends_from(q, j);
+    col.vis_hi = attends_from(q, 0);
+    col.vis_lo = q.ctx - 1 - p.window;
     col.first = first_key(p, q);
     col.slope_log2 = (p.mask_flags & kMaskAlibi) && valid ? p.alibi_slopes[head] * kLog2e : 0.f;
     const char *qrow = p.query + (int64_t)(q.first + (valid ? j : 0)) * p.q_token_bytes + (valid ? head : 0) * p.q_head_bytes;

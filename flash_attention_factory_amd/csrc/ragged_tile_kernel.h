@@ -84,7 +84,9 @@ struct RaggedTile {
   // Key of a step that thread row `load_row` loads in a pass.  Where there are more thread rows than keys the surplus ones repeat the
   // others' (what they have loaded is not stored): a key beyond the step's 64 would lie, with blocks of more than 64, as
   // far beyond the end of its block.
-  static __host__ __device__ constexpr int load_key(int pass, int load_row) { return (pass * kRowsPerPass + load_row) & (kTileKeys - 1); }
+  static __host__ __device__ constexpr int load_key(int pass, int load_row) {
+    return kRowsPerPass > kTileKeys ? load_row & (kTileKeys - 1) : pass * kRowsPerPass + load_row;
+  }
 
   // where 16-byte piece c of row `key` of a step lies in its buffer
   static __device__ __forceinline__ int k_at(int key, int c) {
@@ -217,16 +219,22 @@ struct TileSteps {
 template <int ROWS>
 __device__ __forceinline__ TileSteps tile_steps(const RaggedParams &p, const RaggedSeq &q, int tile) {
   const int row0 = tile * ROWS;
-  const int pos_lo = q.pos0 + row0 / p.group, pos_hi = q.pos0 + (min(row0 + ROWS, q.n * p.group) - 1) / p.group;
-  const int last = min(pos_hi, q.ctx - 1);  // (tokens past the block table see what it holds)
+  const int pos_lo = attends_from(q, row0 / p.group), pos_hi = attends_from(q, (min(row0 + ROWS, q.n * p.group) - 1) / p.group);
   TileSteps s;
   s.first = max(0, pos_lo - p.window) / kTileKeys;
-  s.count = last < 0 ? 0 : max(0, last / kTileKeys + 1 - s.first);
+  s.count = pos_hi < 0 ? 0 : pos_hi / kTileKeys + 1 - s.first;
   return s;
 }
 // Where a cut `off` into a tile of cost `cost` falls between its steps.
 __device__ __forceinline__ int cut_step(int64_t off, int64_t cost, int steps) {
   return min((int)((float)off * (float)steps / (float)cost), steps);
+}
+
+// The same number, as one that the compiler knows nothing of: what is worked out from it at a tile's end is not kept in registers from
+// the tile's start, where it has been worked out before.  Two maps in a work-group for each tile have registers enough.
+__device__ __forceinline__ int anew(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // What the wavefronts of a work-group have of a tile's rows: lane (half, col) holds elements d = 32 dt + 8 k + 4 half + e of row
@@ -235,9 +243,9 @@ __device__ __forceinline__ int cut_step(int64_t off, int64_t cost, int steps) {
 // All wavefronts call it; LDS holds nothing else any more.
 template <int D, int MAPS, int NW>
 __device__ __forceinline__ void tile_finish(const RaggedParams &p, const RaggedSeq &q, int kvh, int row0, f32x16 (&acc)[D / 32], float l,
-                                            char *lds) {
+                                            char *lds, int lane) {
   constexpr int DT = D / 32, kRows = NW * 32 / MAPS;
-  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  const int half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int map = MAPS == 2 ? wave / (NW / 2) : 0, strip = MAPS == 2 ? wave % (NW / 2) : wave;
   const int all_rows = q.n * p.group, row = min(row0 + strip * 32 + col, all_rows - 1);
@@ -311,6 +319,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   constexpr bool KV8 = T::KV8;
   constexpr int KS = D / MAPS / 16;   // k-steps of the scores
   constexpr int DT = D / 32;          // d-tiles of the output
+  constexpr bool kAnew = LINE || MAPS == 1;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -384,17 +393,16 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const bool whole = !LINE || (from == 0 && until == of_tile.count);
   if (whole || from < until) {  // (a tile that sees no keys is whole: its rows get zeros)
   const int all_rows = q.n * G, row0 = tile * T::kRows;
-  const int pos0 = q.pos0, last_key = q.ctx - 1;
   const int step = of_tile.first + from, step_end = of_tile.first + until;
 
   // this lane's row (rows past the end repeat the last one and are not stored)
   const int my_row = row0 + strip * 32 + col;
   const int row = min(my_row, all_rows - 1);
   const int j = row / G, head = kvh * G + (row - j * G);
-  const int pos = pos0 + j;
+  const int pos = attends_from(q, j);
   const int wave_row = row0 + strip * 32;
   const bool wave_live = wave_row < all_rows;
-  const int wave_lo = pos0 + min(wave_row, all_rows - 1) / G, wave_hi = pos0 + (min(wave_row + 32, all_rows) - 1) / G;
+  const int wave_lo = attends_from(q, min(wave_row, all_rows - 1) / G), wave_hi = attends_from(q, (min(wave_row + 32, all_rows) - 1) / G);
 
   // queries: the B operand, d = 16 c + 8 half .. of the map's part
   u32x4 qv[KS];
@@ -436,8 +444,8 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const bool loads = T::kRowsPerPass <= kTileKeys || load_row < kTileKeys;
   const int last_col = p.b.max_blocks_per_seq - 1, in_block = (1 << p.b.block_shift) - 1;
   const int steps = step_end - step;
-  const int seen_lo = max(0, pos0 + row0 / G - p.window);  // keys that some row of the tile sees
-  const int seen_keys = max(0, min(pos0 + (min(row0 + T::kRows, all_rows) - 1) / G, last_key) + 1 - seen_lo);
+  const int seen_lo = max(0, attends_from(q, row0 / G) - p.window);  // keys that some row of the tile sees
+  const int seen_keys = attends_from(q, (min(row0 + T::kRows, all_rows) - 1) / G) + 1 - seen_lo;
   // Blocks of this thread's rows: of the next step of K as the table has them (cut to the pool where they are used, since
   // arithmetic here would wait for the load, and for every load before it), and of the next step of V, one step behind.
   int32_t kid[T::kPasses], vid[T::kPasses];
@@ -552,7 +560,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   u32x4 rest[kTwo ? 4 : 1];  // what their rounding left
   // the steps of which this wavefront sees anything: see_lo .. see_hi - 1 (the same for all its lanes)
   const int see_lo = wave_live ? max(0, (wave_lo - p.window) / kTileKeys - step) : steps;
-  const int see_hi = wave_live && wave_hi >= 0 ? min(steps, min(wave_hi, last_key) / kTileKeys + 1 - step) : 0;
+  const int see_hi = wave_live && wave_hi >= 0 ? min(steps, wave_hi / kTileKeys + 1 - step) : 0;
   // Where this lane reads K (16-byte piece of key `col`) and V (8 bytes of key 4 half + i / 4) within a buffer; the swizzles are
   // exclusive-ors, so a k-step or d-tile is one more of them and keys further on are an offset (see k_at, v_at).
   const int i16 = lane & 15;
@@ -635,8 +643,8 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
 #pragma unroll
       for (int k = 0; k < 4; ++k) cc[k] = 1.f;
     }
-    if (t0 + kTileKeys - 1 > min(wave_lo, last_key) || t0 < wave_hi - p.window) {
-      const int hi = min(pos, last_key) - t0 - 4 * half, lo = pos - p.window - t0 - 4 * half;
+    if (t0 + kTileKeys - 1 > wave_lo || t0 < wave_hi - p.window) {
+      const int hi = pos - t0 - 4 * half, lo = hi - p.window;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -805,7 +813,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   }
   if (whole) {
     meet();  // nobody reads V any more
-    tile_finish<D, MAPS, NW>(p, q, kvh, row0, acc, l, lds);
+    tile_finish<D, MAPS, NW>(p, q, kvh, row0, acc, l, lds, kAnew ? anew(lane) : lane);
   } else {
     // a piece of a tile: as it lies in the registers, 1 KiB at a time (slots: see ragged_tile_merge_kernel)
     const int64_t slot = 2 * (int64_t)g + (first_piece ? 0 : 1);
@@ -887,7 +895,7 @@ __global__ void __launch_bounds__(NW * 64) ragged_tile_merge_kernel(const Ragged
     from = until;
     if (last) break;
   }
-  tile_finish<D, MAPS, NW>(p, q, place.kvh, place.tile * ROWS, acc, l, lds);
+  tile_finish<D, MAPS, NW>(p, q, place.kvh, place.tile * ROWS, acc, l, lds, lane);
 }
 
 }  // namespace fa

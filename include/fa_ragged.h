@@ -19,7 +19,7 @@
  * Block ids outside the pool are never read from or written to (reads take a block of the pool
  * instead, writes are left out); a token at a negative position (context_lens[s] < n) is not stored
  * and its result is zero; one at a position past the table's columns is not stored either, and
- * sees the keys that the table has.
+ * attends as one at the table's last position would.
  * Pool rows that none of the call's tokens sees -- past the context, before every token's window,
  * unused blocks -- and scales of such blocks may hold anything.  Keys that a token does not see
  * have no weight whatever they are; values of one token that are infinite or NaN can reach earlier new

@@ -169,13 +169,13 @@ def test_append_of_more_tokens_in_query_start_than_rows(new, old, kv):
 
 
 def _beyond(batch, query, k, v, scale, columns, maps=1, window=-1, slopes=None):
-    """64-bit form for tables of `columns` columns: positions are the lengths', keys are those of the table."""
+    """64-bit form for tables of `columns` columns: tokens past it attend from its last position."""
     T, H, D = query.shape
     Hk, B, d = k.size(2), batch.B, D // maps
     got = [(torch.zeros(T, H, D, dtype=torch.float64), torch.zeros(T, H, D, dtype=torch.float64)) for _ in range(maps)]
     for s, (n, ctx) in enumerate(zip(batch.new, batch.lens)):
         a, keys = int(batch.start[s]), min(ctx, columns * B)
-        t, pos = torch.arange(keys), torch.arange(ctx - n, ctx)
+        t, pos = torch.arange(keys), torch.arange(ctx - n, ctx).clamp_max(keys - 1)
         ids = batch.tables[s, t // B].long()
         sees = t[None] <= pos[:, None]
         if window >= 0:
