@@ -138,7 +138,8 @@ __device__ __forceinline__ float soft_capped(float t, float cap) {
   return cap * kLog2e * (1.0f - 2.0f * __builtin_amdgcn_rcpf(e2 + 1.0f));
 }
 
-// Sink logit of a head in base-2 units.
+// Sink logit of a head in base-2 units.  It joins maximum and sum at the end of a piece: as the reference of the weights, which go to
+// the matrix cores in 16 bits, one far above the scores would leave them few bits.
 __device__ __forceinline__ float sink_log2(const RaggedParams &p, int head) {
   return (p.q_bf16 ? load_scalar16<BF16>(reinterpret_cast<const char *>(p.sinks) + head * 2)
                    : load_scalar16<F16>(reinterpret_cast<const char *>(p.sinks) + head * 2)) * kLog2e;

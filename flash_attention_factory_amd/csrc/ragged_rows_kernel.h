@@ -293,10 +293,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
     RowState st;
     st.m = st.mt = st.mv = st.mvt = -INFINITY;
     st.l = 0.f;
-    if (p.sinks != nullptr && valid && first == 0 && wave == 0) {
-      st.m = st.mt = sink_log2(p, head);
-      st.l = r == 0 ? 1.f : 0.f;
-    }
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) wa.acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -342,16 +338,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
     // Merge: sums and weights against the true maximum, then the wavefronts' states through LDS.  Wavefront w keeps the
     // slice [w * SL, (w + 1) * SL) of every lane's NR consecutive elements.
     {
-      const float to = st.mt == -INFINITY ? 0.f : st.mt;
+      const float sink = MAPS == 1 && p.sinks != nullptr && valid && first == 0 && wave == 0 ? sink_log2(p, head) : -INFINITY;
+      const float top = fmaxf(st.mt, sink), to = top == -INFINITY ? 0.f : top;
       const float from = KV8 && p.block_scales ? st.mv : st.m;
       const float f = from == -INFINITY ? 0.f : fast_exp2(from - to);
-      st.l = rows_sum(st.l) * (st.m == -INFINITY ? 0.f : fast_exp2(st.m - to));
+      st.l = rows_sum(st.l) * (st.m == -INFINITY ? 0.f : fast_exp2(st.m - to)) + fast_exp2(sink - to);
       float (*sm_acc)[NR][64] = reinterpret_cast<float (*)[NR][64]>(lds);
       float (*sm_m)[16] = reinterpret_cast<float (*)[16]>(lds + NW * NR * 64);
       float (*sm_l)[16] = reinterpret_cast<float (*)[16]>(lds + NW * NR * 64 + NW * 16);
       __syncthreads();  // (the piece before this one has been read)
       if (r == 0) {
-        sm_m[wave][i] = st.mt;
+        sm_m[wave][i] = top;
         sm_l[wave][i] = st.l;
       }
 #pragma unroll

@@ -428,10 +428,6 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const float slope = EXT && (p.mask_flags & kMaskAlibi) ? p.alibi_slopes[head] * kLog2e : 0.f;
 
   float m = -INFINITY, mt = -INFINITY, l = 0.f, mv = -INFINITY, mvt = -INFINITY;
-  if (p.sinks != nullptr && from == 0) {
-    m = mt = sink_log2(p, head);
-    l = half == 0 ? 1.f : 0.f;
-  }
   f32x16 acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -803,11 +799,20 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   // ---- results: element (dt, e) of a lane is d = 32 dt + 8 (e / 4) + 4 half + e % 4 of its row ----
   l = halves_sum(l);
   {
+    float sink = -INFINITY;
+    if constexpr (MAPS == 1) {
+      if (p.sinks != nullptr && from == 0) {
+        const int row = min(row0 + strip * 32 + (kAnew ? anew(col) : col), all_rows - 1);
+        sink = sink_log2(p, kvh * G + row % G);
+        mt = fmaxf(mt, sink);
+      }
+    }
     const float to = mt == -INFINITY ? 0.f : mt;
     const float from = KV8 ? mv : m;
     const float v_mul = !KV8 || p.block_scales ? 1.f : p.v_scales ? load_uniform_f32(p.v_scales + kvh) : p.tensor_scale;
     const float f = (from == -INFINITY ? 0.f : fast_exp2(from - to)) * v_mul;
     l *= m == -INFINITY ? 0.f : fast_exp2(m - to);
+    if constexpr (MAPS == 1) l += fast_exp2(sink - to);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
   }

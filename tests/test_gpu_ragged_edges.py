@@ -277,3 +277,28 @@ def test_differential_without_epsilon_and_without_keys(new, old, lens, longest):
     want = R.differential(refs, lambdas, weight, 0.0, 0.8)
     bound = R.attention_bound(refs, dtype, dtype, lambdas, weight, 0.0, 0.8)
     _close(out.cpu()[~blind], want[~blind], bound[~blind])
+
+
+# ---- sinks far above the scores ----
+
+@pytest.mark.parametrize("kv,dtype", [("16", torch.float16), ("16", torch.bfloat16), ("i8", torch.bfloat16), ("e4m3", torch.bfloat16)])
+@pytest.mark.parametrize("new,old", [([1, 2], [400, 450]), ([1, 1], [1500, 900]), ([40, 3], [700, 900]), ([33], [3000])])
+def test_sinks_far_above_the_scores(kv, dtype, new, old):
+    """A sink takes its share of the sum and leaves the bits of the others' weights alone."""
+    H, Hk, D = 8, 2, 64
+    batch = R.Batch(new, old, B=16)
+    query = _query(batch, H, D, dtype, 13, 0.1)
+    pools = _pools(batch, Hk, D, kv, dtype, "head", 13)
+    (_, k, _), (_, v, _) = pools
+    v = v.abs()  # sums that do not cancel
+    if kv == "16":
+        pools[1] = (pools[1][0].abs(), None, None)
+    elif kv == "i8":
+        pools[1] = (pools[1][0].abs(), None, pools[1][2])
+    else:
+        pools[1] = ((pools[1][0].view(torch.uint8) & 0x7f).view(pools[1][0].dtype), None, pools[1][2])
+    sinks = torch.linspace(8.0, 15.0, H).to(dtype)
+    out = _attend(batch, query, pools, 0.125, sinks=sinks)
+    refs = R.attention(batch, query, k, v, 0.125, sinks=sinks)
+    bound = R.attention_bound(refs, dtype, dtype if kv == "16" else torch.float16) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    _close(out, refs[0][0], bound)
