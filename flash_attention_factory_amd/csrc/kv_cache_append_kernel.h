@@ -10,8 +10,8 @@
 //   scale' = max(scale, max|x| * (1 / 127) over the new rows of the block, 2^-126), scale = 0 in a block whose first row is new;
 //   rows that were there before: byte' = rint(byte * (scale / scale')), touched only where the scale grew;
 //   new rows: byte = rint(x * (1 / scale')).
-// One wavefront owns a (block, kv head) of the new tokens, finds the largest value of its rows, and writes them: no atomics, and
-// the result does not depend on the order of anything.
+// One, two or four wavefronts of a work-group, by the size of a block, own the new rows of (block, kv head, K or V): they find the largest
+// value, by way of LDS where they are several, and write the rows.  No atomics, and the result does not depend on the order of anything.
 #pragma once
 
 #include <type_traits>
@@ -38,7 +38,6 @@ struct KvAppendParams {
   int32_t rotary;          // R
   int32_t num_heads;
   int32_t num_kv_heads;
-  int32_t head_size;
   int32_t block_size;
   int64_t q_token_bytes, q_head_bytes;      // of query
   int64_t qo_token_bytes, qo_head_bytes;    // of query_out
@@ -92,7 +91,7 @@ __device__ __forceinline__ void rotate_halves(float (&x)[8], float (&y)[8], cons
 
 // The two 8-element pieces of unit `u` of a row (element offsets): with pairs half the rotated elements apart, unit u of the
 // rotated part is the pieces at 8u and R/2 + 8u, whose elements are partners; beyond it, and with pairs of neighbours
-// everywhere, two pieces one behind the other.  (R is a multiple of 16, a row of 32.)
+// everywhere, two pieces one behind the other.  (R is a multiple of 16, and so is a row.)
 template <bool INTER>
 __device__ __forceinline__ void unit_pieces(int u, int rotary, int &e0, int &e1) {
   const int half = rotary >> 1;

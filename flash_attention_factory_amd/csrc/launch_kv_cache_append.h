@@ -88,7 +88,6 @@ inline fa_status launch_kv_cache_append(const void *query, void *query_out, cons
   p.rotary = s->rotary_dim;
   p.num_heads = s->num_heads;
   p.num_kv_heads = s->num_kv_heads;
-  p.head_size = s->head_size;
   p.block_size = s->block_size;
   p.q_token_bytes = s->query_token_stride * 2;
   p.q_head_bytes = s->query_head_stride * 2;
@@ -132,9 +131,12 @@ inline fa_status launch_kv_cache_append(const void *query, void *query_out, cons
     // blocks of few tokens leave nothing for more than one wavefront to do
     const int batch = 2 * std::max(1, 64 / units);
     p.team = s->block_size <= batch ? 1 : s->block_size <= 2 * batch ? 2 : 4;
-    // With few tokens every one may own its block: a work-group each.  With many, a block's worth of tokens together holds
-    // about one owner.
-    p.window = T <= 1024 ? 1 : std::min(s->block_size, kAppendMaxTokens);
+    // A work-group for each token finds its owner at once, and most find none where sequences bring many tokens; one for a block's
+    // worth of tokens goes through its owners one after the other.  us of the two (8 kv heads of 128): single tokens of 512
+    // sequences, blocks of 16: 11 and 29, of 1536 29 and 35, of 2048 39 and 35; blocks of 64: 26 and 100, 80 and 108, 113 and
+    // 108.  500 times 2: 18 and 18 (blocks of 64: 46 and 55), 700 times 2 24 and 21 (65 and 59), 250 times 4 17 and 13 (39 and 33); prompts
+    // of 256 tokens 9 and 9 (10 and 11), of 1000 16 and 9 (30 and 11), three of 4000 118 and 21 (315 and 30).
+    p.window = T <= std::min<int64_t>(512 + (int64_t)s->num_seqs, 1536) ? 1 : std::min(s->block_size, kAppendMaxTokens);
     const int teams = 4 / p.team;
     const int64_t unit_groups = (2 * (int64_t)s->num_kv_heads + teams - 1) / teams;
     const int64_t kv_groups = (T + p.window - 1) / p.window * unit_groups;

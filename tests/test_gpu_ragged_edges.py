@@ -302,3 +302,22 @@ def test_sinks_far_above_the_scores(kv, dtype, new, old):
     refs = R.attention(batch, query, k, v, 0.125, sinks=sinks)
     bound = R.attention_bound(refs, dtype, dtype if kv == "16" else torch.float16) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
     _close(out, refs[0][0], bound)
+
+
+# ---- many sequences ----
+
+@pytest.mark.parametrize("B", [16, 64])
+@pytest.mark.parametrize("n", [1100, 1700])
+def test_append_of_many_single_tokens(B, n):
+    """Sequences of one token each, or hardly more, every one of which owns its block: a work-group each, and several to one."""
+    Hk, D, dtype, dev = 1, 64, torch.bfloat16, "cuda"
+    batch = R.Batch([1 if k % 9 else 2 for k in range(n)], [(k * 13) % 40 for k in range(n)], B=B)
+    g = torch.Generator().manual_seed(16)
+    fused = torch.randn(batch.T, 2 * Hk, D, generator=g).to(dtype)
+    pools = [torch.randint(-127, 128, (batch.blocks, B, Hk, D), generator=g, dtype=torch.int8) for _ in range(2)]
+    scales = [0.002 + 0.03 * torch.rand(batch.blocks, Hk, generator=g) for _ in range(2)]
+    d_rows, d_pools, d_scales = fused.to(dev), [p.to(dev) for p in pools], [s.to(dev) for s in scales]
+    torch.ops.fa_amd.kv_cache_append(d_rows[:, :Hk], d_rows[:, Hk:], *d_pools, *batch.on(dev), None, None, None, *d_scales)
+    R.append(batch, fused[:, :Hk], fused[:, Hk:], *pools, None, False, *scales)
+    for got, ref in zip(d_pools + d_scales, pools + scales):
+        assert torch.equal(got.cpu(), ref)
