@@ -16,7 +16,7 @@ LEAST = 2.0 ** -126  # the scale that the append gives to a block of zeros
 
 
 def _attend(batch, query, pools, scale, *, maps=1, most=None, longest=0, window=-1, sinks=None, slopes=None, lambdas=None, weight=None,
-            eps=1e-5, out_scale=1.0, fp8_scale=1.0):
+            eps=1e-5, out_scale=1.0, fp8_scale=1.0, softcap=0.0):
     """The operator's result; rows that it leaves alone are NaN."""
     (kp, _, ks), (vp, _, vs) = pools
     dev = "cuda"
@@ -27,7 +27,8 @@ def _attend(batch, query, pools, scale, *, maps=1, most=None, longest=0, window=
     if maps == 1:
         torch.ops.fa_amd.paged_attention_ragged(*args, most, longest, fp8_scale=fp8_scale, k_scales=ks, v_scales=vs,
                                                 sinks=None if sinks is None else sinks.to(dev),
-                                                alibi_slopes=None if slopes is None else slopes.to(dev), window_left=window)
+                                                alibi_slopes=None if slopes is None else slopes.to(dev), softcap=softcap,
+                                                window_left=window)
     else:
         torch.ops.fa_amd.paged_attention_differential(*args, lambdas.to(dev), None if weight is None else weight.to(dev), most, longest,
                                                       norm_eps=eps, out_scale=out_scale, k_scales=ks, v_scales=vs, window_left=window)
@@ -302,6 +303,74 @@ def test_sinks_far_above_the_scores(kv, dtype, new, old):
     refs = R.attention(batch, query, k, v, 0.125, sinks=sinks)
     bound = R.attention_bound(refs, dtype, dtype if kv == "16" else torch.float16) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
     _close(out, refs[0][0], bound)
+
+
+# ---- value scales of very different size ----
+
+@pytest.mark.parametrize("new,old", [([1] * 4, [100, 40, 300, 800]), ([40, 1, 70], [100, 200, 20]), ([33], [1500])])
+@pytest.mark.parametrize("small,zeros", [(LEAST, True), (2.0 ** -100, False), (0.0, True)])
+@pytest.mark.parametrize("every", [2, 5])
+def test_value_scales_that_lie_binary_orders_apart(new, old, small, zeros, every):
+    """Blocks of zero (or hardly any) values among others: their keys count in the sum like all the others."""
+    H, Hk, D, dtype = 8, 2, 64, torch.bfloat16
+    batch = R.Batch(new, old, B=16)
+    query = _query(batch, H, D, dtype, 14)
+    pools = _pools(batch, Hk, D, "i8", dtype, "head", 14)
+    (kp, k, ks), (vp, v, vs) = pools
+    some = torch.arange(batch.blocks) % every == 0
+    there = (some & batch.used.any(1)).cuda()
+    vs[there] = small
+    if zeros:
+        vp[there] = 0
+    v = v.masked_fill(some[:, None, None, None], 0.0)
+    for maps in (1, 2):
+        lambdas = torch.full((H,), 0.4)
+        out = _attend(batch, query, [(kp, k, ks), (vp, v, vs)], 0.125, maps=maps, lambdas=lambdas)
+        refs = R.attention(batch, query, k, v, 0.125, maps=maps)
+        if maps == 1:
+            _close(out, refs[0][0], R.attention_bound(refs, dtype, torch.float16))
+        else:
+            _close(out, R.differential(refs, lambdas, None, 0.0, 1.0), R.attention_bound(refs, dtype, torch.float16, lambdas))
+
+
+# ---- the difference of two maps that are nearly alike ----
+
+def _alike(batch, H, Hk, D, dtype, seed):
+    """Queries whose halves differ by some hundredths, keys whose halves are the same: the maps differ little, and the rounding of
+    their weights has nothing in common."""
+    g = torch.Generator().manual_seed(seed)
+    half = 0.3 * torch.randn(batch.T, H, D // 2, generator=g)
+    query = torch.cat([half, half + 0.03 * torch.randn(batch.T, H, D // 2, generator=g)], -1).to(dtype)
+    k = torch.randn(batch.blocks, batch.B, Hk, D // 2, generator=g)
+    k = torch.cat([k, k], -1).to(dtype)
+    v = torch.randn(batch.blocks, batch.B, Hk, D, generator=g).to(dtype)
+    return query, k, v
+
+
+def _alike_bound(refs, lambdas, dtype, weights):
+    """Normalised difference (no epsilon, no weights of the norm): weights in two parts carry the square of one rounding, sums
+    of 32 products of about 1 in 32 bits and their exponentials 2e-5; the result is rounded to its type once."""
+    (o1, a1), (o2, a2) = refs
+    o = o1 - lambdas.double()[:, None] * o2
+    e = (weights + 2e-5) * (a1 + lambdas.double()[:, None] * a2)
+    rms = torch.sqrt((o * o).mean(-1, keepdim=True) + 1e-5)
+    off = e.square().mean(-1, keepdim=True).sqrt() / rms
+    return (e + o.abs() * off * 1.1 + R.UNIT[dtype] * o.abs()) / rms + 1e-6
+
+
+@pytest.mark.parametrize("dtype,new,old", [(torch.bfloat16, [1, 2, 1], [5, 9, 30]), (torch.float16, [1, 2, 1], [5, 9, 30]),
+                                           (torch.bfloat16, [20, 33], [0, 0]), (torch.bfloat16, [1], [700])])
+def test_weights_in_two_parts(dtype, new, old):
+    """Over 16-bit pools the weights of two maps go to the matrix cores in two parts (prompts of fp16: in one)."""
+    H, Hk, D = 4, 2, 64
+    batch = R.Batch(new, old, B=16)
+    query, k, v = _alike(batch, H, Hk, D, dtype, 15)
+    lambdas = torch.full((H,), 0.95)
+    refs = R.attention(batch, query, k.double(), v.double(), 0.17, maps=2)
+    out = _attend(batch, query, [(k.cuda(), None, None), (v.cuda(), None, None)], 0.17, maps=2, lambdas=lambdas, weight=torch.ones(D))
+    want = R.differential(refs, lambdas, torch.ones(D), 1e-5, 1.0)
+    _close(out, want, _alike_bound(refs, lambdas, dtype, R.UNIT[dtype] ** 2))
+
 
 
 # ---- many sequences ----
