@@ -74,6 +74,11 @@ def check_scales(k_scales: Optional[torch.Tensor], v_scales: Optional[torch.Tens
               "(per block and kv head)")
 
 
+def bound(v: int) -> int:
+    """A bound of the caller's (a window, a number of keys) for a 32-bit field: beyond 2^31 - 1 it bounds nothing more."""
+    return max(-1, min(int(v), 0x7fffffff))
+
+
 def pointer(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -101,5 +106,5 @@ def attention_shape(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Ten
     sh.max_blocks_per_seq = block_tables.size(1)
     sh.kv_block_stride, sh.kv_token_stride, sh.kv_head_stride = key_cache.stride()[:3]
     sh.query_token_stride, sh.query_head_stride = query.stride()[:2]
-    sh.max_query_len, sh.max_context_len = int(max_query_len), int(max_context_len)
+    sh.max_query_len, sh.max_context_len = bound(max_query_len), bound(max_context_len)
     return sh

@@ -48,7 +48,7 @@ def run(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_c
     op = _cabi.Options()
     if window_left >= 0:
         op.mask_flags |= _cabi.FA_MASK_WINDOW
-        op.window_left = int(window_left)
+        op.window_left = _ragged.bound(window_left)
     if sh.cache_dtype == _cabi.FA_KV_CACHE_16BIT and k_scales is not None:
         raise _ragged.bad("k_scales / v_scales belong to byte pools", _cabi.FA_ERR_UNSUPPORTED_DTYPE)
     op.kv_scale_mode = _ragged.check_scales(k_scales, v_scales, sh.num_kv_heads, sh.num_pool_blocks)

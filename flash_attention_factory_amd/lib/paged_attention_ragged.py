@@ -51,7 +51,7 @@ def run(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_c
         op.softcap = softcap
     if window_left >= 0:
         op.mask_flags |= _cabi.FA_MASK_WINDOW
-        op.window_left = int(window_left)
+        op.window_left = _ragged.bound(window_left)
     if sh.cache_dtype == _cabi.FA_KV_CACHE_16BIT and k_scales is not None:
         raise _ragged.bad("k_scales / v_scales belong to byte pools", _cabi.FA_ERR_UNSUPPORTED_DTYPE)
     op.fp8_scale = fp8_scale

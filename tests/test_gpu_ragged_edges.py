@@ -390,3 +390,21 @@ def test_append_of_many_single_tokens(B, n):
     R.append(batch, fused[:, :Hk], fused[:, Hk:], *pools, None, False, *scales)
     for got, ref in zip(d_pools + d_scales, pools + scales):
         assert torch.equal(got.cpu(), ref)
+
+
+# ---- bounds beyond 32 bits ----
+
+@pytest.mark.parametrize("new,old", [([1, 2], [40, 30]), ([40, 1], [50, 7])])
+@pytest.mark.parametrize("maps", [1, 2])
+def test_bounds_beyond_32_bits_bound_nothing(new, old, maps):
+    """A window, a number of tokens or keys of 2^32 and a few is not one of those few."""
+    H, Hk, D, dtype = 4, 2, 64, torch.float16
+    batch = R.Batch(new, old, B=16)
+    query = _query(batch, H, D, dtype, 17)
+    pools = _pools(batch, Hk, D, "16", dtype, "head", 17)
+    (_, k, _), (_, v, _) = pools
+    lambdas = torch.full((H,), 0.4)
+    out = _attend(batch, query, pools, 0.125, maps=maps, lambdas=lambdas, most=(1 << 32) + 1, longest=(1 << 32) + 3, window=(1 << 32) + 5)
+    refs = R.attention(batch, query, k, v, 0.125, maps=maps)
+    want = refs[0][0] if maps == 1 else R.differential(refs, lambdas, None, 0.0, 1.0)
+    _close(out, want, R.attention_bound(refs, dtype, dtype, None if maps == 1 else lambdas))
