@@ -243,14 +243,14 @@ inline fa_status launch_ragged_attention(void *out, const void *query, const voi
   p.v_scales = mode != FA_KV_SCALE_TENSOR ? o->v_scales : nullptr;
   p.scale_pitch = mode == FA_KV_SCALE_BLOCK ? s->num_kv_heads : 0;
   p.block_scales = mode == FA_KV_SCALE_BLOCK;
-  p.tensor_scale = kv8 && o && o->fp8_scale != 0.f ? o->fp8_scale : 1.0f;
+  p.tensor_scale = kv8 && mode == FA_KV_SCALE_TENSOR && o && o->fp8_scale != 0.f ? o->fp8_scale : 1.0f;
   p.sinks = o ? o->sinks : nullptr;
   p.alibi_slopes = o ? o->alibi_slopes : nullptr;
   p.softcap = o ? o->softcap : 0.f;
   p.window = (flags & FA_MASK_WINDOW) ? std::min<int32_t>(o->window_left, kNoWindow) : kNoWindow;
   p.mask_flags = flags & (FA_MASK_ALIBI | FA_MASK_SOFTCAP);
   p.score_scale_log2 = std::abs(scale) * kLog2e;
-  p.query_flip = scale < 0.f ? 0x80008000u : 0u;
+  p.query_flip = (scale < 0.f) != (p.tensor_scale < 0.f) ? 0x80008000u : 0u;
   p.q_bf16 = s->q_dtype == FA_DTYPE_BF16;
   p.num_heads = s->num_heads;
   p.num_kv_heads = s->num_kv_heads;

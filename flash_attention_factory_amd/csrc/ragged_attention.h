@@ -22,14 +22,14 @@ struct RaggedParams {
   const float *v_scales;
   int32_t scale_pitch;
   int32_t block_scales;         // scales differ from block to block
-  float tensor_scale;           // byte pools without scale arrays
+  float tensor_scale;           // byte pools without scale arrays: of V, and, but for its sign, of K
   const void *sinks;
   const float *alibi_slopes;
   float softcap;
   int32_t window;               // keys before a token's own that it sees; INT32_MAX / 2 without a window
   int32_t mask_flags;           // kMaskAlibi | kMaskSoftcap (the window is in `window`)
   float score_scale_log2;       // |scale| * log2(e)
-  uint32_t query_flip;          // 0x80008000 for a negative scale: the queries change their sign instead
+  uint32_t query_flip;          // 0x80008000 for negative scores (scale x tensor_scale): the queries change their sign instead
   int32_t q_bf16;               // type of query and out: bf16, or fp16
   int32_t num_heads, num_kv_heads, group;
   int32_t max_query_len;

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) r
         x.lv[t] = 0.f;
         if constexpr (KV8) {
           if (p.k_scales == nullptr) {
-            x.k[t] *= p.tensor_scale;
+            x.k[t] *= fabsf(p.tensor_scale);
           } else {
             const int64_t idx = (int64_t)ids.v[t] * p.scale_pitch + kvh;
             const int tok = c * W::CT + t * 16;

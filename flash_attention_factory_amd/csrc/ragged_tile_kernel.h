@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
 
   // ---- the two phases of a step ----
   // (always inlined: a call would have everything that they work on, accumulators and all, go through memory)
-  const float c_all = p.score_scale_log2 * q_mul * (KV8 && !scaled ? p.tensor_scale : 1.f);
+  const float c_all = p.score_scale_log2 * q_mul * (KV8 && !scaled ? fabsf(p.tensor_scale) : 1.f);
   f32x16 x[2];   // scores of the step that softmax comes to next
   u32x4 pb[4];   // weights of the step before it, as the B operands of V^T P^T
   // (here the second part is products: prompts with two maps 64 us without, 80 with it.  bf16 takes it, with its 8 bits; fp16 does not)

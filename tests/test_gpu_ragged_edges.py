@@ -408,3 +408,21 @@ def test_bounds_beyond_32_bits_bound_nothing(new, old, maps):
     refs = R.attention(batch, query, k, v, 0.125, maps=maps)
     want = refs[0][0] if maps == 1 else R.differential(refs, lambdas, None, 0.0, 1.0)
     _close(out, want, R.attention_bound(refs, dtype, dtype, None if maps == 1 else lambdas))
+
+
+# ---- a scalar scale below zero ----
+
+@pytest.mark.parametrize("kv", ["e5m2", "e4m3"])
+@pytest.mark.parametrize("new,old", [([1, 2], [40, 300]), ([40, 1], [50, 7]), ([33], [1500])])
+@pytest.mark.parametrize("scale", [0.125, -0.125])
+@pytest.mark.parametrize("softcap", [0.0, 3.0])
+def test_scalar_scale_below_zero(kv, new, old, scale, softcap):
+    """fp8_scale multiplies keys and values, whatever its sign, as in the other operators over FP8 pools."""
+    H, Hk, D, dtype = 4, 2, 64, torch.bfloat16
+    batch = R.Batch(new, old, B=16)
+    query = _query(batch, H, D, dtype, 18, 8.0)  # scores that spread over tens of binary orders
+    pools = _pools(batch, Hk, D, kv, dtype, "head", 18, None)
+    (_, k, _), (_, v, _) = pools
+    out = _attend(batch, query, pools, scale, fp8_scale=-0.5, softcap=softcap)
+    refs = R.attention(batch, query, k * -0.5, v * -0.5, scale, softcap=softcap)
+    _close(out, refs[0][0], R.attention_bound(refs, dtype, torch.float16))
