@@ -90,6 +90,11 @@ class Server:
 
     def serve(self, prompts: Sequence[Sequence[int]], answer: int, piece: int = 256) -> List[List[int]]:
         """Greedy answers of ``answer`` tokens; a step takes at most ``piece`` tokens of each prompt."""
+        lengths = [len(prompt) + max(answer, 1) - 1 for prompt in prompts]  # tokens in the pools at the end
+        if piece < 1 or not all(prompts) or max(lengths, default=0) > self.max_length:
+            raise ValueError(f"prompts hold at least one token, with their answers at most {self.max_length}, and a piece one")
+        if sum(-(-n // BLOCK) for n in lengths) > len(self.free):
+            raise ValueError(f"the requests need more blocks than the {len(self.free)} that are free")
         answers: List[List[int]] = [[] for _ in prompts]
         tables: List[List[int]] = [[] for _ in prompts]
         done = [0] * len(prompts)  # tokens in the pools
