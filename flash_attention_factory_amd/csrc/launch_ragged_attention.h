@@ -84,17 +84,19 @@ inline RaggedPlan ragged_plan(const fa_ragged_shape &s, int maps, int cus) {
   if (r.tiles) {
     // 8 wavefronts halve what K and V cost per row, and take turns in the matrix phase; 4 start and end a tile sooner, and two
     // such work-groups share a compute unit.  4 where rows do not fill more or keys are few: one prompt of 1000 tokens (8 kv heads, 4
-    // query heads each, integers) 33 us with 4, 40 with 8; 16 such 230 and 239; 64 new tokens of 16 sequences of 1000 keys
-    // 37 and 45; 8 prompts of 2000 tokens 371 and 357; of 3000 763 and 725; 300 new tokens of 64 sequences of 2300 keys 927 and 864.
+    // query heads each, integers) 32 us with 4, 38 with 8; 16 such 225 and 226; 64 new tokens of 16 sequences of 1000 keys
+    // 33 and 40; 8 prompts of 1400 tokens 191 and 182; of 1700 265 and 254; of 3000 757 and 717; 100 new tokens of 64 sequences of 2300
+    // keys 370 and 343, 30 new tokens 120 and 134.  16-bit pools: 29 and 34, 219 and 214, 30 and 38, 178 and 171, 254 and 243, 714 and
+    // 667, 366 and 335, 133 and 142.  Two maps, five prompts of 513 to 1546 tokens: fp16 78 and 76, bf16 88 and 87.
     r.wavefronts = most * G * maps <= 128 || keys <= 1536 ? 4 : 8;
     r.tile_rows = r.wavefronts * 32 / maps;
     const int64_t each = (most * G + r.tile_rows - 1) / r.tile_rows;
     r.tile_bound = equal ? S * each : std::min(S * each, T * G / r.tile_rows + S);
     // Tiles for each compute unit: from two on, a work-group each, longest first, keeps them all busy.  With fewer, the longest
     // tile (or two one after the other) leaves compute units idle for so many keys; shares of a line do not, but cost a second
-    // kernel and their bookkeeping, about what 20 steps take: 20 new tokens of one sequence of 8000 keys 65 us as shares, 196 as
-    // tiles, of 2000 keys 36 and 56, of 4 sequences of 1000 keys 37 and 31; 64 of 8 sequences of 4000 keys 76 and 133; two prompts
-    // of 2000 tokens 123 and 94.
+    // kernel and their bookkeeping, about what 20 steps take: 20 new tokens of one sequence of 8000 keys 58 us as shares, 196 as
+    // tiles, of 2000 keys 32 and 54, of 1000 28 and 30, of 4 sequences of 1000 keys 33 and 31, of 2000 39 and 55; 64 of 8 sequences of
+    // 4000 keys 71 and 127; two prompts of 2000 tokens 110 and 95, one of 1500 58 and 45.
     const double x = (double)(r.tile_bound * Hk) / cus, mean = std::max<double>(keys - most / 2, 0);
     const bool line = x < 2 && std::max<double>(keys, x > 1 ? 2 * mean : mean) - x * mean > 20 * kTileKeys;
     if (line) {

@@ -1,6 +1,6 @@
 // Ragged paged attention, rows form: at most 16 rows (new token, query head, map) per (sequence, kv head), the 16 columns of an
 // MFMA tile; bound by the bytes of K and V.  Measured on an MI355X: 2.0 GB of integer K and V (990 000 keys of 128 sequences, 8 kv
-// heads) 344 us, 5.9 TB/s; 0.37 GB of 16-bit ones (32 sequences, 8 kv heads, two maps) 65 us, 5.7 TB/s; a single sequence of
+// heads) 341 us, 6.0 TB/s; 0.37 GB of 16-bit ones (32 sequences, 8 kv heads, two maps) 65 us, 5.7 TB/s; a single sequence of
 // 30 000 keys and 4 kv heads (62 MB) 20 us, of which 5 are the two launches and 3 the second kernel.
 //
 // Split of the work: the keys of every sequence are cut into units of 128 and the units of all sequences are laid end to end; that

@@ -1,8 +1,9 @@
 // Ragged paged attention, tile form: many rows (new token, query head) per (sequence, kv head); bound by the matrix cores.
-// Measured on an MI355X: 4096 new tokens after 12288 of a document, E4M3 pool (0.96 PFLOP), 0.95 to 1.0 ms, 1.0 PFLOP/s,
-// where a large matrix product reaches 1.3; prompts with two maps (33 TFLOP) 64 us, 0.51 PFLOP/s; prompts next to
-// running sequences (50 TFLOP) 125 us, of which the line of tiles takes 99 and its joins 16.  In the long case the vector phase
-// (exponentials, maxima, conversion of bytes) and the matrix phase of two wavefronts fill a SIMD's time to about three quarters.
+// Measured on an MI355X: 4096 new tokens after 12288 of a document, E4M3 pool (0.96 TFLOP), 0.95 to 1.0 ms, 1.0 PFLOP/s,
+// where a large matrix product reaches 1.3; prompts with two maps (33 GFLOP) 65 us, 0.51 PFLOP/s; prompts next to
+// running sequences (50 GFLOP) 111 us, of which the line of tiles takes 88 and its joins 16.  In the long case the matrix cores are busy
+// for 43 % of the time and the vector units (exponentials, maxima, conversion of bytes) for 56 %, in the others for 20 to 23 % and 33
+// to 39 %.
 //
 // A work-group takes 32 rows per wavefront -- rows are (token, head of the kv head's group) in that order, so one pass over K and V
 // serves the whole group -- and goes through the keys 64 at a time.  K and V of a step lie in LDS, both row by row as in the
@@ -551,7 +552,8 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
   const float c_all = p.score_scale_log2 * q_mul * (KV8 && !scaled ? fabsf(p.tensor_scale) : 1.f);
   f32x16 x[2];   // scores of the step that softmax comes to next
   u32x4 pb[4];   // weights of the step before it, as the B operands of V^T P^T
-  // (here the second part is products: prompts with two maps 64 us without, 80 with it.  bf16 takes it, with its 8 bits; fp16 does not)
+  // (here the second part is products: prompts with two maps 64 us without, 80 with it.  bf16 takes it, with its 8 bits; fp16 does not,
+  // and has an error of 0.00030 of the norm for it, where rounding the result alone makes 0.00021)
   constexpr bool kTwo = two_parts<KVF, MAPS>() && std::is_same<OT, BF16>::value;
   u32x4 rest[kTwo ? 4 : 1];  // what their rounding left
   // the steps of which this wavefront sees anything: see_lo .. see_hi - 1 (the same for all its lanes)

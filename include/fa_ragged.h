@@ -22,8 +22,8 @@
  * attends as one at the table's last position would.
  * Pool rows that none of the call's tokens sees -- past the context, before every token's window,
  * unused blocks -- and scales of such blocks may hold anything.  Keys that a token does not see
- * have no weight whatever they are; values of one token that are infinite or NaN can reach earlier new
- * tokens of the same call, whose weight for them is zero, as products of zero.
+ * have no weight whatever they are; values of one new token that are infinite or NaN can reach earlier
+ * new tokens of its sequence in the same call, whose weight for them is zero, as products of zero.
  *
  * Pools are addressed as in fa_paged_attention.h.  Nothing but kernel launches is put on
  * options->stream unless options->elapsed_us is given.  No exception crosses this boundary.

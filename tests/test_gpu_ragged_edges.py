@@ -426,3 +426,30 @@ def test_scalar_scale_below_zero(kv, new, old, scale, softcap):
     out = _attend(batch, query, pools, scale, fp8_scale=-0.5, softcap=softcap)
     refs = R.attention(batch, query, k * -0.5, v * -0.5, scale, softcap=softcap)
     _close(out, refs[0][0], R.attention_bound(refs, dtype, torch.float16))
+
+
+# ---- halves of rows ----
+
+@pytest.mark.parametrize("layout", ["head", "token"])
+def test_append_of_halves_that_are_rotated_for_themselves(layout):
+    """Two calls over the halves of rows and 16-bit pools: pairs a quarter of a row apart."""
+    H, Hk, D, dtype, dev = 4, 2, 128, torch.bfloat16, "cuda"
+    batch = R.Batch([3, 40, 1], [14, 0, 77], B=16)
+    g = torch.Generator().manual_seed(19)
+    fused = torch.randn(batch.T, H + 2 * Hk, D, generator=g).to(dtype)
+    table = R.angle_table(max(batch.lens), D // 2)
+    shape = (batch.blocks, Hk, 16, D) if layout == "head" else (batch.blocks, 16, Hk, D)
+    pools = [torch.randn(shape, generator=g).to(dtype) for _ in range(2)]
+    views = [p.permute(0, 2, 1, 3) if layout == "head" else p for p in pools]
+    d_fused, d_pools, d_table = fused.to(dev), [p.to(dev) for p in pools], table.to(dev)
+    d_views = [p.permute(0, 2, 1, 3) if layout == "head" else p for p in d_pools]
+    q, k, v = d_fused.split([H, Hk, Hk], 1)
+    want = []
+    for half in (slice(0, D // 2), slice(D // 2, D)):
+        torch.ops.fa_amd.kv_cache_append(k[..., half], v[..., half], *(p[..., half] for p in d_views), *batch.on(dev), d_table,
+                                         q[..., half], q[..., half])
+        want.append(R.append(batch, fused[:, H:H + Hk, half], fused[:, H + Hk:, half], *(p[..., half] for p in views), table, False,
+                             query=fused[:, :H, half]))
+    for got, ref in zip(d_pools, pools):
+        assert torch.equal(got.cpu(), ref)
+    assert torch.equal(d_fused[:, :H].cpu(), torch.cat(want, -1))
