@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)
     float sink = -INFINITY;
     if constexpr (MAPS == 1) {
       if (p.sinks != nullptr && from == 0) {
-        const int row = min(row0 + strip * 32 + (kAnew ? anew(col) : col), all_rows - 1);
+        const int row = min(row0 + strip * 32 + anew(col), all_rows - 1);
         sink = sink_log2(p, kvh * G + row % G);
         mt = fmaxf(mt, sink);
       }
