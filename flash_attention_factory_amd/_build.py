@@ -7,6 +7,7 @@ import subprocess
 _PKG = os.path.dirname(os.path.abspath(__file__))
 SOURCE = os.path.join(_PKG, "csrc", "fa_paged_attention.hip")
 RAGGED_SOURCE = os.path.join(_PKG, "csrc", "fa_ragged.hip")
+LATENT_SOURCE = os.path.join(_PKG, "csrc", "fa_latent.hip")
 LIBRARY = os.path.join(_PKG, "libfa_paged_attention.so")
 
 TORCH_OPS_SOURCE = os.path.join(_PKG, "csrc", "torch_ops.cpp")
@@ -25,7 +26,7 @@ def build(verbose: bool = False, extra_flags=(), output: str = LIBRARY) -> str:
     (-DFA_TIMELINE: in-kernel timeline; -DFA_COST_PROBE=1|2: the segment kernels without their stores
     of partials), which FA_PAGED_ATTENTION_LIBRARY selects at run time."""
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, SOURCE, RAGGED_SOURCE, "-o", output]
+    cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, SOURCE, RAGGED_SOURCE, LATENT_SOURCE, "-o", output]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)

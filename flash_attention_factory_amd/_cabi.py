@@ -1,5 +1,5 @@
 """ctypes binding of libfa_paged_attention.so (declarations: include/fa_paged_attention.h,
-include/fa_kv_cache.h, include/fa_ragged.h).
+include/fa_kv_cache.h, include/fa_ragged.h, include/fa_latent.h).
 
 There is no fallback: if the HIP library is missing or a call fails, this raises.
 """
@@ -50,6 +50,16 @@ RAGGED_EXPORTS = (
     "fa_paged_attention_ragged",
     "fa_paged_attention_ragged_workspace_bytes",
     "fa_paged_attention_differential",
+)
+
+# of include/fa_latent.h
+LATENT_EXPORTS = (
+    "fa_latent_cache_append",
+    "fa_latent_cache_gather",
+    "fa_paged_attention_latent",
+    "fa_paged_attention_latent_workspace_bytes",
+    "fa_attention_latent_expanded",
+    "fa_attention_latent_expanded_workspace_bytes",
 )
 
 ABI_REVISION = 8
@@ -185,6 +195,54 @@ class RaggedShape(_Versioned):
     ]
 
 
+def _int32(*names):
+    return [(name, ctypes.c_int32) for name in names]
+
+
+def _int64(*names):
+    return [(name, ctypes.c_int64) for name in names]
+
+
+class LatentAppendShape(_Versioned):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        *_int32("num_seqs", "num_tokens", "num_heads", "latent_dim", "rope_dim", "block_size", "max_blocks_per_seq"),
+        *_int64("block_stride", "token_stride", "latent_token_stride", "rope_key_token_stride", "query_token_stride", "query_head_stride",
+                "query_out_token_stride", "query_out_head_stride"),
+        *_int32("src_dtype", "cache_dtype", "num_pool_blocks", "max_positions", "interleaved"),
+        ("norm_eps", ctypes.c_float),
+    ]
+
+
+class LatentGatherShape(_Versioned):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        *_int32("num_seqs", "num_rows", "latent_dim", "rope_dim", "block_size", "max_blocks_per_seq", "num_pool_blocks"),
+        *_int64("block_stride", "token_stride", "out_stride"),
+        *_int32("out_dtype", "cache_dtype"),
+    ]
+
+
+class LatentAttentionShape(_Versioned):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        *_int32("num_seqs", "num_tokens", "num_heads", "latent_dim", "rope_dim", "block_size", "max_blocks_per_seq"),
+        *_int64("block_stride", "token_stride", "query_latent_token_stride", "query_latent_head_stride", "query_rope_token_stride",
+                "query_rope_head_stride", "out_token_stride", "out_head_stride"),
+        *_int32("q_dtype", "cache_dtype", "num_pool_blocks", "max_query_len", "max_context_len"),
+    ]
+
+
+class LatentExpandedShape(_Versioned):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        *_int32("num_seqs", "num_tokens", "num_keys", "num_heads", "head_size", "rope_dim", "dtype"),
+        *_int64("query_token_stride", "query_head_stride", "key_token_stride", "key_head_stride", "rope_key_token_stride",
+                "value_token_stride", "value_head_stride", "out_token_stride", "out_head_stride"),
+        *_int32("max_query_len", "max_key_len"),
+    ]
+
+
 class SplitPlan(_Versioned):
     _fields_ = [
         ("struct_size", ctypes.c_uint32),
@@ -277,7 +335,7 @@ def load() -> ctypes.CDLL:
             f"{LIBRARY} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
             "(there is no CPU or PyTorch fallback for the paged-attention kernels)")
     L = ctypes.CDLL(LIBRARY)
-    missing = [name for name in EXPORTS + RAGGED_EXPORTS if not hasattr(L, name)]
+    missing = [name for name in EXPORTS + RAGGED_EXPORTS + LATENT_EXPORTS if not hasattr(L, name)]
     if missing:
         raise RuntimeError(f"{LIBRARY} lacks {', '.join(missing)}: it was built from older sources, rebuild the library")
     P = ctypes.c_void_p
@@ -305,6 +363,15 @@ def load() -> ctypes.CDLL:
     L.fa_paged_attention_differential.argtypes = [P] * 7 + [ctypes.c_float, P, P, ctypes.c_float, ctypes.c_float, P,
                                                            ctypes.c_int64, R, O]
     L.fa_paged_attention_differential.restype = ctypes.c_int32
+    F, N = ctypes.c_float, ctypes.c_int64
+    for name, arguments, result in (
+            ("fa_latent_cache_append", [P] * 11 + [ctypes.POINTER(LatentAppendShape), O], ctypes.c_int32),
+            ("fa_latent_cache_gather", [P] * 6 + [ctypes.POINTER(LatentGatherShape), O], ctypes.c_int32),
+            ("fa_paged_attention_latent", [P] * 8 + [F, P, N, ctypes.POINTER(LatentAttentionShape), O], ctypes.c_int32),
+            ("fa_paged_attention_latent_workspace_bytes", [ctypes.POINTER(LatentAttentionShape)], N),
+            ("fa_attention_latent_expanded", [P] * 7 + [F, P, N, ctypes.POINTER(LatentExpandedShape), O], ctypes.c_int32),
+            ("fa_attention_latent_expanded_workspace_bytes", [ctypes.POINTER(LatentExpandedShape)], N)):
+        getattr(L, name).argtypes, getattr(L, name).restype = arguments, result
     L.fa_last_error.restype = ctypes.c_char_p
     L.fa_paged_attention_abi_version.restype = ctypes.c_int32
     L.fa_paged_attention_reduce_plan.argtypes = [ctypes.POINTER(Shape), ctypes.POINTER(Options), ctypes.c_int32,

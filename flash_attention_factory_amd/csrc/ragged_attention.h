@@ -77,13 +77,14 @@ __device__ __forceinline__ uint32_t rest_of_pair(uint32_t rounded, float lo, flo
 }
 
 // The tokens that the call has bounds for: the first max_query_len ones, and the keys that those see.
-__device__ __forceinline__ RaggedSeq ragged_seq_cut(const RaggedParams &p, RaggedSeq q) {
+template <typename Params>
+__device__ __forceinline__ RaggedSeq ragged_seq_cut(const Params &p, RaggedSeq q) {
   q.n = min(q.n, p.max_query_len);
   q.ctx = max(0, min(q.ctx, q.pos0 + q.n));
   return q;
 }
-template <int MAPS>
-__device__ __forceinline__ bool in_rows_form(const RaggedParams &p, const RaggedSeq &q) {
+template <int MAPS, typename Params>
+__device__ __forceinline__ bool in_rows_form(const Params &p, const RaggedSeq &q) {
   return q.n * p.group * MAPS <= p.row_limit;
 }
 // Position that the j-th new token attends from: its own, or the last one that the block table has.
@@ -99,8 +100,8 @@ __device__ __forceinline__ int row_units(const RaggedParams &p, RaggedSeq q) {
   return (q.ctx + kRowUnit - 1) / kRowUnit - first_key(p, q) / kRowUnit;
 }
 // Tiles of `rows` rows that the tile form has to go through for one kv head of a sequence.
-template <int MAPS, int ROWS>
-__device__ __forceinline__ int row_tiles(const RaggedParams &p, RaggedSeq q) {
+template <int MAPS, int ROWS, typename Params>
+__device__ __forceinline__ int row_tiles(const Params &p, RaggedSeq q) {
   q = ragged_seq_cut(p, q);
   if (q.n <= 0 || in_rows_form<MAPS>(p, q)) return 0;
   return (q.n * p.group + ROWS - 1) / ROWS;

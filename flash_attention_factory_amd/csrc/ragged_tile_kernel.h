@@ -116,8 +116,8 @@ struct TileCosts {
   __device__ __forceinline__ int64_t upto(int64_t t) const { return first * t + more * (t * (t - 1) / 2); }
   __device__ __forceinline__ int64_t of_head() const { return upto(tiles); }
 };
-template <int MAPS, int ROWS>
-__device__ __forceinline__ TileCosts tile_costs(const RaggedParams &p, RaggedSeq q) {
+template <int MAPS, int ROWS, typename Params>
+__device__ __forceinline__ TileCosts tile_costs(const Params &p, RaggedSeq q) {
   TileCosts c;
   c.tiles = row_tiles<MAPS, ROWS>(p, q);
   q = ragged_seq_cut(p, q);
@@ -155,12 +155,12 @@ __device__ __forceinline__ int64_t divide(int64_t n, int d) {
   if ((q + 1) * d <= n) ++q;
   return q;
 }
-template <int MAPS, int ROWS>
+template <int MAPS, int ROWS, typename Params = RaggedParams>
 struct TileLine {
   int64_t total;
   int groups;
   int64_t mine, upto;  // of the first 64 sequences: this lane's, and the sum up to it
-  __device__ __forceinline__ TileLine(const RaggedParams &p, int lane) {
+  __device__ __forceinline__ TileLine(const Params &p, int lane) {
     mine = costs(p, lane);
     upto = wave_inclusive_scan64(mine, lane);
     total = readlane64(upto, 63);
@@ -171,12 +171,12 @@ struct TileLine {
     }
     groups = (int)min((int64_t)p.tile_groups, total / kLeastShare + (total > 0));
   }
-  static __device__ __forceinline__ int64_t costs(const RaggedParams &p, int s) {  // of all kv heads of sequence s
+  static __device__ __forceinline__ int64_t costs(const Params &p, int s) {  // of all kv heads of sequence s
     return s < p.b.num_seqs ? tile_costs<MAPS, ROWS>(p, ragged_seq_of_lane(p.b, s)).of_head() * p.num_kv_heads : 0;
   }
   __device__ __forceinline__ int64_t cut(int g) const { return divide(total * g, groups); }
   // `at` < total
-  __device__ __forceinline__ TilePlace find(const RaggedParams &p, int64_t at, int lane) const {
+  __device__ __forceinline__ TilePlace find(const Params &p, int64_t at, int lane) const {
     TilePlace r;
     int64_t before = 0, of_lane = mine, sum = upto;
     for (int base = 0;; base += 64) {
@@ -217,8 +217,8 @@ struct TileLine {
 struct TileSteps {
   int first, count;
 };
-template <int ROWS>
-__device__ __forceinline__ TileSteps tile_steps(const RaggedParams &p, const RaggedSeq &q, int tile) {
+template <int ROWS, typename Params>
+__device__ __forceinline__ TileSteps tile_steps(const Params &p, const RaggedSeq &q, int tile) {
   const int row0 = tile * ROWS;
   const int pos_lo = attends_from(q, row0 / p.group), pos_hi = attends_from(q, (min(row0 + ROWS, q.n * p.group) - 1) / p.group);
   TileSteps s;

@@ -19,6 +19,7 @@
 #include <limits>
 
 #include "../../include/fa_kv_cache.h"
+#include "../../include/fa_latent.h"
 #include "../../include/fa_paged_attention.h"
 #include "../../include/fa_ragged.h"
 
@@ -37,6 +38,12 @@ struct Entries {
   decltype(&fa_paged_attention_ragged) ragged;
   decltype(&fa_paged_attention_differential) differential;
   decltype(&fa_paged_attention_ragged_workspace_bytes) ragged_workspace_bytes;
+  decltype(&fa_latent_cache_append) latent_append;
+  decltype(&fa_latent_cache_gather) latent_gather;
+  decltype(&fa_paged_attention_latent) latent;
+  decltype(&fa_paged_attention_latent_workspace_bytes) latent_workspace_bytes;
+  decltype(&fa_attention_latent_expanded) latent_expanded;
+  decltype(&fa_attention_latent_expanded_workspace_bytes) latent_expanded_workspace_bytes;
 };
 Entries entries = {};
 
@@ -413,6 +420,207 @@ bool ragged_attend(const Tensor &out, const Tensor &query, const Tensor &key_cac
                         ints(block_tables), ints(query_start), ints(context_lens), (float)scale, at_space, need, &sh, &op) == FA_OK;
 }
 
+// ---- latent attention ---------------------------------------------------------------------------
+
+constexpr int64_t kRope = 64;  // elements of a latent pool's rotated part
+
+// The fa_kv_cache_dtype of a latent pool for rows of `type`; -1: not a pool the kernels take.
+int32_t latent_pool(const Tensor &cache, const OptTensor &scales, at::ScalarType type) {
+  if (cache.dim() != 3 || cache.stride(2) != 1 || cache.size(2) <= kRope) return -1;
+  for (int64_t d = 0; d < 3; ++d)
+    if (!fits_int32(cache.size(d))) return -1;
+  if (cache.scalar_type() == type) return scales.has_value() ? -1 : FA_KV_CACHE_16BIT;
+  if (cache.scalar_type() != at::kFloat8_e4m3fn || !scales.has_value() || !is_floats(*scales) || scales->dim() != 2 ||
+      scales->size(0) != cache.size(0) || scales->size(1) != cache.size(1))
+    return -1;
+  return FA_KV_CACHE_E4M3;
+}
+bool rows_of(const Tensor &t, at::ScalarType type, std::initializer_list<int64_t> sizes) {
+  return t.scalar_type() == type && t.sizes() == at::IntArrayRef(sizes.begin(), sizes.size()) && (t.size(-1) <= 1 || t.stride(-1) == 1);
+}
+bool all_on(const Tensor &anchor, std::initializer_list<const Tensor *> tensors, std::initializer_list<const OptTensor *> more) {
+  for (const Tensor *t : tensors)
+    if (!same_device(anchor, *t)) return false;
+  for (const OptTensor *t : more)
+    if (!same_device(anchor, *t)) return false;
+  return true;
+}
+int32_t dtype_of(at::ScalarType type) { return type == at::kBFloat16 ? FA_DTYPE_BF16 : FA_DTYPE_F16; }
+// Workspace from PyTorch's stream-ordered allocator.
+struct Space {
+  Tensor space;
+  int64_t bytes;
+  Space(int64_t need, const Tensor &like) : bytes(need) {
+    if (need > 0) space = at::empty({need}, like.options().dtype(at::kByte));
+  }
+  void *data() const { return bytes > 0 ? space.data_ptr() : nullptr; }
+};
+
+bool append_latent(const Tensor &latent, const Tensor &rope_key, const Tensor &cache, const Tensor &block_tables, const Tensor &query_start,
+                   const Tensor &context_lens, const OptTensor &norm_weight, const OptTensor &cos_sin, const OptTensor &query_rope,
+                   const OptTensor &query_rope_out, const OptTensor &scales, double norm_eps, bool interleaved) {
+  if (!entries.loop || !latent.is_cuda()) return false;
+  if (!all_on(latent, {&rope_key, &cache, &block_tables, &query_start, &context_lens}, {&norm_weight, &cos_sin, &query_rope, &query_rope_out, &scales}))
+    return false;
+  const auto type = latent.scalar_type();
+  if (!is_16bit(type) || latent.dim() != 2 || query_rope.has_value() != query_rope_out.has_value()) return false;
+  const int32_t kind = latent_pool(cache, scales, type);
+  const int64_t S = batch_of(block_tables, query_start, context_lens), T = latent.size(0);
+  if (kind < 0 || S < 0 || !fits_int32(T)) return false;
+  const int64_t width = cache.size(2) - kRope;
+  if (!rows_of(latent, type, {T, width}) || !rows_of(rope_key, type, {T, kRope})) return false;
+  fa_latent_append_shape sh = FA_LATENT_APPEND_SHAPE_INIT;
+  if (query_rope.has_value()) {
+    if (query_rope->dim() != 3 || !fits_int32(query_rope->size(1))) return false;
+    const int64_t H = query_rope->size(1);
+    if (!rows_of(*query_rope, type, {T, H, kRope}) || !rows_of(*query_rope_out, type, {T, H, kRope})) return false;
+    sh.num_heads = (int32_t)H;
+    sh.query_token_stride = query_rope->stride(0);
+    sh.query_head_stride = query_rope->stride(1);
+    sh.query_out_token_stride = query_rope_out->stride(0);
+    sh.query_out_head_stride = query_rope_out->stride(1);
+  }
+  if (norm_weight.has_value() && (!is_floats(*norm_weight) || norm_weight->dim() != 1 || norm_weight->size(0) != width)) return false;
+  if (cos_sin.has_value()) {
+    if (!is_floats(*cos_sin) || cos_sin->dim() != 2 || cos_sin->size(1) != kRope || cos_sin->size(0) == 0 || !fits_int32(cos_sin->size(0))) return false;
+    sh.max_positions = (int32_t)cos_sin->size(0);
+  }
+  sh.num_seqs = (int32_t)S;
+  sh.num_tokens = (int32_t)T;
+  sh.latent_dim = (int32_t)width;
+  sh.rope_dim = (int32_t)kRope;
+  sh.block_size = (int32_t)cache.size(1);
+  sh.max_blocks_per_seq = (int32_t)block_tables.size(1);
+  sh.block_stride = cache.stride(0);
+  sh.token_stride = cache.stride(1);
+  sh.latent_token_stride = latent.stride(0);
+  sh.rope_key_token_stride = rope_key.stride(0);
+  sh.src_dtype = dtype_of(type);
+  sh.cache_dtype = kind;
+  sh.num_pool_blocks = (int32_t)cache.size(0);
+  sh.interleaved = interleaved;
+  sh.norm_eps = (float)norm_eps;
+  fa_paged_attention_options op = FA_PAGED_ATTENTION_OPTIONS_INIT;
+  const c10::DeviceGuard guard(latent.device());
+  op.stream = c10::hip::getCurrentHIPStream(latent.device().index()).stream();
+  return entries.latent_append(latent.const_data_ptr(), rope_key.const_data_ptr(), cache.data_ptr(), floats(norm_weight), floats(cos_sin),
+                               query_rope.has_value() ? query_rope->const_data_ptr() : nullptr,
+                               query_rope_out.has_value() ? query_rope_out->data_ptr() : nullptr, const_cast<float *>(floats(scales)),
+                               ints(block_tables), ints(query_start), ints(context_lens), &sh, &op) == FA_OK;
+}
+
+bool gather_latent(const Tensor &out, const Tensor &cache, const Tensor &block_tables, const Tensor &row_start, const OptTensor &first_keys,
+                   const OptTensor &scales) {
+  if (!entries.loop || !out.is_cuda() || !all_on(out, {&cache, &block_tables, &row_start}, {&first_keys, &scales})) return false;
+  const auto type = out.scalar_type();
+  const int32_t kind = is_16bit(type) ? latent_pool(cache, scales, type) : -1;
+  if (kind < 0 || out.dim() != 2 || !fits_int32(out.size(0)) || !rows_of(out, type, {out.size(0), cache.size(2)})) return false;
+  auto is_ints = [](const Tensor &t, int64_t dims) { return t.scalar_type() == at::kInt && t.is_contiguous() && t.dim() == dims; };
+  if (!is_ints(block_tables, 2) || !is_ints(row_start, 1)) return false;
+  const int64_t S = block_tables.size(0);
+  if (row_start.size(0) != S + 1 || !fits_int32(S) || !fits_int32(block_tables.size(1))) return false;
+  if (first_keys.has_value() && (!is_ints(*first_keys, 1) || first_keys->size(0) != S)) return false;
+  fa_latent_gather_shape sh = FA_LATENT_GATHER_SHAPE_INIT;
+  sh.num_seqs = (int32_t)S;
+  sh.num_rows = (int32_t)out.size(0);
+  sh.latent_dim = (int32_t)(cache.size(2) - kRope);
+  sh.rope_dim = (int32_t)kRope;
+  sh.block_size = (int32_t)cache.size(1);
+  sh.max_blocks_per_seq = (int32_t)block_tables.size(1);
+  sh.num_pool_blocks = (int32_t)cache.size(0);
+  sh.block_stride = cache.stride(0);
+  sh.token_stride = cache.stride(1);
+  sh.out_stride = out.stride(0);
+  sh.out_dtype = dtype_of(type);
+  sh.cache_dtype = kind;
+  fa_paged_attention_options op = FA_PAGED_ATTENTION_OPTIONS_INIT;
+  const c10::DeviceGuard guard(out.device());
+  op.stream = c10::hip::getCurrentHIPStream(out.device().index()).stream();
+  return entries.latent_gather(out.data_ptr(), cache.const_data_ptr(), floats(scales), ints(block_tables), ints(row_start),
+                               first_keys.has_value() ? ints(*first_keys) : nullptr, &sh, &op) == FA_OK;
+}
+
+bool attend_latent(const Tensor &out, const Tensor &query_latent, const Tensor &query_rope, const Tensor &cache, const Tensor &block_tables,
+                   const Tensor &query_start, const Tensor &context_lens, double scale, int64_t most, int64_t longest, const OptTensor &scales) {
+  if (!entries.loop || !query_latent.is_cuda()) return false;
+  if (!all_on(query_latent, {&out, &query_rope, &cache, &block_tables, &query_start, &context_lens}, {&scales})) return false;
+  const auto type = query_latent.scalar_type();
+  const int32_t kind = is_16bit(type) ? latent_pool(cache, scales, type) : -1;
+  const int64_t S = batch_of(block_tables, query_start, context_lens);
+  if (kind < 0 || S < 0 || query_latent.dim() != 3 || !fits_int32(most) || !fits_int32(longest)) return false;
+  const int64_t T = query_latent.size(0), H = query_latent.size(1), width = cache.size(2) - kRope;
+  if (!fits_int32(T) || !fits_int32(H) || !rows_of(query_latent, type, {T, H, width}) || !rows_of(out, type, {T, H, width}) ||
+      !rows_of(query_rope, type, {T, H, kRope}))
+    return false;
+  fa_latent_attention_shape sh = FA_LATENT_ATTENTION_SHAPE_INIT;
+  sh.num_seqs = (int32_t)S;
+  sh.num_tokens = (int32_t)T;
+  sh.num_heads = (int32_t)H;
+  sh.latent_dim = (int32_t)width;
+  sh.rope_dim = (int32_t)kRope;
+  sh.block_size = (int32_t)cache.size(1);
+  sh.max_blocks_per_seq = (int32_t)block_tables.size(1);
+  sh.block_stride = cache.stride(0);
+  sh.token_stride = cache.stride(1);
+  sh.query_latent_token_stride = query_latent.stride(0);
+  sh.query_latent_head_stride = query_latent.stride(1);
+  sh.query_rope_token_stride = query_rope.stride(0);
+  sh.query_rope_head_stride = query_rope.stride(1);
+  sh.out_token_stride = out.stride(0);
+  sh.out_head_stride = out.stride(1);
+  sh.q_dtype = dtype_of(type);
+  sh.cache_dtype = kind;
+  sh.num_pool_blocks = (int32_t)cache.size(0);
+  sh.max_query_len = (int32_t)most;
+  sh.max_context_len = (int32_t)longest;
+  fa_paged_attention_options op = FA_PAGED_ATTENTION_OPTIONS_INIT;
+  const c10::DeviceGuard guard(query_latent.device());
+  op.stream = c10::hip::getCurrentHIPStream(query_latent.device().index()).stream();
+  const Space space(entries.latent_workspace_bytes(&sh), query_latent);
+  return entries.latent(out.data_ptr(), query_latent.const_data_ptr(), query_rope.const_data_ptr(), cache.const_data_ptr(), floats(scales),
+                        ints(block_tables), ints(query_start), ints(context_lens), (float)scale, space.data(), space.bytes, &sh, &op) == FA_OK;
+}
+
+bool attend_expanded(const Tensor &out, const Tensor &query, const Tensor &key, const Tensor &rope_key, const Tensor &value,
+                     const Tensor &query_start, const Tensor &key_start, double scale, int64_t most, int64_t longest) {
+  if (!entries.loop || !query.is_cuda() || !all_on(query, {&out, &key, &rope_key, &value, &query_start, &key_start}, {})) return false;
+  const auto type = query.scalar_type();
+  if (!is_16bit(type) || query.dim() != 3 || key.dim() != 3 || !fits_int32(most) || !fits_int32(longest)) return false;
+  const int64_t T = query.size(0), H = query.size(1), N = key.size(0), D = key.size(2);
+  if (!fits_int32(T) || !fits_int32(H) || !fits_int32(N) || !fits_int32(D)) return false;
+  if (!rows_of(query, type, {T, H, D + kRope}) || !rows_of(out, type, {T, H, D}) || !rows_of(key, type, {N, H, D}) ||
+      !rows_of(value, type, {N, H, D}) || !rows_of(rope_key, type, {N, kRope}))
+    return false;
+  for (const Tensor *t : {&query_start, &key_start})
+    if (t->scalar_type() != at::kInt || !t->is_contiguous() || t->dim() != 1 || t->size(0) < 1 || !fits_int32(t->size(0))) return false;
+  if (query_start.size(0) != key_start.size(0)) return false;
+  fa_latent_expanded_shape sh = FA_LATENT_EXPANDED_SHAPE_INIT;
+  sh.num_seqs = (int32_t)(query_start.size(0) - 1);
+  sh.num_tokens = (int32_t)T;
+  sh.num_keys = (int32_t)N;
+  sh.num_heads = (int32_t)H;
+  sh.head_size = (int32_t)D;
+  sh.rope_dim = (int32_t)kRope;
+  sh.dtype = dtype_of(type);
+  sh.query_token_stride = query.stride(0);
+  sh.query_head_stride = query.stride(1);
+  sh.key_token_stride = key.stride(0);
+  sh.key_head_stride = key.stride(1);
+  sh.rope_key_token_stride = rope_key.stride(0);
+  sh.value_token_stride = value.stride(0);
+  sh.value_head_stride = value.stride(1);
+  sh.out_token_stride = out.stride(0);
+  sh.out_head_stride = out.stride(1);
+  sh.max_query_len = (int32_t)most;
+  sh.max_key_len = (int32_t)longest;
+  fa_paged_attention_options op = FA_PAGED_ATTENTION_OPTIONS_INIT;
+  const c10::DeviceGuard guard(query.device());
+  op.stream = c10::hip::getCurrentHIPStream(query.device().index()).stream();
+  const Space space(entries.latent_expanded_workspace_bytes(&sh), query);
+  return entries.latent_expanded(out.data_ptr(), query.const_data_ptr(), key.const_data_ptr(), rope_key.const_data_ptr(), value.const_data_ptr(),
+                                 ints(query_start), ints(key_start), (float)scale, space.data(), space.bytes, &sh, &op) == FA_OK;
+}
+
 // ---- dispatcher kernels -------------------------------------------------------------------------
 // Boxed, one for all operators: which arguments there are and which of them are written is the schema's to say.
 
@@ -546,9 +754,54 @@ void differential(const c10::OperatorHandle &op, torch::jit::Stack *stack) {
   torch::jit::drop(*stack, n);
 }
 
+void latent_append(const c10::OperatorHandle &op, torch::jit::Stack *stack) {
+  const size_t n = op.schema().arguments().size();
+  Args a{stack, n};
+  const Tensor &latent = a.tensor(), &rope_key = a.tensor(), &cache = a.tensor(), &tables = a.tensor(), &start = a.tensor(), &lens = a.tensor();
+  const OptTensor weight = a.maybe(), cos_sin = a.maybe(), query = a.maybe(), query_out = a.maybe(), scales = a.maybe();
+  const double eps = a.real();
+  const bool interleaved = a.next().toBool();
+  if (!append_latent(latent, rope_key, cache, tables, start, lens, weight, cos_sin, query, query_out, scales, eps, interleaved))
+    return in_python(op).callBoxed(stack);
+  torch::jit::drop(*stack, n);
+}
+
+void latent_gather(const c10::OperatorHandle &op, torch::jit::Stack *stack) {
+  const size_t n = op.schema().arguments().size();
+  Args a{stack, n};
+  const Tensor &out = a.tensor(), &cache = a.tensor(), &tables = a.tensor(), &start = a.tensor();
+  const OptTensor first = a.maybe(), scales = a.maybe();
+  if (!gather_latent(out, cache, tables, start, first, scales)) return in_python(op).callBoxed(stack);
+  torch::jit::drop(*stack, n);
+}
+
+void latent(const c10::OperatorHandle &op, torch::jit::Stack *stack) {
+  const size_t n = op.schema().arguments().size();
+  Args a{stack, n};
+  const Tensor &out = a.tensor(), &query = a.tensor(), &rope = a.tensor(), &cache = a.tensor(), &tables = a.tensor(), &start = a.tensor(),
+               &lens = a.tensor();
+  const double scale = a.real();
+  const int64_t most = a.integer(), longest = a.integer();
+  const OptTensor scales = a.maybe();
+  if (!attend_latent(out, query, rope, cache, tables, start, lens, scale, most, longest, scales)) return in_python(op).callBoxed(stack);
+  torch::jit::drop(*stack, n);
+}
+
+void latent_expanded(const c10::OperatorHandle &op, torch::jit::Stack *stack) {
+  const size_t n = op.schema().arguments().size();
+  Args a{stack, n};
+  const Tensor &out = a.tensor(), &query = a.tensor(), &key = a.tensor(), &rope_key = a.tensor(), &value = a.tensor(), &start = a.tensor(),
+               &key_start = a.tensor();
+  const double scale = a.real();
+  const int64_t most = a.integer(), longest = a.integer();
+  if (!attend_expanded(out, query, key, rope_key, value, start, key_start, scale, most, longest)) return in_python(op).callBoxed(stack);
+  torch::jit::drop(*stack, n);
+}
+
 constexpr const char *kNames[] = {"paged_attention_loop", "paged_attention_fp8_loop", "paged_attention_reduce",
                                   "paged_attention_fp8_reduce", "kv_cache_write", "kv_cache_append", "paged_attention_ragged",
-                                  "paged_attention_differential"};
+                                  "paged_attention_differential", "latent_cache_append", "latent_cache_gather",
+                                  "paged_attention_latent", "attention_latent_expanded"};
 
 }  // namespace
 
@@ -590,6 +843,15 @@ TORCH_LIBRARY_FRAGMENT(fa_amd, m) {
         "Tensor block_tables, Tensor query_start, Tensor context_lens, float scale, Tensor lambdas, Tensor? norm_weight, "
         "SymInt max_query_len, SymInt max_context_len=0, float norm_eps=1.0000000000000001e-05, float out_scale=1., "
         "Tensor? k_scales=None, Tensor? v_scales=None, SymInt window_left=-1) -> ()", tags);
+  m.def("latent_cache_append(Tensor latent, Tensor rope_key, Tensor(a2!) cache, Tensor block_tables, Tensor query_start, "
+        "Tensor context_lens, Tensor? norm_weight=None, Tensor? cos_sin=None, Tensor? query_rope=None, "
+        "Tensor(a9!)? query_rope_out=None, Tensor(a10!)? scales=None, float norm_eps=9.9999999999999995e-07, bool interleaved=False) -> ()", tags);
+  m.def("latent_cache_gather(Tensor(a0!) out, Tensor cache, Tensor block_tables, Tensor row_start, Tensor? first_keys=None, "
+        "Tensor? scales=None) -> ()", tags);
+  m.def("paged_attention_latent(Tensor(a0!) out, Tensor query_latent, Tensor query_rope, Tensor cache, Tensor block_tables, "
+        "Tensor query_start, Tensor context_lens, float scale, SymInt max_query_len, SymInt max_context_len=0, Tensor? scales=None) -> ()", tags);
+  m.def("attention_latent_expanded(Tensor(a0!) out, Tensor query, Tensor key, Tensor rope_key, Tensor value, Tensor query_start, "
+        "Tensor key_start, float scale, SymInt max_query_len, SymInt max_key_len=0) -> ()", tags);
 }
 
 TORCH_LIBRARY_IMPL(fa_amd, CUDA, m) {
@@ -601,6 +863,10 @@ TORCH_LIBRARY_IMPL(fa_amd, CUDA, m) {
   m.impl("kv_cache_append", torch::CppFunction::makeFromBoxedFunction<&cache_append>());
   m.impl("paged_attention_ragged", torch::CppFunction::makeFromBoxedFunction<&ragged>());
   m.impl("paged_attention_differential", torch::CppFunction::makeFromBoxedFunction<&differential>());
+  m.impl("latent_cache_append", torch::CppFunction::makeFromBoxedFunction<&latent_append>());
+  m.impl("latent_cache_gather", torch::CppFunction::makeFromBoxedFunction<&latent_gather>());
+  m.impl("paged_attention_latent", torch::CppFunction::makeFromBoxedFunction<&latent>());
+  m.impl("attention_latent_expanded", torch::CppFunction::makeFromBoxedFunction<&latent_expanded>());
 }
 
 TORCH_LIBRARY_IMPL(fa_amd, Autograd, m) {

@@ -28,6 +28,17 @@ and, for ragged batches (any number of new tokens per sequence: ``query_start``,
                                                   query_start, context_lens, scale, lambdas,
                                                   norm_weight, max_query_len)
 
+and, for models whose keys and values come from one latent vector per token,
+
+    torch.ops.fa_amd.latent_cache_append(latent, rope_key, cache, block_tables, query_start,
+                                         context_lens, norm_weight, cos_sin, query_rope,
+                                         query_rope_out, scales)
+    torch.ops.fa_amd.latent_cache_gather(out, cache, block_tables, row_start, first_keys, scales)
+    torch.ops.fa_amd.paged_attention_latent(out, query_latent, query_rope, cache, block_tables,
+                                            query_start, context_lens, scale, max_query_len)
+    torch.ops.fa_amd.attention_latent_expanded(out, query, key, rope_key, value, query_start,
+                                               key_start, scale, max_query_len)
+
 Further optional arguments, all off by default: ``alibi_slopes`` (fp32 ``[heads]``), ``softcap``
 (> 0) and ``window_left`` (>= 0) apply the score modifiers -- here a modifier that is passed is
 applied, unlike ``lib.*.run``, which mirrors upstream in taking and ignoring slopes and cap; the
@@ -61,9 +72,11 @@ import torch
 from torch import Tensor
 
 from . import _build, _cabi
-from .lib import (kv_cache_append as _kv_cache_append, kv_cache_write as _kv_cache_write,
-                  paged_attention_differential as _differential, paged_attention_fp8_loop as _fp8_loop,
-                  paged_attention_fp8_reduce as _fp8_reduce, paged_attention_loop as _loop,
+from .lib import (attention_latent_expanded as _latent_expanded, kv_cache_append as _kv_cache_append,
+                  kv_cache_write as _kv_cache_write, latent_cache_append as _latent_append,
+                  latent_cache_gather as _latent_gather, paged_attention_differential as _differential,
+                  paged_attention_fp8_loop as _fp8_loop, paged_attention_fp8_reduce as _fp8_reduce,
+                  paged_attention_latent as _latent, paged_attention_loop as _loop,
                   paged_attention_ragged as _ragged, paged_attention_reduce as _reduce)
 
 _NS = "fa_amd_py"
@@ -196,8 +209,38 @@ def paged_attention_differential(out: Tensor, query: Tensor, key_cache: Tensor, 
                       timed=False)
 
 
+@torch.library.custom_op(f"{_NS}::latent_cache_append", mutates_args=("cache", "query_rope_out", "scales"), device_types="cuda")
+def latent_cache_append(latent: Tensor, rope_key: Tensor, cache: Tensor, block_tables: Tensor, query_start: Tensor,
+                        context_lens: Tensor, norm_weight: Optional[Tensor] = None, cos_sin: Optional[Tensor] = None,
+                        query_rope: Optional[Tensor] = None, query_rope_out: Optional[Tensor] = None,
+                        scales: Optional[Tensor] = None, norm_eps: float = 1e-6, interleaved: bool = False) -> None:
+    _latent_append.run(latent, rope_key, cache, block_tables, query_start, context_lens, norm_weight, cos_sin, query_rope,
+                       query_rope_out, scales, norm_eps, interleaved, timed=False)
+
+
+@torch.library.custom_op(f"{_NS}::latent_cache_gather", mutates_args=("out",), device_types="cuda")
+def latent_cache_gather(out: Tensor, cache: Tensor, block_tables: Tensor, row_start: Tensor, first_keys: Optional[Tensor] = None,
+                        scales: Optional[Tensor] = None) -> None:
+    _latent_gather.run(out, cache, block_tables, row_start, first_keys, scales, timed=False)
+
+
+@torch.library.custom_op(f"{_NS}::paged_attention_latent", mutates_args=("out",), device_types="cuda")
+def paged_attention_latent(out: Tensor, query_latent: Tensor, query_rope: Tensor, cache: Tensor, block_tables: Tensor,
+                           query_start: Tensor, context_lens: Tensor, scale: float, max_query_len: int, max_context_len: int = 0,
+                           scales: Optional[Tensor] = None) -> None:
+    _latent.run(out, query_latent, query_rope, cache, block_tables, query_start, context_lens, scale, max_query_len, max_context_len,
+                scales, timed=False)
+
+
+@torch.library.custom_op(f"{_NS}::attention_latent_expanded", mutates_args=("out",), device_types="cuda")
+def attention_latent_expanded(out: Tensor, query: Tensor, key: Tensor, rope_key: Tensor, value: Tensor, query_start: Tensor,
+                              key_start: Tensor, scale: float, max_query_len: int, max_key_len: int = 0) -> None:
+    _latent_expanded.run(out, query, key, rope_key, value, query_start, key_start, scale, max_query_len, max_key_len, timed=False)
+
+
 _NAMES = ("paged_attention_loop", "paged_attention_fp8_loop", "paged_attention_reduce", "paged_attention_fp8_reduce",
-          "kv_cache_write", "kv_cache_append", "paged_attention_ragged", "paged_attention_differential")
+          "kv_cache_write", "kv_cache_append", "paged_attention_ragged", "paged_attention_differential", "latent_cache_append",
+          "latent_cache_gather", "paged_attention_latent", "attention_latent_expanded")
 
 
 def _bind(L: ctypes.CDLL) -> None:
@@ -205,7 +248,9 @@ def _bind(L: ctypes.CDLL) -> None:
     entries = (L.fa_paged_attention_loop, L.fa_paged_attention_fp8_loop, L.fa_paged_attention_reduce,
                L.fa_paged_attention_fp8_reduce, L.fa_kv_cache_write, L.fa_paged_attention_loop_workspace_bytes,
                L.fa_kv_cache_append, L.fa_paged_attention_ragged, L.fa_paged_attention_differential,
-               L.fa_paged_attention_ragged_workspace_bytes)
+               L.fa_paged_attention_ragged_workspace_bytes, L.fa_latent_cache_append, L.fa_latent_cache_gather,
+               L.fa_paged_attention_latent, L.fa_paged_attention_latent_workspace_bytes, L.fa_attention_latent_expanded,
+               L.fa_attention_latent_expanded_workspace_bytes)
     table = (ctypes.c_void_p * len(entries))(*(ctypes.cast(e, ctypes.c_void_p).value for e in entries))
     global _native
     native = ctypes.CDLL(_build.TORCH_OPS_LIBRARY)
