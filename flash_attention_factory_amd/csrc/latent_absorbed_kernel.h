@@ -5,18 +5,23 @@
 //   S^T[key, row] = [c, r] Q^T      MFMA 16x16x32, A = cached rows from LDS, B = queries, in registers for good
 //   O^T[d, row]  += c^T P^T         MFMA 32x32x16, A = the same rows by transposing LDS reads, B = weights from LDS
 //
-// A work-group of eight wavefronts takes a tile of M rows and goes through 32 keys a step.  Scores: 16 rows and 16 keys to a wavefront
-// (M = 128: all 32; M = 32: four wavefronts have none).  Results: an eighth of the elements of all rows to a wavefront, so
-// that a value read from LDS serves M / 32 products; weights go through LDS.  Cached rows go from memory to LDS by themselves (loads that
-// write LDS), into a ring of steps, bytes of FP8 pools as they are: they are decoded on their way into the products.  One barrier a
-// step: between two of them a wavefront makes its scores of the next step and its results of this one.
+// A work-group of eight wavefronts takes a tile of M rows (32 or 64) and goes through 32 keys a step (bytes: 64).  Cached rows go from memory
+// to LDS by themselves (loads that write LDS), into a ring of steps, bytes of FP8 pools as they are: they are decoded on their way
+// into the products.  A round is a matrix phase -- scores of the next step, results of this one -- and a vector phase, the softmax:
+//   M = 64: four wavefronts, one on each SIMD, have the first 32 rows, the other four the others, one phase later, so that one
+//           wavefront of a SIMD is in its matrix phase while the other is in its vector phase.  Of its rows a wavefront has scores for 16 of them
+//           and half of the keys, and results for a quarter of the elements.
+//   M = 32: all wavefronts are in the same phase; 16 rows and 16 keys (with 32 keys a step, four wavefronts have none), an eighth of the elements.
+// Weights go through LDS, and so do the maxima of a row's keys, which several wavefronts have.
 //
 // Softmax against a reference m of each row that follows the maximum only where weights would pass 2^14 (kRefresh), and is set 2^6 below
-// it then (kHeadroom).  A step in which some row's reference has to move is done again after its barrier (raise), by all wavefronts
-// together.  Weights carry the scale of their row (FP8 pools): w = 2^(score - m) scale, and so does the maximum; the sum does not.
+// it then (kHeadroom); what there is of sums and results is multiplied then.  Weights carry the scale of their cached row (FP8 pools): w =
+// 2^(score - m) scale, and so does the maximum; the sum does not.
 //
 // All tiles of the batch lie end to end on a line, each as long as its steps, and every work-group takes an equal share (LatentLine);
-// pieces of cut tiles are joined by a second kernel.
+// pieces of cut tiles are joined by a second kernel.  Where sequences have several tiles, `team` of them lie side by side, and a share is
+// that of as many work-groups, on one XCC: they go through the same keys at the same time, which come from memory once (64
+// sequences of 512 to 16384 keys, 128 heads: 145 us and 15 us for the join).
 #pragma once
 
 #include "latent_cache_kernel.h"
@@ -24,6 +29,7 @@
 
 namespace fa {
 
+struct LatentJoin;
 struct LatentParams {
   RaggedBatch b;
   const char *cache;
@@ -36,45 +42,56 @@ struct LatentParams {
   int32_t num_heads, max_query_len;
   float score_scale_log2;  // |scale| * log2(e)
   uint32_t query_flip;     // 0x80008000 for a negative scale
-  int32_t groups;          // > 0: work-groups that share the line; 0: a work-group for each tile
-  float *part_o;           // pieces: [2 * work-group + (0: its first, 1: a later one)][registers of its wavefronts]
+  int32_t groups;          // > 0: shares of the line, at most; 0: a work-group for each tile
+  int32_t team;            // tiles side by side on the line
+  float *part_o;           // pieces: [2 * (share * team + place in the team) + (0: its first, 1: a later one)][registers of its wavefronts]
   float *part_ml;          // [...][2][row]
+  LatentJoin *joins;       // [share * team + place in the team]: the tile whose first cut is the end of the share
+  int32_t *shares;         // how many shares there are
 };
 
-constexpr int kLatentKeys = 32;       // keys of a step
-constexpr int kLatentStart = 6;       // what a tile costs apart from its steps, in steps
-constexpr int kLatentLeastShare = 8;  // no shares smaller than that, in steps
+// A tile that is cut: its pieces are those of the shares first .. last (none: first > last).
+struct LatentJoin {
+  int32_t seq, tile, first, last, first_slot;  // first_slot: of the first share's piece; of the others 2 * (share * team + place in the team)
+};
+
+// Keys of a step, what a tile costs apart from its steps, and the smallest share of the line (both in steps).
+template <bool KV8>
+struct LatentSteps {
+  static constexpr int kKeys = KV8 ? 64 : 32, kStart = KV8 ? 4 : 6, kLeast = KV8 ? 4 : 8;
+};
 constexpr float kNoReference = -1e30f;
 
 // A sequence as its tiles see it.
 struct LatentTiles {
   RaggedSeq q;
-  int rows, tiles, steps;  // steps of the last tile, at most what any tile has
-  __device__ __forceinline__ int64_t cost() const { return steps + kLatentStart; }
-  __device__ __forceinline__ int64_t all() const { return tiles * cost(); }
+  int rows, tiles, teams, steps;  // steps of the last tile, at most what any tile has
+  int64_t cost;                   // of a tile, or of those side by side
 };
-template <int M>
+template <typename T>
 __device__ __forceinline__ LatentTiles latent_tiles(const LatentParams &p, RaggedSeq q) {
   LatentTiles t;
   q.n = min(q.n, p.max_query_len);
   q.ctx = max(0, min(q.ctx, q.pos0 + q.n));
   t.q = q;
   t.rows = q.n * p.num_heads;
-  t.tiles = (t.rows + M - 1) / M;
-  t.steps = (q.ctx + kLatentKeys - 1) / kLatentKeys;
+  t.tiles = (t.rows + T::kRows - 1) / T::kRows;
+  t.teams = p.team == 1 ? t.tiles : (t.tiles + p.team - 1) / p.team;
+  t.steps = (q.ctx + T::kKeys - 1) / T::kKeys;
+  t.cost = t.steps + T::kStart;
   return t;
 }
 // Keys that the rows of a tile see: 0 .. latent_keys - 1.
-template <int M>
+template <typename T>
 __device__ __forceinline__ int latent_keys(const LatentParams &p, const LatentTiles &t, int tile) {
-  return max(0, attends_from(t.q, (min(tile * M + M, t.rows) - 1) / p.num_heads) + 1);
+  return max(0, attends_from(t.q, (min((tile + 1) * T::kRows, t.rows) - 1) / p.num_heads) + 1);
 }
 
 struct LatentPlace {
-  int seq, tile;
-  int64_t off;  // from the tile's start
+  int seq, team;  // team: which of the sequence's
+  int64_t off;    // from its start
 };
-template <int M>
+template <typename T>
 struct LatentLine {
   int64_t total;
   int groups;
@@ -88,10 +105,12 @@ struct LatentLine {
       for (int s = 64 + lane; s < p.b.num_seqs; s += 64) more += costs(p, s);
       total += readlane64(wave_inclusive_scan64(more, lane), 63);
     }
-    groups = (int)min((int64_t)p.groups, total / kLatentLeastShare + (total > 0));
+    groups = (int)min((int64_t)p.groups, total / T::kLeast + (total > 0));
   }
   static __device__ __forceinline__ int64_t costs(const LatentParams &p, int s) {
-    return s < p.b.num_seqs ? latent_tiles<M>(p, ragged_seq_of_lane(p.b, s)).all() : 0;
+    if (s >= p.b.num_seqs) return 0;
+    const LatentTiles t = latent_tiles<T>(p, ragged_seq_of_lane(p.b, s));
+    return t.teams * t.cost;
   }
   __device__ __forceinline__ int64_t cut(int g) const { return divide(total * g, groups); }
   // `at` < total
@@ -112,38 +131,52 @@ struct LatentLine {
       }
       before += readlane64(sum, 63);
     }
-    const LatentTiles t = latent_tiles<M>(p, ragged_seq_uniform(p.b, r.seq));
+    const LatentTiles t = latent_tiles<T>(p, ragged_seq_uniform(p.b, r.seq));
     const int64_t in = at - before;
-    r.tile = __builtin_amdgcn_readfirstlane((int)divide(in, (int)t.cost()));
-    r.off = in - r.tile * t.cost();
+    r.team = __builtin_amdgcn_readfirstlane((int)divide(in, (int)t.cost));
+    r.off = in - r.team * t.cost;
     return r;
   }
 };
 // The step that a cut `off` into a tile of `steps` steps lies before.
-__device__ __forceinline__ int latent_cut_step(int64_t off, int steps) { return min(max((int)off - kLatentStart, 0), steps); }
+template <typename T>
+__device__ __forceinline__ int latent_cut_step(int64_t off, int steps) {
+  return min(max((int)off - T::kStart, 0), steps);
+}
 
 template <int L, typename OT, bool KV8, int M>
-struct LatentAbsorbed {
+struct LatentAbsorbed : LatentSteps<KV8> {
+  static constexpr int kRows = M, kKeys = LatentSteps<KV8>::kKeys;
+  static constexpr bool kTurns = M == 64;
   static constexpr int kRowElements = L + kLatentRope;
   static constexpr int kRowBytes = kRowElements * (KV8 ? 1 : 2);
-  static constexpr int kStepBytes = kLatentKeys * kRowBytes;
-  static constexpr int kRing = !KV8 && M == 128 && L == 512 ? 3 : 4;  // steps in LDS (4 of 36 KiB and more weights pass 160 KiB)
-  static constexpr int kWeights = kRing * kStepBytes;                 // [2][M][32] 16-bit
-  static constexpr int kScales = kWeights + 2 * M * 64;               // [ring][32]
-  static constexpr int kTops = kScales + (KV8 ? kRing * 128 : 0);     // [2][M]: maxima of a step's halves, factors, sums
-  static constexpr int kFlags = kTops + 2 * M * 4;                    // [2]: whether a reference has to move
+  static constexpr int kStepBytes = kKeys * kRowBytes;
+  static constexpr int kParts = kTurns ? 2 : kKeys / 16;        // of a step's keys, among wavefronts with the same rows
+  static constexpr int kTiles = kKeys / 16 / kParts;            // of 16 keys, in a part
+  static constexpr int kOthers = M * kKeys * 2 + (kParts + 1) * M * 4 + 16;  // LDS beside the ring and its scales
+  static constexpr int kRing = (160 * 1024 - kOthers) / (kStepBytes + kKeys * 4) < 7 ? (160 * 1024 - kOthers) / (kStepBytes + kKeys * 4) : 7;
+  static constexpr int kScales = kRing * kStepBytes;            // [ring][key]
+  static constexpr int kWeights = kScales + (KV8 ? kRing * kKeys * 4 : 0);  // [row][key] 16-bit
+  static constexpr int kTops = kWeights + M * kKeys * 2;        // [part][row]: maxima
+  static constexpr int kFactors = kTops + kParts * M * 4;       // [row]: what sums and results are multiplied with
+  static constexpr int kFlags = kFactors + M * 4;               // [strip of 16 rows]: whether there are factors
   static constexpr int kLdsBytes = kFlags + 16;
-  static constexpr int kPieces = kRowBytes / 16;                      // of 16 bytes, of a row
-  static constexpr int kLoads = (4 * kPieces + 63) / 64;              // instructions for a wavefront's four rows
-  static constexpr int kInFlight = kLoads + KV8;                      // ... and for their scales
-  static constexpr int KT = M == 128 ? 2 : 1;                         // 16-key tiles of a wavefront's scores
-  static constexpr int RT = M / 32, DT = L / 256, KS = kRowElements / 32;
-  static_assert(kLdsBytes <= 160 * 1024, "");
+  static constexpr int kOwn = kKeys / 8;                        // rows of a step that a wavefront loads
+  static constexpr int kPieces = kRowBytes / 16;                // of 16 bytes, of a row
+  static constexpr int kLoads = (kOwn * kPieces + 63) / 64;     // instructions for them
+  static constexpr int kInFlight = kLoads + KV8;                // ... and for their scales
+  static constexpr int kSlices = kTurns ? 4 : 8;                // of the results' elements
+  static constexpr int DT = L / kSlices / 32, KS = kRowElements / 32;
+  static_assert(kLdsBytes <= 160 * 1024 && kRing >= 4 && (kRing - 3) * kInFlight < 64, "");
 
   // Which 16-byte piece of a row lies at piece c of its place in LDS (and the other way round).  16 lanes that read one piece of 16
   // rows, and 32 that read 4 rows of 64 bytes (16-bit pools) or 8 rows of 32 bytes (bytes), meet in no bank.
   static __device__ __forceinline__ int swizzle(int key) {
     return KV8 ? ((key >> 2) & 1) * 2 + ((key >> 3) & 1) : ((key >> 1) & 1) * 4 + ((key >> 2) & 3);
+  }
+  // Where 16-byte piece c of a row of weights lies: 16 rows' same piece meets in no bank.
+  static __device__ __forceinline__ int weights_at(int row, int c) {
+    return kWeights + row * kKeys * 2 + (c ^ (kKeys == 32 ? (row >> 2) & 3 : (row >> 1) & 7)) * 16;
   }
 };
 
@@ -180,34 +213,52 @@ __device__ __forceinline__ u32x4 decoded(u32x2 bytes) {
 template <int L, typename OT, bool KV8, int M>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) latent_absorbed_kernel(const LatentParams p) {
   using T = LatentAbsorbed<L, OT, KV8, M>;
-  constexpr int RT = T::RT, DT = T::DT, KS = T::KS, KT = T::KT;
+  constexpr int DT = T::DT, KS = T::KS, KT = T::kTiles;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
 
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, quarter = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int strip = KT == 2 ? wave : wave >> 1, key0 = KT == 2 ? 0 : (wave & 1) * 16;  // this wavefront's rows and keys of the scores
-  const bool scores_here = strip * 16 < M;
+  // this wavefront's rows and keys of the scores, rows and elements of the results
+  const int strip = wave / T::kParts, key_part = wave % T::kParts, key0 = key_part * 16 * KT;
+  const bool scores_here = T::kTurns || strip * 16 < M;
+  const int result_row0 = T::kTurns ? (wave >> 2) * 32 : 0, slice = wave % T::kSlices;
+  const bool late = T::kTurns && wave >= 4;
   const int H = p.num_heads;
 
   // ---- this work-group's tiles ----
-  int seq, tile, from = 0, g = blockIdx.x, end_seq, end_tile, end_cut = 0x7fffffff;
+  int seq, team, from = 0, place = 0, part = blockIdx.x, end_seq, end_team, end_cut = 0x7fffffff;  // place: in the team
   if (p.groups > 0) {
-    const LatentLine<M> line(p, lane);
-    const int per = (line.groups + 7) >> 3;  // work-groups go to the eight XCCs in turn: each gets an eighth of the line
-    g = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
-    if (((int)blockIdx.x >> 3) >= per || g >= line.groups) return;
+    const LatentLine<T> line(p, lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.shares = line.groups;
+    const int per = (line.groups + 7) >> 3, in_xcc = (int)blockIdx.x >> 3;  // work-groups go to the eight XCCs in turn: each gets an eighth of the line
+    const int g = ((int)blockIdx.x & 7) * per + in_xcc / p.team;
+    if (in_xcc / p.team >= per || g >= line.groups) return;
+    place = in_xcc % p.team, part = g * p.team + place;
     const LatentPlace at = line.find(p, line.cut(g), lane), to = line.find(p, line.cut(g + 1) - 1, lane);
-    seq = at.seq, tile = at.tile, end_seq = to.seq, end_tile = to.tile;
-    const LatentTiles t0 = latent_tiles<M>(p, ragged_seq_uniform(p.b, seq)), t1 = latent_tiles<M>(p, ragged_seq_uniform(p.b, end_seq));
-    from = latent_cut_step(at.off, (latent_keys<M>(p, t0, tile) + kLatentKeys - 1) / kLatentKeys);
-    if (to.off + 1 < t1.cost()) end_cut = latent_cut_step(to.off + 1, (latent_keys<M>(p, t1, end_tile) + kLatentKeys - 1) / kLatentKeys);
+    seq = at.seq, team = at.team, end_seq = to.seq, end_team = to.team;
+    const LatentTiles t0 = latent_tiles<T>(p, ragged_seq_uniform(p.b, seq)), t1 = latent_tiles<T>(p, ragged_seq_uniform(p.b, end_seq));
+    const int end_tile = to.team * p.team + place;
+    const int end_steps = end_tile < t1.tiles ? (latent_keys<T>(p, t1, end_tile) + T::kKeys - 1) / T::kKeys : 0;
+    from = latent_cut_step<T>(at.off, t0.steps);
+    if (to.off + 1 < t1.cost) end_cut = latent_cut_step<T>(to.off + 1, t1.steps);
     from = __builtin_amdgcn_readfirstlane(from), end_cut = __builtin_amdgcn_readfirstlane(end_cut);
+    if (wave == 7) {  // what the join is told of the cut at this share's end
+      LatentJoin join = {to.seq, end_tile, 1, 0, 0};
+      const int64_t start = line.cut(g + 1) - 1 - to.off;
+      if (to.off + 1 < t1.cost && line.cut(g) <= start && end_steps > 0) {
+        int first = g, last = min((int)divide((start + T::kStart + end_steps - 1) * line.groups, line.total) + 1, line.groups - 1);
+        while (latent_cut_step<T>(line.cut(first + 1) - start, end_steps) == 0) ++first;
+        while (line.cut(last) - start - T::kStart >= end_steps) --last;
+        if (first < last) join.first = first, join.last = last, join.first_slot = 2 * (first * p.team + place) + (first == g && line.cut(g) < start);
+      }
+      if (lane == 0) p.joins[part] = join;
+    }
   } else {
-    const RaggedPlace at = ragged_find(p.b.num_seqs, blockIdx.x, lane, [&](int s) { return latent_tiles<M>(p, ragged_seq_of_lane(p.b, s)).tiles; });
+    const RaggedPlace at = ragged_find(p.b.num_seqs, blockIdx.x, lane, [&](int s) { return latent_tiles<T>(p, ragged_seq_of_lane(p.b, s)).tiles; });
     seq = end_seq = __builtin_amdgcn_readfirstlane(at.seq);
     if (seq >= p.b.num_seqs) return;
-    tile = end_tile = (int)blockIdx.x - __builtin_amdgcn_readfirstlane(at.before);
+    team = end_team = (int)blockIdx.x - __builtin_amdgcn_readfirstlane(at.before);
   }
   auto meet = [&]() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -219,44 +270,40 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   uint32_t load_off[T::kLoads];
 #pragma unroll
   for (int i = 0; i < T::kLoads; ++i) {
-    const int slot = i * 64 + lane, r = min(slot / T::kPieces, 3), c = slot - slot / T::kPieces * T::kPieces;
-    load_off[i] = (uint32_t)r * p.token_bytes + (c ^ T::swizzle(wave * 4 + r)) * 16;
+    const int slot = i * 64 + lane, r = min(slot / T::kPieces, T::kOwn - 1), c = slot - slot / T::kPieces * T::kPieces;
+    load_off[i] = (uint32_t)r * p.token_bytes + (c ^ T::swizzle(wave * T::kOwn + r)) * 16;
   }
-  const bool last_load = (T::kLoads - 1) * 64 + lane < 4 * T::kPieces;
-  // Where this lane reads: a cached row's piece for the scores, its transposed pieces for the results, weights.  The swizzles are
-  // exclusive-ors in the low bits of the pieces' numbers, so that some products or result tiles further on is an offset.
-  constexpr int kRowBases = 2;
-  int row_at[kRowBases], value_at[4];
+  const bool last_load = (T::kLoads - 1) * 64 + lane < T::kOwn * T::kPieces;
+  // Where this lane reads: a cached row's piece for the scores, its transposed pieces for the results.  The swizzles are exclusive-ors in
+  // the low bits of the pieces' numbers, so that two products or result tiles further on is an offset.
+  int row_at[2], value_at[4];
 #pragma unroll
-  for (int k = 0; k < kRowBases; ++k) {
+  for (int k = 0; k < 2; ++k) {
     const int key = key0 + i16;
     row_at[k] = key * T::kRowBytes + (KV8 ? ((2 * k + (quarter >> 1)) ^ T::swizzle(key)) * 16 + (quarter & 1) * 8 : ((4 * k + quarter) ^ T::swizzle(key)) * 16);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    if constexpr (KV8) {
-      const int key = 8 * half + (i16 >> 1), c = wave * (L / 128) + (k & 1) * 2 + ((lane >> 4) & 1);
-      value_at[k] = key * T::kRowBytes + (c ^ T::swizzle(key)) * 16 + (i16 & 1) * 8;
-    } else {
-      const int key = 8 * half + (i16 >> 2) + (k >> 1) * 4, c = wave * (L / 64) + (k & 1) * 4 + ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1);
-      value_at[k] = key * T::kRowBytes + (c ^ T::swizzle(key)) * 16 + (i16 & 1) * 8;
-    }
+    const int key = 8 * half + (KV8 ? i16 >> 1 : (i16 >> 2) + (k >> 1) * 4);
+    const int c = slice * (L / T::kSlices * (KV8 ? 1 : 2) / 16) + (KV8 ? (k & 1) * 2 + ((lane >> 4) & 1) : (k & 1) * 4 + ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1));
+    value_at[k] = key * T::kRowBytes + (c ^ T::swizzle(key)) * 16 + (i16 & 1) * 8;
   }
-  float *tops = reinterpret_cast<float *>(lds + T::kTops);
+  float *tops = reinterpret_cast<float *>(lds + T::kTops), *factors = reinterpret_cast<float *>(lds + T::kFactors);
   int *flags = reinterpret_cast<int *>(lds + T::kFlags);
 
   bool first_piece = true;
   for (;; first_piece = false) {
-    const LatentTiles t = latent_tiles<M>(p, ragged_seq_uniform(p.b, seq));
+    const LatentTiles t = latent_tiles<T>(p, ragged_seq_uniform(p.b, seq));
     const RaggedSeq &q = t.q;
-    const bool last_tile = seq == end_seq && tile == end_tile;
-    const int keys = __builtin_amdgcn_readfirstlane(latent_keys<M>(p, t, tile));
-    const int all_steps = (keys + kLatentKeys - 1) / kLatentKeys, until = last_tile ? min(end_cut, all_steps) : all_steps;
+    const bool last_team = seq == end_seq && team == end_team;
+    const int tile = team * p.team + place;
+    const int keys = __builtin_amdgcn_readfirstlane(latent_keys<T>(p, t, tile));
+    const int all_steps = (keys + T::kKeys - 1) / T::kKeys, until = last_team ? min(end_cut, all_steps) : all_steps;
     const bool whole = from == 0 && until == all_steps;
-    if (t.rows > 0 && (whole || from < until)) {  // (a tile that sees no keys is whole: its rows get zeros)
+    if (tile < t.tiles && (whole || from < until)) {  // (a tile that sees no keys is whole: its rows get zeros)
       const int steps = until - from, row0 = tile * M;
       // this lane's row of the scores (rows past the end repeat the last one and are not stored)
-      const int my_row = (strip * 16 + i16) % M, row = min(row0 + my_row, t.rows - 1);
+      const int my_row = (strip * 16 + i16) & (M - 1), row = min(row0 + my_row, t.rows - 1);
       const int j = row / H, head = row - j * H, pos = attends_from(q, j);
       const int wave_lo = attends_from(q, min(row0 + strip * 16, t.rows - 1) / H);
 
@@ -271,43 +318,41 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
           for (int k = 0; k < 4; ++k) qv[c][k] ^= p.query_flip;
         }
       }
-      float m = kNoReference, l = 0.f, part = 0.f;  // part: of the sum, by the step at hand
-      f32x16 acc[DT][RT];
+      float m = kNoReference, l = 0.f;
+      f32x16 acc[DT];
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[d][r][e] = 0.f;
+        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
 
-      // ---- loads of a step: a wavefront has four of its rows, which lie in one block ----
+      // ---- loads of a step: a wavefront has an eighth of its rows, which lie in one block ----
       const int32_t *table = p.b.block_tables + (int64_t)seq * p.b.max_blocks_per_seq;
       const int last_col = p.b.max_blocks_per_seq - 1, in_block = (1 << p.b.block_shift) - 1;
-      auto id_of = [&](int n) { return load_uniform_i32(table + min(((from + n) * kLatentKeys + wave * 4) >> p.b.block_shift, last_col)); };
+      auto id_of = [&](int n) { return load_uniform_i32(table + min(((from + n) * T::kKeys + wave * T::kOwn) >> p.b.block_shift, last_col)); };
       int32_t next_id = id_of(0);
       auto issue = [&](int n, int slot) __attribute__((always_inline)) {
         const uint32_t id = min((uint32_t)__builtin_amdgcn_readfirstlane(next_id), (uint32_t)p.b.max_block_id);
-        const uint32_t r0 = (uint32_t)((from + n) * kLatentKeys + wave * 4) & in_block;
+        const uint32_t r0 = (uint32_t)((from + n) * T::kKeys + wave * T::kOwn) & in_block;
         const char *base = uniform_address(p.cache + ((uint64_t)id * p.block_bytes + (uint64_t)r0 * p.token_bytes));
-        const uint32_t to = lds_at + slot * T::kStepBytes + wave * 4 * T::kRowBytes;
+        const uint32_t to = lds_at + slot * T::kStepBytes + wave * T::kOwn * T::kRowBytes;
 #pragma unroll
         for (int i = 0; i < T::kLoads; ++i) {
-          if ((i + 1) * 64 <= 4 * T::kPieces || last_load) load_to_lds_16(__builtin_amdgcn_readfirstlane(to + i * 1024), load_off[i], base);
+          if ((i + 1) * 64 <= T::kOwn * T::kPieces || last_load) load_to_lds_16(__builtin_amdgcn_readfirstlane(to + i * 1024), load_off[i], base);
         }
         if constexpr (KV8) {
           const char *scales = uniform_address(reinterpret_cast<const char *>(p.scales + (((uint64_t)id << p.b.block_shift) + r0)));
-          if (lane < 4) load_to_lds_4(__builtin_amdgcn_readfirstlane(lds_at + T::kScales + slot * 128 + wave * 16), lane * 4, scales);
+          if (lane < T::kOwn) load_to_lds_4(__builtin_amdgcn_readfirstlane(lds_at + T::kScales + (slot * T::kKeys + wave * T::kOwn) * 4), lane * 4, scales);
         }
         next_id = id_of(n + 1);
       };
       // Rows of a step that no row of the tile sees may hold anything: zeros instead.  By the wavefront that has loaded them.
       auto clear_unseen = [&](int n, int slot) {
-        const int k0 = (from + n) * kLatentKeys + wave * 4;
-        for (int r = min(max(keys - k0, 0), 4); r < 4; ++r) {
-          char *dst = lds + slot * T::kStepBytes + (wave * 4 + r) * T::kRowBytes;
+        const int k0 = (from + n) * T::kKeys + wave * T::kOwn;
+        for (int r = min(max(keys - k0, 0), T::kOwn); r < T::kOwn; ++r) {
+          char *dst = lds + slot * T::kStepBytes + (wave * T::kOwn + r) * T::kRowBytes;
           if (lane < T::kPieces) *reinterpret_cast<u32x4 *>(dst + lane * 16) = u32x4{0u, 0u, 0u, 0u};
           if (64 + lane < T::kPieces) *reinterpret_cast<u32x4 *>(dst + (64 + lane) * 16) = u32x4{0u, 0u, 0u, 0u};
-          if (KV8 && lane == 0) *reinterpret_cast<float *>(lds + T::kScales + slot * 128 + (wave * 4 + r) * 4) = 0.f;
+          if (KV8 && lane == 0) *reinterpret_cast<float *>(lds + T::kScales + (slot * T::kKeys + wave * T::kOwn + r) * 4) = 0.f;
         }
       };
 
@@ -317,139 +362,126 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         if constexpr (KV8) return decoded<OT>(a);
         else return a;
       };
-      auto row_operand = [&](const char *rows, int c, int kt) {
-        rows += kt * 16 * T::kRowBytes;
+      auto row_operand = [&](const char *rows, int o) {  // product o: k-step o / KT of key tile o % KT
+        const int c = o / KT;
+        rows += o % KT * 16 * T::kRowBytes;
         if constexpr (KV8) return *reinterpret_cast<const u32x2 *>(rows + row_at[c & 1] + (c >> 1) * 64);
         else return *reinterpret_cast<const u32x4 *>(rows + row_at[c & 1] + (c >> 1) * 128);
       };
       auto value_operand = [&](const char *rows, int ks, int d) {
         rows += 16 * ks * T::kRowBytes;
         if constexpr (KV8) {
-          return lds_read_transposed_bytes(rows + value_at[d & 1]);
+          return lds_read_transposed_bytes(rows + value_at[d & 1] + (d >> 1) * 64);
         } else {
-          const u32x2 a0 = lds_read_transposed(rows + value_at[d & 1]);
-          const u32x2 a1 = lds_read_transposed(rows + value_at[2 + (d & 1)]);
+          const u32x2 a0 = lds_read_transposed(rows + value_at[d & 1] + (d >> 1) * 128);
+          const u32x2 a1 = lds_read_transposed(rows + value_at[2 + (d & 1)] + (d >> 1) * 128);
           return u32x4{a0[0], a0[1], a1[0], a1[1]};
         }
       };
 
-      f32x4 x[KT];  // scores of the step that is not summed yet: element e is key key0 + 16 kt + 4 quarter + e of the step
-      auto scores = [&](int slot) __attribute__((always_inline)) {
-        const char *rows = lds + slot * T::kStepBytes;
-        // kAhead operands are on their way at any time; the order is held with scheduling barriers, since left to itself the compiler
-        // asks for as many as there are and spills the rest
-        constexpr int kAhead = 4, kAll = KS * KT;
-        Raw a[kAhead];
+      // Scores of the step that softmax comes to next, times scale and log2(e): element e of tile kt is key key0 + 16 kt + 4 quarter + e.
+      f32x4 x[KT], s[KT];  // s: the rows' scales
+      // The matrix phase: scores of step n + 1, then results of step n.  kAhead operands are on their way at any time; the order is held with
+      // scheduling barriers, since left to itself the compiler asks for as many as there are and spills the rest.
+      auto matrix_phase = [&](int n, int here, int next, auto with_scores, auto with_results) __attribute__((always_inline)) {
+        constexpr bool kScores = decltype(with_scores)::value, kResults = decltype(with_results)::value;
+        constexpr int kAhead = 6, kAll = KS * KT, kSteps = T::kKeys / 16;
+        const char *values = lds + here * T::kStepBytes, *rows = lds + next * T::kStepBytes;
+        u32x2 moved = {0u, 0u};
+        u32x4 b[kSteps];
+        if constexpr (kResults) {
+          moved = *reinterpret_cast<const u32x2 *>(flags + result_row0 / 16);
 #pragma unroll
-        for (int o = 0; o < kAhead; ++o) a[o] = row_operand(rows, o / KT, o % KT);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int ks = 0; ks < kSteps; ++ks) b[ks] = *reinterpret_cast<const u32x4 *>(lds + T::weights_at(result_row0 + col, 2 * ks + half));
+        }
+        if constexpr (kScores) {
+          f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // two, for products that need not wait for each other
+          Raw a[kAhead];
 #pragma unroll
-        for (int o = 0; o < kAll; ++o) {
-          const int c = o / KT, kt = o % KT;
-          x[kt] = mfma_16x16x32<OT>(operand(a[o % kAhead]), qv[c], c == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : x[kt]);
-          if (o + kAhead < kAll) a[o % kAhead] = row_operand(rows, (o + kAhead) / KT, (o + kAhead) % KT);
+          for (int o = 0; o < kAhead; ++o) a[o] = row_operand(rows, o);
           __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int o = 0; o < kAll; ++o) {
+            sum[o & 1] = mfma_16x16x32<OT>(operand(a[o % kAhead]), qv[o / KT], sum[o & 1]);
+            if (o + kAhead < kAll) a[o % kAhead] = row_operand(rows, o + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if constexpr (KT == 1) x[0] = sum[0] + sum[1];
+          else x[0] = sum[0], x[KT - 1] = sum[1];
+        }
+        if constexpr (kResults) {
+          constexpr int kValues = kSteps * DT, kFirst = 4;
+          Raw v[kFirst];
+#pragma unroll
+          for (int o = 0; o < kFirst && o < kValues; ++o) v[o] = value_operand(values, o / DT, o % DT);
+          if (__builtin_expect(__builtin_amdgcn_readfirstlane((int)(moved[0] | moved[1])), 0)) {
+            const bool is = col < 16 ? moved[0] != 0u : moved[1] != 0u;
+            const float f = is ? factors[result_row0 + col] : 1.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= f;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int o = 0; o < kValues; ++o) {
+            acc[o % DT] = mfma_32x32x16<OT>(operand(v[o % kFirst]), b[o / DT], acc[o % DT]);
+            if (o + kFirst < kValues) v[o % kFirst] = value_operand(values, (o + kFirst) / DT, (o + kFirst) % DT);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        if constexpr (kScores) {  // the largest of each row's keys, for the other wavefronts that have keys of it
+          const int t0 = (from + n + 1) * T::kKeys + key0;
+          float top = -INFINITY;
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            if constexpr (KV8) s[kt] = *reinterpret_cast<const f32x4 *>(lds + T::kScales + (next * T::kKeys + key0 + 16 * kt + 4 * quarter) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[kt][e] *= KV8 ? p.score_scale_log2 * s[kt][e] : p.score_scale_log2;
+          }
+          if (t0 + 16 * KT - 1 > wave_lo) {
+            const int hi = pos - t0 - 4 * quarter;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[kt][e] = 16 * kt + e > hi ? -INFINITY : x[kt][e];
+          }
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, KV8 ? x[kt][e] + __builtin_amdgcn_logf(s[kt][e]) : x[kt][e]);
+          top = rows_max(top);
+          if (quarter == 0) tops[key_part * M + my_row] = top;
         }
       };
-      float s[4 * KT];  // scales of the step's rows
-      auto weights = [&](int n) __attribute__((always_inline)) {  // stores them, returns the largest
-        float most = 0.f;
+      // The vector phase: weights of the scores, to LDS.
+      auto softmax = [&]() __attribute__((always_inline)) {
+        float top = tops[my_row];
+#pragma unroll
+        for (int k = 1; k < T::kParts; ++k) top = fmaxf(top, tops[k * M + my_row]);
+        int moved = 0;
+        if (__builtin_expect(__any(top - m > kRefresh), 0)) {
+          const float to = top - m > kRefresh ? top - kHeadroom : m, alpha = fast_exp2(m - to);
+          l *= alpha;
+          m = to;
+          moved = 1;
+          if (key_part == 0 && quarter == 0) factors[my_row] = alpha;
+        }
+        if (key_part == 0 && lane == 0) flags[strip] = moved;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
           float w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float v = fast_exp2(x[kt][e] - m);
-            part = kt == 0 && e == 0 ? v : part + v;
-            w[e] = KV8 ? v * s[4 * kt + e] : v;
+            w[e] = fast_exp2(x[kt][e] - m);
+            l += w[e];
+            if constexpr (KV8) w[e] *= s[kt][e];
           }
-          most = max3(max3(most, w[0], w[1]), w[2], w[3]);
-          const int at = key0 / 8 + 2 * kt + (quarter >> 1);
-          *reinterpret_cast<u32x2 *>(lds + T::kWeights + ((n & 1) * M + my_row) * 64 + ((at ^ ((my_row >> 2) & 3)) * 16) + (quarter & 1) * 8) =
+          *reinterpret_cast<u32x2 *>(lds + T::weights_at(my_row, key0 / 8 + 2 * kt + (quarter >> 1)) + (quarter & 1) * 8) =
               u32x2{pack2<OT>(w[0], w[1]), pack2<OT>(w[2], w[3])};
-        }
-        return most;
-      };
-      auto softmax = [&](int n, int slot) __attribute__((always_inline)) {
-        const int t0 = (from + n) * kLatentKeys + key0;
-        l += part;
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          f32x4 v = {1.f, 1.f, 1.f, 1.f};
-          if constexpr (KV8) v = *reinterpret_cast<const f32x4 *>(lds + T::kScales + slot * 128 + (key0 + 16 * kt + 4 * quarter) * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[4 * kt + e] = v[e];
-            x[kt][e] *= KV8 ? p.score_scale_log2 * v[e] : p.score_scale_log2;
-          }
-        }
-        if (t0 + 16 * KT - 1 > wave_lo) {
-          const int hi = pos - t0 - 4 * quarter;
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[kt][e] = 16 * kt + e > hi ? -INFINITY : x[kt][e];
-        }
-        constexpr float kMost = 16384.f;  // 2^kRefresh
-        if (__builtin_expect(__any(weights(n) > kMost), 0) && lane == 0) flags[n & 1] = 1;
-      };
-      // The references of step n move, where weights pass 2^kRefresh, and with them what there is of sums and results.
-      auto raise = [&](int n) {
-        if (scores_here) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, KV8 ? x[kt][e] + __builtin_amdgcn_logf(s[4 * kt + e]) : x[kt][e]);
-          top = rows_max(top);
-          if (quarter == 0) tops[(KT == 1 ? wave & 1 : 0) * M + my_row] = top;
-        }
-        meet();
-        float alpha = 1.f;
-        if (scores_here) {
-          float top = tops[my_row];
-          if (KT == 1) top = fmaxf(top, tops[M + my_row]);
-          const float to = top > m + kRefresh ? top - kHeadroom : m;
-          alpha = fast_exp2(m - to);
-          l *= alpha;
-          m = to;
-          weights(n);
-        }
-        meet();
-        if (scores_here && quarter == 0 && key0 == 0) tops[my_row] = alpha;
-        if (threadIdx.x == 0) flags[n & 1] = 0;
-        meet();
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const float f = tops[r * 32 + col];
-#pragma unroll
-          for (int d = 0; d < DT; ++d) acc[d][r] *= f;
-        }
-      };
-      auto results = [&](int n, int slot) __attribute__((always_inline)) {
-        const char *rows = lds + slot * T::kStepBytes;
-        const char *from_weights = lds + T::kWeights + ((n & 1) * M + col) * 64;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          Raw a[DT];
-          u32x4 b[RT];
-#pragma unroll
-          for (int d = 0; d < DT; ++d) a[d] = value_operand(rows, ks, d);
-#pragma unroll
-          for (int r = 0; r < RT; ++r)
-            b[r] = *reinterpret_cast<const u32x4 *>(from_weights + r * 32 * 64 + (((2 * ks + half) ^ ((col >> 2) & 3)) * 16));
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const u32x4 v = operand(a[d]);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) acc[d][r] = mfma_32x32x16<OT>(v, b[r], acc[d][r]);
-          }
         }
       };
 
-      // ---- steps: in round n the scores of step n + 1 and the results of step n ----
+      // ---- rounds: in round n the scores of step n + 1, the results of step n, and the softmax of step n + 1 ----
       if (!first_piece) meet();  // LDS of the piece before has been read
-      if (threadIdx.x < 2) flags[threadIdx.x] = 0;
       if (steps > 0) {
         constexpr int R = T::kRing;
         for (int n = 0; n < min(R - 2, steps); ++n) issue(n, n);
@@ -457,147 +489,169 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         else wait_loads<0>();
         if (steps == 1) clear_unseen(0, 0);
         meet();
-        int here = 0, next = 1, far = R - 2;  // places in the ring of steps n, n + 1, n + R - 2
-        auto land = [&](int n) {              // step n has landed, those after it are on their way
+        if (late) meet();
+        int here = R - 1, next = 0, far = R - 2;  // places in the ring of steps n, n + 1, n + R - 1
+        auto land = [&](int n) __attribute__((always_inline)) {  // step n has landed, those after it are on their way
           if (n + R - 3 < steps) wait_loads<(R - 3) * T::kInFlight>();
           else wait_loads<0>();
-          if (n == steps - 1) clear_unseen(n, next);
-          meet();
+          if (n == steps - 1) clear_unseen(n, next + 1 == R ? 0 : next + 1);
         };
-        if (R - 2 < steps) issue(R - 2, far);
-        if (scores_here) {
-          scores(0);
-          softmax(0, 0);
-        }
-        land(1);
-        for (int n = 0; n < steps - 1;) {
-          if (__builtin_amdgcn_readfirstlane(flags[n & 1])) raise(n);
-          do {
-            far = far + 1 == R ? 0 : far + 1;
-            if (n + R - 1 < steps) issue(n + R - 1, far);
-            if (scores_here) scores(next);
-            results(n, here);
-            if (scores_here) softmax(n + 1, next);
-            here = next, next = next + 1 == R ? 0 : next + 1;
-            land(n + 2);
-            ++n;
-          } while (n < steps - 1 && !__builtin_amdgcn_readfirstlane(flags[n & 1]));
-        }
-        if (__builtin_amdgcn_readfirstlane(flags[(steps - 1) & 1])) raise(steps - 1);
-        results(steps - 1, here);
-        l += part;
+        auto round = [&](int n, auto with_results) __attribute__((always_inline)) {
+          if (n + R - 1 < steps) issue(n + R - 1, far);
+          if (scores_here) matrix_phase(n, here, next, std::true_type{}, with_results);
+          else matrix_phase(n, here, next, std::false_type{}, with_results);
+          if (late) land(n + 2);
+          meet();
+          if (scores_here) softmax();
+          if (!late) land(n + 2);
+          meet();
+          here = next, next = next + 1 == R ? 0 : next + 1, far = far + 1 == R ? 0 : far + 1;
+        };
+        round(-1, std::false_type{});
+        for (int n = 0; n < steps - 1; ++n) round(n, std::true_type{});
+        matrix_phase(steps - 1, here, next, std::false_type{}, std::true_type{});
+        if (T::kTurns && !late) meet();
         meet();
       }
 
-      // ---- results: element e of acc[d][r] is element w L / 8 + 32 d + 8 (e / 4) + 4 half + e % 4 of row 32 r + col ----
-      float *stats = reinterpret_cast<float *>(lds + T::kWeights);  // references [M], then sums [M] of each half of the keys
+      // ---- results: element e of acc[d] is element slice L / slices + 32 d + 8 (e / 4) + 4 half + e % 4 of row result_row0 + col ----
+      float *stats = reinterpret_cast<float *>(lds + T::kWeights);  // references [M], then sums [M] of each part of the keys
       if (scores_here) {
         l = rows_sum(l);
         if (quarter == 0) {
-          if (key0 == 0) stats[my_row] = m;
-          stats[(KT == 1 ? 1 + (wave & 1) : 1) * M + my_row] = l;
+          if (key_part == 0) stats[my_row] = m;
+          stats[(1 + key_part) * M + my_row] = l;
         }
       }
       meet();
-      auto sum_of = [&](int r) { return KT == 1 ? stats[M + r] + stats[2 * M + r] : stats[M + r]; };
+      auto sum_of = [&](int r) {
+        float sum = stats[M + r];
+#pragma unroll
+        for (int k = 1; k < T::kParts; ++k) sum += stats[(1 + k) * M + r];
+        return sum;
+      };
       if (whole) {
+        const int out_row = row0 + result_row0 + col, stored = min(out_row, t.rows - 1), token = stored / H;
+        const float sum = sum_of(result_row0 + col), inv = sum == 0.f ? 0.f : 1.0f / sum;
+        char *dst = p.out + (int64_t)(q.first + token) * p.out_token_bytes + (stored - token * H) * p.out_head_bytes + slice * (DT * 64) + half * 8;
+        if (out_row < t.rows) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const int out_row = row0 + r * 32 + col, stored = min(out_row, t.rows - 1), token = stored / H;
-          const float sum = sum_of(r * 32 + col), inv = sum == 0.f ? 0.f : 1.0f / sum;
-          char *dst = p.out + (int64_t)(q.first + token) * p.out_token_bytes + (stored - token * H) * p.out_head_bytes + wave * (L / 4) + half * 8;
-          if (out_row < t.rows) {
+          for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<u32x2 *>(dst + d * 64 + k * 16) = u32x2{pack2<OT>(acc[d][r][4 * k] * inv, acc[d][r][4 * k + 1] * inv),
-                                                                          pack2<OT>(acc[d][r][4 * k + 2] * inv, acc[d][r][4 * k + 3] * inv)};
-          }
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<u32x2 *>(dst + d * 64 + k * 16) =
+                  u32x2{pack2<OT>(acc[d][4 * k] * inv, acc[d][4 * k + 1] * inv), pack2<OT>(acc[d][4 * k + 2] * inv, acc[d][4 * k + 3] * inv)};
         }
       } else {
         // a piece: as it lies in the registers, 1 KiB at a time
-        const int64_t slot = 2 * (int64_t)g + (first_piece ? 0 : 1);
-        float *dst = p.part_o + (slot * 8 + wave) * (DT * RT * 1024) + lane * 4;
+        const int64_t slot = 2 * (int64_t)part + (first_piece ? 0 : 1);
+        float *dst = p.part_o + (slot * 8 + wave) * (DT * 1024) + lane * 4;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<f32x4 *>(dst + (d * RT + r) * 1024 + k * 256) = f32x4{acc[d][r][4 * k], acc[d][r][4 * k + 1], acc[d][r][4 * k + 2], acc[d][r][4 * k + 3]};
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<f32x4 *>(dst + d * 1024 + k * 256) = f32x4{acc[d][4 * k], acc[d][4 * k + 1], acc[d][4 * k + 2], acc[d][4 * k + 3]};
         if (threadIdx.x < M) {
           p.part_ml[slot * 2 * M + threadIdx.x] = stats[threadIdx.x];
           p.part_ml[slot * 2 * M + M + threadIdx.x] = sum_of(threadIdx.x);
         }
       }
     }
-    if (last_tile) return;
+    if (last_team) return;
     from = 0;
-    if (++tile >= t.tiles) {
-      tile = 0;
+    if (++team >= t.teams) {
+      team = 0;
       do {
         if (++seq >= p.b.num_seqs) return;  // (not while the arrays stay as they are)
-      } while (latent_tiles<M>(p, ragged_seq_uniform(p.b, seq)).tiles == 0);
+      } while (latent_tiles<T>(p, ragged_seq_uniform(p.b, seq)).teams == 0);
     }
   }
 }
 
-// Joins the pieces of a cut tile.  Work-groups (g, x) look at the cut between the shares of g and g + 1: if it is the first one within its
-// tile, the pieces are those of g (its first, if its share begins with the tile, else its second one) and of the work-groups after
-// it, whose first pieces they are.  x = d RT + r: one product tile of each wavefront.
+// Joins the pieces of cut tiles.  Work-group (share * team + place, x) has the tile whose first cut is the end of that share, if there is
+// one; x: the wavefront whose results it joins.  Its four wavefronts go through the pieces in turn, two at a time so that their loads overlap, and meet in LDS.
 template <int L, typename OT, bool KV8, int M>
-__global__ void __launch_bounds__(512) latent_absorbed_join_kernel(const LatentParams p) {
+__global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentParams p) {
   using T = LatentAbsorbed<L, OT, KV8, M>;
-  constexpr int RT = T::RT, DT = T::DT;
+  constexpr int DT = T::DT;
+  __shared__ float pieces[4][DT * 16][64], refs[4][2][64];
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const LatentLine<M> line(p, lane);
-  const int g = blockIdx.x, x = blockIdx.y, r = x % RT, d = x / RT;
-  if (g + 1 >= line.groups) return;
-  const int64_t at = line.cut(g + 1);
-  const LatentPlace place = line.find(p, at, lane);
-  const int64_t start = at - place.off, before = line.cut(g);  // of the tile; of the share of g
-  if (place.off == 0 || before > start) return;  // a cut between two tiles, or not the first one within its tile
-  const LatentTiles t = latent_tiles<M>(p, ragged_seq_uniform(p.b, place.seq));
-  const int steps = (latent_keys<M>(p, t, place.tile) + kLatentKeys - 1) / kLatentKeys;
-  const int64_t cost = t.cost();
+  if ((int)blockIdx.x >= load_uniform_i32(p.shares) * p.team) return;
+  const LatentJoin join = p.joins[blockIdx.x];
+  const int first = __builtin_amdgcn_readfirstlane(join.first), last = __builtin_amdgcn_readfirstlane(join.last);
+  if (first > last) return;
+  const int of_wave = blockIdx.y, slice = of_wave % T::kSlices, row0 = T::kTurns ? (of_wave >> 2) * 32 : 0, first_slot = join.first_slot;
+  const int place = p.team == 1 ? 0 : (int)blockIdx.x % p.team;
   float m = kNoReference, l = 0.f;
-  f32x16 acc;
+  f32x16 acc[DT];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-  int from = 0;
-  for (int h = g;; ++h) {
-    const int64_t share_end = h + 1 < line.groups ? line.cut(h + 1) : line.total;
-    const bool last = share_end >= start + cost;
-    const int until = __builtin_amdgcn_readfirstlane(last ? steps : latent_cut_step(share_end - start, steps));
-    if (from == 0 && until == steps) return;  // one piece has it all: its work-group has stored the rows
-    if (from < until) {
-      const int64_t slot = 2 * (int64_t)h + (h == g && before < start ? 1 : 0);
-      const float *ml = p.part_ml + slot * 2 * M + r * 32 + col;
-      const float *src = p.part_o + ((slot * 8 + wave) * (DT * RT) + x) * 1024 + lane * 4;
-      const float pm = ml[0], to = fmaxf(m, pm), mine = fast_exp2(m - to), its = fast_exp2(pm - to);
-      l = l * mine + ml[M] * its;
-      m = to;
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4 o = *reinterpret_cast<const f32x4 *>(src + k * 256);
+    for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+  struct Piece {
+    float m, l;
+    f32x4 o[DT][4];
+  };
+  auto load = [&](int h) {
+    Piece x;
+    const int64_t slot = h == first ? first_slot : 2 * ((int64_t)h * p.team + place);
+    const float *ml = p.part_ml + slot * 2 * M + row0 + col;
+    const float *src = p.part_o + (slot * 8 + of_wave) * (DT * 1024) + lane * 4;
+    x.m = ml[0], x.l = ml[M];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[4 * k + e] = acc[4 * k + e] * mine + o[e] * its;
-      }
-    }
-    from = until;
-    if (last) break;
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x.o[d][k] = *reinterpret_cast<const f32x4 *>(src + d * 1024 + k * 256);
+    return x;
+  };
+  auto add = [&](const Piece &x) {
+    const float to = fmaxf(m, x.m), mine = fast_exp2(m - to), its = fast_exp2(x.m - to);
+    l = l * mine + x.l * its;
+    m = to;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[d][e] = acc[d][e] * mine + x.o[d][e >> 2][e & 3] * its;
+  };
+  for (int h = first + wave; h <= last; h += 8) {
+    const Piece x = load(h), y = load(min(h + 4, last));
+    add(x);
+    if (h + 4 <= last) add(y);
   }
-  const int row = place.tile * M + r * 32 + col;
+  refs[wave][0][lane] = m, refs[wave][1][lane] = l;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) pieces[wave][d * 16 + e][lane] = acc[d][e];
+  __syncthreads();
+  // wavefront w finishes registers 4 w DT .. of the product tiles: elements d = 8 k + 4 half + e of 32 for one k of each tile
+  float to = refs[0][0][lane], sum = 0.f, f[4];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) to = fmaxf(to, refs[w][0][lane]);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = fast_exp2(refs[w][0][lane] - to);
+    sum += refs[w][1][lane] * f[w];
+  }
+  const LatentTiles t = latent_tiles<T>(p, ragged_seq_uniform(p.b, __builtin_amdgcn_readfirstlane(join.seq)));
+  const int row = join.tile * M + row0 + col;
   if (row >= t.rows) return;
   const int token = row / p.num_heads, head = row - token * p.num_heads;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  char *dst = p.out + (int64_t)(t.q.first + token) * p.out_token_bytes + head * p.out_head_bytes + wave * (L / 4) + d * 64 + half * 8;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  char *dst = p.out + (int64_t)(t.q.first + token) * p.out_token_bytes + head * p.out_head_bytes + slice * (DT * 64) + wave * 16 + half * 8;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    *reinterpret_cast<u32x2 *>(dst + k * 16) =
-        u32x2{pack2<OT>(acc[4 * k] * inv, acc[4 * k + 1] * inv), pack2<OT>(acc[4 * k + 2] * inv, acc[4 * k + 3] * inv)};
+  for (int d = 0; d < DT; ++d) {
+    float o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) o[e] += pieces[w][d * 16 + 4 * wave + e][lane] * f[w];
+      o[e] *= inv;
+    }
+    *reinterpret_cast<u32x2 *>(dst + d * 64) = u32x2{pack2<OT>(o[0], o[1]), pack2<OT>(o[2], o[3])};
+  }
 }
 
 }  // namespace fa
