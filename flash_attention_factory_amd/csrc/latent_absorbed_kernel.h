@@ -47,18 +47,18 @@ struct LatentParams {
   float *part_o;           // pieces: [2 * (share * team + place in the team) + (0: its first, 1: a later one)][registers of its wavefronts]
   float *part_ml;          // [...][2][row]
   LatentJoin *joins;       // [share * team + place in the team]: the tile whose first cut is the end of the share
-  int32_t *shares;         // how many shares there are
 };
 
 // A tile that is cut: its pieces are those of the shares first .. last (none: first > last).
 struct LatentJoin {
-  int32_t seq, tile, first, last, first_slot;  // first_slot: of the first share's piece; of the others 2 * (share * team + place in the team)
+  int32_t first, last, first_slot;  // first_slot: of the first share's piece; of the others 2 * (share * team + place in the team)
+  int32_t first_token, row, rows;   // of the sequence; the tile's first row, the sequence's rows
 };
 
 // Keys of a step, what a tile costs apart from its steps, and the smallest share of the line (both in steps).
-template <bool KV8>
+template <bool KV8, int M>
 struct LatentSteps {
-  static constexpr int kKeys = KV8 ? 64 : 32, kStart = KV8 ? 4 : 6, kLeast = KV8 ? 4 : 8;
+  static constexpr int kKeys = KV8 && M < 128 ? 64 : 32, kStart = KV8 && M < 128 ? 4 : 6, kLeast = KV8 && M < 128 ? 4 : 8;
 };
 constexpr float kNoReference = -1e30f;
 
@@ -87,40 +87,59 @@ __device__ __forceinline__ int latent_keys(const LatentParams &p, const LatentTi
   return max(0, attends_from(t.q, (min((tile + 1) * T::kRows, t.rows) - 1) / p.num_heads) + 1);
 }
 
+// Sum over the lanes below and with this one.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t lanes_moved(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)((uint64_t)v >> 32), CTRL, ROWS, 0xf, false);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t wave_sums64(int64_t v) {
+  v += lanes_moved<0x111, 0xf>(v);  // the lanes 1, 2, 4, 8 below, of 16
+  v += lanes_moved<0x112, 0xf>(v);
+  v += lanes_moved<0x114, 0xf>(v);
+  v += lanes_moved<0x118, 0xf>(v);
+  v += lanes_moved<0x142, 0xa>(v);  // lane 15 of the 16 before, to the second and the fourth 16
+  v += lanes_moved<0x143, 0xc>(v);  // lane 31, to the last 32
+  return v;
+}
+template <typename T>
 struct LatentPlace {
   int seq, team;  // team: which of the sequence's
   int64_t off;    // from its start
+  LatentTiles t;
 };
 template <typename T>
 struct LatentLine {
   int64_t total;
   int groups;
-  int64_t mine, upto;  // of the first 64 sequences: this lane's, and the sum up to it
+  RaggedSeq own;       // of the first 64 sequences: this lane's ...
+  int64_t mine, upto;  // ... its length, and the sum up to it
   __device__ __forceinline__ LatentLine(const LatentParams &p, int lane) {
-    mine = costs(p, lane);
-    upto = wave_inclusive_scan64(mine, lane);
+    own = ragged_seq_of_lane(p.b, min(lane, p.b.num_seqs - 1));
+    mine = lane < p.b.num_seqs ? cost(p, own) : 0;
+    upto = wave_sums64(mine);
     total = readlane64(upto, 63);
     if (p.b.num_seqs > 64) {
       int64_t more = 0;
-      for (int s = 64 + lane; s < p.b.num_seqs; s += 64) more += costs(p, s);
-      total += readlane64(wave_inclusive_scan64(more, lane), 63);
+      for (int s = 64 + lane; s < p.b.num_seqs; s += 64) more += cost(p, ragged_seq_of_lane(p.b, s));
+      total += readlane64(wave_sums64(more), 63);
     }
     groups = (int)min((int64_t)p.groups, total / T::kLeast + (total > 0));
   }
-  static __device__ __forceinline__ int64_t costs(const LatentParams &p, int s) {
-    if (s >= p.b.num_seqs) return 0;
-    const LatentTiles t = latent_tiles<T>(p, ragged_seq_of_lane(p.b, s));
+  static __device__ __forceinline__ int64_t cost(const LatentParams &p, RaggedSeq q) {
+    const LatentTiles t = latent_tiles<T>(p, q);
     return t.teams * t.cost;
   }
   __device__ __forceinline__ int64_t cut(int g) const { return divide(total * g, groups); }
   // `at` < total
-  __device__ __forceinline__ LatentPlace find(const LatentParams &p, int64_t at, int lane) const {
-    LatentPlace r;
+  __device__ __forceinline__ LatentPlace<T> find(const LatentParams &p, int64_t at, int lane) const {
+    LatentPlace<T> r;
     int64_t before = 0, of_lane = mine, sum = upto;
     for (int base = 0;; base += 64) {
       if (base > 0) {
-        of_lane = costs(p, base + lane);
-        sum = wave_inclusive_scan64(of_lane, lane);
+        of_lane = base + lane < p.b.num_seqs ? cost(p, ragged_seq_of_lane(p.b, base + lane)) : 0;
+        sum = wave_sums64(of_lane);
       }
       const unsigned long long beyond = __ballot(before + sum > at);
       if (beyond || base + 64 >= p.b.num_seqs) {
@@ -131,10 +150,15 @@ struct LatentLine {
       }
       before += readlane64(sum, 63);
     }
-    const LatentTiles t = latent_tiles<T>(p, ragged_seq_uniform(p.b, r.seq));
+    if (r.seq < 64) {
+      r.t = latent_tiles<T>(p, RaggedSeq{__builtin_amdgcn_readlane(own.first, r.seq), __builtin_amdgcn_readlane(own.n, r.seq),
+                                         __builtin_amdgcn_readlane(own.ctx, r.seq), __builtin_amdgcn_readlane(own.pos0, r.seq)});
+    } else {
+      r.t = latent_tiles<T>(p, ragged_seq_uniform(p.b, r.seq));
+    }
     const int64_t in = at - before;
-    r.team = __builtin_amdgcn_readfirstlane((int)divide(in, (int)t.cost));
-    r.off = in - r.team * t.cost;
+    r.team = __builtin_amdgcn_readfirstlane((int)divide(in, (int)r.t.cost));
+    r.off = in - r.team * r.t.cost;
     return r;
   }
 };
@@ -145,34 +169,46 @@ __device__ __forceinline__ int latent_cut_step(int64_t off, int steps) {
 }
 
 template <int L, typename OT, bool KV8, int M>
-struct LatentAbsorbed : LatentSteps<KV8> {
-  static constexpr int kRows = M, kKeys = LatentSteps<KV8>::kKeys;
-  static constexpr bool kTurns = M == 64;
+struct LatentAbsorbed : LatentSteps<KV8, M> {
+  static constexpr int kRows = M, kKeys = LatentSteps<KV8, M>::kKeys;
+  static constexpr bool kTurns = M >= 64;
   static constexpr int kRowElements = L + kLatentRope;
   static constexpr int kRowBytes = kRowElements * (KV8 ? 1 : 2);
   static constexpr int kStepBytes = kKeys * kRowBytes;
-  static constexpr int kParts = kTurns ? 2 : kKeys / 16;        // of a step's keys, among wavefronts with the same rows
+  static constexpr int kParts = kTurns ? 128 / M : kKeys / 16;  // of a step's keys, among wavefronts with the same rows
   static constexpr int kTiles = kKeys / 16 / kParts;            // of 16 keys, in a part
-  static constexpr int kOthers = M * kKeys * 2 + (kParts + 1) * M * 4 + 16;  // LDS beside the ring and its scales
+  static constexpr int kOthers = M * kKeys * 2 + (kParts + 1) * M * 4 + M / 4;  // LDS beside the ring and its scales
   static constexpr int kRing = (160 * 1024 - kOthers) / (kStepBytes + kKeys * 4) < 7 ? (160 * 1024 - kOthers) / (kStepBytes + kKeys * 4) : 7;
   static constexpr int kScales = kRing * kStepBytes;            // [ring][key]
   static constexpr int kWeights = kScales + (KV8 ? kRing * kKeys * 4 : 0);  // [row][key] 16-bit
   static constexpr int kTops = kWeights + M * kKeys * 2;        // [part][row]: maxima
   static constexpr int kFactors = kTops + kParts * M * 4;       // [row]: what sums and results are multiplied with
   static constexpr int kFlags = kFactors + M * 4;               // [strip of 16 rows]: whether there are factors
-  static constexpr int kLdsBytes = kFlags + 16;
-  static constexpr int kOwn = kKeys / 8;                        // rows of a step that a wavefront loads
+  static constexpr int kLdsBytes = kFlags + M / 4;
+  static constexpr int kOwn = KV8 ? 16 : 8;                     // rows of a step that a wavefront loads
+  static constexpr int kLoaders = kKeys / kOwn;                 // wavefronts that load, the last ones
   static constexpr int kPieces = kRowBytes / 16;                // of 16 bytes, of a row
-  static constexpr int kLoads = (kOwn * kPieces + 63) / 64;     // instructions for them
+  static constexpr int kLine = 64 / kOwn;                       // pieces of a row that one instruction loads
+  static constexpr int kBefore = kRing / 2;                     // steps that are asked for before the queries
+  static constexpr int kQueryWaves = kTurns ? 8 : 2 * kParts;   // wavefronts with scores
+  static constexpr int kQueryRows = (kRing - kBefore) * kStepBytes >= kQueryWaves * 16 * kRowElements * 2 ? 16 : 8;  // in LDS at a time, of a wavefront
+  static constexpr int kLoads = kPieces / kLine;                // instructions for the rows
   static constexpr int kInFlight = kLoads + KV8;                // ... and for their scales
   static constexpr int kSlices = kTurns ? 4 : 8;                // of the results' elements
+  static constexpr int kResultTiles = M == 128 ? 2 : 1;         // of 32 rows
   static constexpr int DT = L / kSlices / 32, KS = kRowElements / 32;
-  static_assert(kLdsBytes <= 160 * 1024 && kRing >= 4 && (kRing - 3) * kInFlight < 64, "");
+  static_assert((kRing - kBefore) * kStepBytes >= kQueryWaves * kQueryRows * kRowElements * 2, "");
+  static_assert(kLdsBytes <= 160 * 1024 && kRing >= 4 && (kRing - 2) * kInFlight < 64 && kPieces % kLine == 0, "");
 
-  // Which 16-byte piece of a row lies at piece c of its place in LDS (and the other way round).  16 lanes that read one piece of 16
-  // rows, and 32 that read 4 rows of 64 bytes (16-bit pools) or 8 rows of 32 bytes (bytes), meet in no bank.
+  // Where 16-byte piece c of a row lies in a step's place in LDS: kOwn rows together, of each kLine pieces at a time, as the loads leave
+  // them.  Which of the kLine goes by the row: then the 16 lanes of a read of 16 bytes that go together (0 .. 3, 12 .. 15 and 20 .. 27,
+  // and the others) meet in no bank where they read two neighbouring pieces of 16 rows, nor do 32 lanes that read 4 rows of 64 bytes
+  // (16-bit pools) or 8 rows of 32 bytes (bytes).
   static __device__ __forceinline__ int swizzle(int key) {
-    return KV8 ? ((key >> 2) & 1) * 2 + ((key >> 3) & 1) : ((key >> 1) & 1) * 4 + ((key >> 2) & 3);
+    return KV8 ? ((key >> 2) & 1) * 2 + ((key >> 3) & 1) : ((key >> 1) & 1) * 4 + (((key >> 2) ^ (key >> 3)) & 1) * 2 + ((key >> 3) & 1);
+  }
+  static __device__ __forceinline__ int piece_at(int key, int c) {
+    return key / kOwn * kOwn * kRowBytes + c / kLine * 1024 + key % kOwn * kLine * 16 + ((c % kLine) ^ swizzle(key)) * 16;
   }
   // Where 16-byte piece c of a row of weights lies: 16 rows' same piece meets in no bank.
   static __device__ __forceinline__ int weights_at(int row, int c) {
@@ -188,10 +224,23 @@ __device__ __forceinline__ void load_to_lds_16(uint32_t to, uint32_t offset, con
 __device__ __forceinline__ void load_to_lds_4(uint32_t to, uint32_t offset, const char *base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
 }
+__device__ __forceinline__ void load_to_lds_16_from(uint32_t to, uint64_t address) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(address) : "memory");
+}
 // All but the last N loads of this wavefront have landed.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// All but the last `steps` steps (MOST at most) of EACH loads.
+template <int MOST, int EACH>
+__device__ __forceinline__ void wait_steps(int steps) {
+  if constexpr (MOST == 0) {
+    wait_loads<0>();
+  } else {
+    if (steps >= MOST) wait_loads<MOST * EACH>();
+    else wait_steps<MOST - 1, EACH>(steps);
+  }
 }
 __device__ __forceinline__ const char *uniform_address(const char *p) {
   const uint64_t v = (uint64_t)(uintptr_t)p;
@@ -213,7 +262,7 @@ __device__ __forceinline__ u32x4 decoded(u32x2 bytes) {
 template <int L, typename OT, bool KV8, int M>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) latent_absorbed_kernel(const LatentParams p) {
   using T = LatentAbsorbed<L, OT, KV8, M>;
-  constexpr int DT = T::DT, KS = T::KS, KT = T::kTiles;
+  constexpr int DT = T::DT, KS = T::KS, KT = T::kTiles, RT = T::kResultTiles;
   __shared__ __attribute__((aligned(16))) char lds[T::kLdsBytes];
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
 
@@ -222,29 +271,35 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   // this wavefront's rows and keys of the scores, rows and elements of the results
   const int strip = wave / T::kParts, key_part = wave % T::kParts, key0 = key_part * 16 * KT;
   const bool scores_here = T::kTurns || strip * 16 < M;
-  const int result_row0 = T::kTurns ? (wave >> 2) * 32 : 0, slice = wave % T::kSlices;
-  const bool late = T::kTurns && wave >= 4;
+  const int result_row0 = T::kTurns ? (wave >> 2) * (M / 2) : 0, slice = wave % T::kSlices;
+  const bool late = T::kTurns && wave >= 4, loads_here = wave >= 8 - T::kLoaders;
+  const int loader = wave - (8 - T::kLoaders);  // which of those that load
   const int H = p.num_heads;
 
   // ---- this work-group's tiles ----
+  LatentTiles t;
   int seq, team, from = 0, place = 0, part = blockIdx.x, end_seq, end_team, end_cut = 0x7fffffff;  // place: in the team
   if (p.groups > 0) {
     const LatentLine<T> line(p, lane);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.shares = line.groups;
-    const int per = (line.groups + 7) >> 3, in_xcc = (int)blockIdx.x >> 3;  // work-groups go to the eight XCCs in turn: each gets an eighth of the line
-    const int g = ((int)blockIdx.x & 7) * per + in_xcc / p.team;
-    if (in_xcc / p.team >= per || g >= line.groups) return;
+    const int per = (line.groups + 7) >> 3, xcc = (int)blockIdx.x & 7, in_xcc = (int)blockIdx.x >> 3;  // work-groups go to the eight XCCs in turn:
+    const int of_xcc = in_xcc / p.team, g = xcc * per + of_xcc;                                       // each gets an eighth of the line
     place = in_xcc % p.team, part = g * p.team + place;
-    const LatentPlace at = line.find(p, line.cut(g), lane), to = line.find(p, line.cut(g + 1) - 1, lane);
+    if (of_xcc >= per || g >= line.groups) {  // no share: nothing to join at its end
+      const int idle = of_xcc >= per ? 8 * per + (of_xcc - per) * 8 + xcc : g;
+      if (threadIdx.x == 0) p.joins[idle * p.team + place] = LatentJoin{1, 0, 0, 0, 0, 0};
+      return;
+    }
+    const LatentPlace<T> at = line.find(p, line.cut(g), lane), to = line.find(p, line.cut(g + 1) - 1, lane);
     seq = at.seq, team = at.team, end_seq = to.seq, end_team = to.team;
-    const LatentTiles t0 = latent_tiles<T>(p, ragged_seq_uniform(p.b, seq)), t1 = latent_tiles<T>(p, ragged_seq_uniform(p.b, end_seq));
+    const LatentTiles &t1 = to.t;
+    t = at.t;
     const int end_tile = to.team * p.team + place;
     const int end_steps = end_tile < t1.tiles ? (latent_keys<T>(p, t1, end_tile) + T::kKeys - 1) / T::kKeys : 0;
-    from = latent_cut_step<T>(at.off, t0.steps);
+    from = latent_cut_step<T>(at.off, t.steps);
     if (to.off + 1 < t1.cost) end_cut = latent_cut_step<T>(to.off + 1, t1.steps);
     from = __builtin_amdgcn_readfirstlane(from), end_cut = __builtin_amdgcn_readfirstlane(end_cut);
-    if (wave == 7) {  // what the join is told of the cut at this share's end
-      LatentJoin join = {to.seq, end_tile, 1, 0, 0};
+    if (wave == 0) {  // what the join is told of the cut at this share's end
+      LatentJoin join = {1, 0, 0, t1.q.first, end_tile * M, t1.rows};
       const int64_t start = line.cut(g + 1) - 1 - to.off;
       if (to.off + 1 < t1.cost && line.cut(g) <= start && end_steps > 0) {
         int first = g, last = min((int)divide((start + T::kStart + end_steps - 1) * line.groups, line.total) + 1, line.groups - 1);
@@ -259,6 +314,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     seq = end_seq = __builtin_amdgcn_readfirstlane(at.seq);
     if (seq >= p.b.num_seqs) return;
     team = end_team = (int)blockIdx.x - __builtin_amdgcn_readfirstlane(at.before);
+    t = latent_tiles<T>(p, ragged_seq_uniform(p.b, seq));
   }
   auto meet = [&]() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -266,34 +322,24 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   };
 
-  // Bytes from a wavefront's first row of a step to the piece that this lane loads, for each of its loads.
-  uint32_t load_off[T::kLoads];
-#pragma unroll
-  for (int i = 0; i < T::kLoads; ++i) {
-    const int slot = i * 64 + lane, r = min(slot / T::kPieces, T::kOwn - 1), c = slot - slot / T::kPieces * T::kPieces;
-    load_off[i] = (uint32_t)r * p.token_bytes + (c ^ T::swizzle(wave * T::kOwn + r)) * 16;
-  }
-  const bool last_load = (T::kLoads - 1) * 64 + lane < T::kOwn * T::kPieces;
-  // Where this lane reads: a cached row's piece for the scores, its transposed pieces for the results.  The swizzles are exclusive-ors in
-  // the low bits of the pieces' numbers, so that two products or result tiles further on is an offset.
+  // Bytes from a wavefront's first row of a step to the piece that this lane loads first; the next ones are kLine pieces on.
+  const uint32_t load_off = (uint32_t)(lane / T::kLine) * p.token_bytes + ((lane % T::kLine) ^ T::swizzle(lane / T::kLine + loader * T::kOwn)) * 16;
+  // Where this lane reads: a cached row's piece for the scores, its transposed pieces for the results.  Two products or result tiles further on
+  // are the next line.
   int row_at[2], value_at[4];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int key = key0 + i16;
-    row_at[k] = key * T::kRowBytes + (KV8 ? ((2 * k + (quarter >> 1)) ^ T::swizzle(key)) * 16 + (quarter & 1) * 8 : ((4 * k + quarter) ^ T::swizzle(key)) * 16);
-  }
+  for (int k = 0; k < 2; ++k) row_at[k] = KV8 ? T::piece_at(key0 + i16, 2 * k + (quarter >> 1)) + (quarter & 1) * 8 : T::piece_at(key0 + i16, 4 * k + quarter);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int key = 8 * half + (KV8 ? i16 >> 1 : (i16 >> 2) + (k >> 1) * 4);
     const int c = slice * (L / T::kSlices * (KV8 ? 1 : 2) / 16) + (KV8 ? (k & 1) * 2 + ((lane >> 4) & 1) : (k & 1) * 4 + ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1));
-    value_at[k] = key * T::kRowBytes + (c ^ T::swizzle(key)) * 16 + (i16 & 1) * 8;
+    value_at[k] = T::piece_at(key, c) + (i16 & 1) * 8;
   }
   float *tops = reinterpret_cast<float *>(lds + T::kTops), *factors = reinterpret_cast<float *>(lds + T::kFactors);
   int *flags = reinterpret_cast<int *>(lds + T::kFlags);
 
   bool first_piece = true;
   for (;; first_piece = false) {
-    const LatentTiles t = latent_tiles<T>(p, ragged_seq_uniform(p.b, seq));
     const RaggedSeq &q = t.q;
     const bool last_team = seq == end_seq && team == end_team;
     const int tile = team * p.team + place;
@@ -307,52 +353,84 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       const int j = row / H, head = row - j * H, pos = attends_from(q, j);
       const int wave_lo = attends_from(q, min(row0 + strip * 16, t.rows - 1) / H);
 
+      // This lane's row of queries.  It comes by way of LDS, where a wavefront has a place of its own behind the steps that are asked for first:
+      // rows may lie a power of two apart (heads outermost), and then 16 rows' same pieces, as the products take them, come from few
+      // channels; a whole row at a time does not (128 heads of 64 tokens: 10 us less for each tile).
       u32x4 qv[KS];
-      if (scores_here) {
-        const char *ql = p.query_latent + (int64_t)(q.first + j) * p.ql_token_bytes + head * p.ql_head_bytes + quarter * 16;
-        const char *qr = p.query_rope + (int64_t)(q.first + j) * p.qr_token_bytes + head * p.qr_head_bytes + quarter * 16;
+      const char *ql = p.query_latent + (int64_t)(q.first + j) * p.ql_token_bytes + head * p.ql_head_bytes;
+      const char *qr = p.query_rope + (int64_t)(q.first + j) * p.qr_token_bytes + head * p.qr_head_bytes;
+      auto load_queries = [&]() __attribute__((always_inline)) {
+        constexpr int kPer = T::kQueryRows, kOfRow = L / 8, kRows1 = 512 / L;  // pieces of a row; rows to an instruction
+        int lane_here = lane;  // (addresses are computed here, not kept over the steps)
+        asm volatile("" : "+v"(lane_here));
+        const int i16 = lane_here & 15, quarter = lane_here >> 4;
+        const int place_at = T::kBefore * T::kStepBytes + wave * kPer * T::kRowElements * 2;
+        const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane(lds_at) + place_at;
 #pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          qv[c] = c < L / 32 ? *reinterpret_cast<const u32x4 *>(ql + c * 64) : *reinterpret_cast<const u32x4 *>(qr + (c - L / 32) * 64);
+        for (int first = 0; first < 16; first += kPer) {
+#pragma unroll
+          for (int i = 0; i < kPer / kRows1; ++i) {
+            const int r = first + i * kRows1, piece = lane_here % kOfRow;
+            uint64_t at = (uint64_t)readlane64((int64_t)(uintptr_t)ql, r);
+            if (kRows1 == 2 && lane_here >= 32) at = (uint64_t)readlane64((int64_t)(uintptr_t)ql, r + 1);
+            load_to_lds_16_from(to + i * 1024, at + ((piece ^ ((r + lane_here / kOfRow) & 7)) * 16));
+          }
+#pragma unroll
+          for (int i = 0; i < kPer / 8; ++i) {
+            const int r = first + i * 8 + (lane_here >> 3);
+            load_to_lds_16_from(to + kPer * L * 2 + i * 1024, (uint64_t)__shfl((long long)(uintptr_t)qr, r) + (((lane_here & 7) ^ (r & 7)) * 16));
+          }
+          wait_loads<0>();
+          if (i16 / kPer == first / kPer) {
+            const char *from_lds = lds + place_at + i16 % kPer * L * 2, *rope = lds + place_at + kPer * L * 2 + i16 % kPer * 128;
+#pragma unroll
+            for (int c = 0; c < KS; ++c)
+              qv[c] = c < L / 32 ? *reinterpret_cast<const u32x4 *>(from_lds + ((4 * c + quarter) ^ (i16 & 7)) * 16)
+                                 : *reinterpret_cast<const u32x4 *>(rope + ((4 * (c - L / 32) + quarter) ^ (i16 & 7)) * 16);
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next rows go to the same place
+        }
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
 #pragma unroll
           for (int k = 0; k < 4; ++k) qv[c][k] ^= p.query_flip;
-        }
-      }
+      };
       float m = kNoReference, l = 0.f;
-      f32x16 acc[DT];
+      f32x16 acc[RT][DT];
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[r][d][e] = 0.f;
 
-      // ---- loads of a step: a wavefront has an eighth of its rows, which lie in one block ----
+      // ---- loads of a step: a wavefront has a quarter (an eighth) of its rows, which lie in one block ----
       const int32_t *table = p.b.block_tables + (int64_t)seq * p.b.max_blocks_per_seq;
       const int last_col = p.b.max_blocks_per_seq - 1, in_block = (1 << p.b.block_shift) - 1;
-      auto id_of = [&](int n) { return load_uniform_i32(table + min(((from + n) * T::kKeys + wave * T::kOwn) >> p.b.block_shift, last_col)); };
-      int32_t next_id = id_of(0);
+      auto id_of = [&](int n) { return load_uniform_i32(table + min(((from + n) * T::kKeys + loader * T::kOwn) >> p.b.block_shift, last_col)); };
+      int32_t next_id = loads_here ? id_of(0) : 0;
       auto issue = [&](int n, int slot) __attribute__((always_inline)) {
         const uint32_t id = min((uint32_t)__builtin_amdgcn_readfirstlane(next_id), (uint32_t)p.b.max_block_id);
-        const uint32_t r0 = (uint32_t)((from + n) * T::kKeys + wave * T::kOwn) & in_block;
+        const uint32_t r0 = (uint32_t)((from + n) * T::kKeys + loader * T::kOwn) & in_block;
         const char *base = uniform_address(p.cache + ((uint64_t)id * p.block_bytes + (uint64_t)r0 * p.token_bytes));
-        const uint32_t to = lds_at + slot * T::kStepBytes + wave * T::kOwn * T::kRowBytes;
+        const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane(lds_at) + slot * T::kStepBytes + loader * T::kOwn * T::kRowBytes;
 #pragma unroll
-        for (int i = 0; i < T::kLoads; ++i) {
-          if ((i + 1) * 64 <= T::kOwn * T::kPieces || last_load) load_to_lds_16(__builtin_amdgcn_readfirstlane(to + i * 1024), load_off[i], base);
-        }
+        for (int i = 0; i < T::kLoads; ++i) load_to_lds_16(to + i * 1024, load_off, base + i * T::kLine * 16);
         if constexpr (KV8) {
           const char *scales = uniform_address(reinterpret_cast<const char *>(p.scales + (((uint64_t)id << p.b.block_shift) + r0)));
-          if (lane < T::kOwn) load_to_lds_4(__builtin_amdgcn_readfirstlane(lds_at + T::kScales + (slot * T::kKeys + wave * T::kOwn) * 4), lane * 4, scales);
+          if (lane < T::kOwn) load_to_lds_4((uint32_t)__builtin_amdgcn_readfirstlane(lds_at) + T::kScales + (slot * T::kKeys + loader * T::kOwn) * 4, lane * 4, scales);
         }
         next_id = id_of(n + 1);
       };
       // Rows of a step that no row of the tile sees may hold anything: zeros instead.  By the wavefront that has loaded them.
       auto clear_unseen = [&](int n, int slot) {
-        const int k0 = (from + n) * T::kKeys + wave * T::kOwn;
+        const int k0 = (from + n) * T::kKeys + loader * T::kOwn;
+#pragma unroll 1
         for (int r = min(max(keys - k0, 0), T::kOwn); r < T::kOwn; ++r) {
-          char *dst = lds + slot * T::kStepBytes + (wave * T::kOwn + r) * T::kRowBytes;
-          if (lane < T::kPieces) *reinterpret_cast<u32x4 *>(dst + lane * 16) = u32x4{0u, 0u, 0u, 0u};
-          if (64 + lane < T::kPieces) *reinterpret_cast<u32x4 *>(dst + (64 + lane) * 16) = u32x4{0u, 0u, 0u, 0u};
-          if (KV8 && lane == 0) *reinterpret_cast<float *>(lds + T::kScales + (slot * T::kKeys + wave * T::kOwn + r) * 4) = 0.f;
+          char *dst = lds + slot * T::kStepBytes + loader * T::kOwn * T::kRowBytes + r * T::kLine * 16;
+#pragma unroll 1
+          for (int c = lane; c < T::kPieces; c += 64) *reinterpret_cast<u32x4 *>(dst + c / T::kLine * 1024 + c % T::kLine * 16) = u32x4{0u, 0u, 0u, 0u};
+          if (KV8 && lane == 0) *reinterpret_cast<float *>(lds + T::kScales + (slot * T::kKeys + loader * T::kOwn + r) * 4) = 0.f;
         }
       };
 
@@ -365,34 +443,88 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       auto row_operand = [&](const char *rows, int o) {  // product o: k-step o / KT of key tile o % KT
         const int c = o / KT;
         rows += o % KT * 16 * T::kRowBytes;
-        if constexpr (KV8) return *reinterpret_cast<const u32x2 *>(rows + row_at[c & 1] + (c >> 1) * 64);
-        else return *reinterpret_cast<const u32x4 *>(rows + row_at[c & 1] + (c >> 1) * 128);
+        if constexpr (KV8) return *reinterpret_cast<const u32x2 *>(rows + row_at[c & 1] + (c >> 1) * 1024);
+        else return *reinterpret_cast<const u32x4 *>(rows + row_at[c & 1] + (c >> 1) * 1024);
       };
       auto value_operand = [&](const char *rows, int ks, int d) {
         rows += 16 * ks * T::kRowBytes;
         if constexpr (KV8) {
-          return lds_read_transposed_bytes(rows + value_at[d & 1] + (d >> 1) * 64);
+          return lds_read_transposed_bytes(rows + value_at[d & 1] + (d >> 1) * 1024);
         } else {
-          const u32x2 a0 = lds_read_transposed(rows + value_at[d & 1] + (d >> 1) * 128);
-          const u32x2 a1 = lds_read_transposed(rows + value_at[2 + (d & 1)] + (d >> 1) * 128);
+          const u32x2 a0 = lds_read_transposed(rows + value_at[d & 1] + (d >> 1) * 1024);
+          const u32x2 a1 = lds_read_transposed(rows + value_at[2 + (d & 1)] + (d >> 1) * 1024);
           return u32x4{a0[0], a0[1], a1[0], a1[1]};
         }
       };
 
-      // Scores of the step that softmax comes to next, times scale and log2(e): element e of tile kt is key key0 + 16 kt + 4 quarter + e.
+      // Scores of the step that softmax comes to next: element e of tile kt is key key0 + 16 kt + 4 quarter + e.
       f32x4 x[KT], s[KT];  // s: the rows' scales
-      // The matrix phase: scores of step n + 1, then results of step n.  kAhead operands are on their way at any time; the order is held with
+      // ... times scale and log2(e), -inf where a key is not seen, and the largest of each row (in weights: with the rows' scales).
+      auto scaled = [&](int n, int at) __attribute__((always_inline)) {
+        const int t0 = (from + n) * T::kKeys + key0;
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          if constexpr (KV8) s[kt] = *reinterpret_cast<const f32x4 *>(lds + T::kScales + (at * T::kKeys + key0 + 16 * kt + 4 * quarter) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[kt][e] *= KV8 ? p.score_scale_log2 * s[kt][e] : p.score_scale_log2;
+        }
+        if (t0 + 16 * KT - 1 > wave_lo) {
+          const int hi = pos - t0 - 4 * quarter;
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[kt][e] = 16 * kt + e > hi ? -INFINITY : x[kt][e];
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, KV8 ? x[kt][e] + __builtin_amdgcn_logf(s[kt][e]) : x[kt][e]);
+        return rows_max(top);
+      };
+      // The matrix phase: results of step n, then scores of step n + 1.  kAhead operands are on their way at any time; the order is held with
       // scheduling barriers, since left to itself the compiler asks for as many as there are and spills the rest.
       auto matrix_phase = [&](int n, int here, int next, auto with_scores, auto with_results) __attribute__((always_inline)) {
         constexpr bool kScores = decltype(with_scores)::value, kResults = decltype(with_results)::value;
-        constexpr int kAhead = 6, kAll = KS * KT, kSteps = T::kKeys / 16;
+        constexpr int kAhead = M == 128 ? 4 : 6, kAll = KS * KT, kSteps = T::kKeys / 16, kFlagWords = M == 128 ? 4 : 2;
         const char *values = lds + here * T::kStepBytes, *rows = lds + next * T::kStepBytes;
-        u32x2 moved = {0u, 0u};
-        u32x4 b[kSteps];
-        if constexpr (kResults) {
-          moved = *reinterpret_cast<const u32x2 *>(flags + result_row0 / 16);
+        uint32_t moved[kFlagWords] = {};
+        u32x4 b[kSteps][RT];
+        auto weights = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
-          for (int ks = 0; ks < kSteps; ++ks) b[ks] = *reinterpret_cast<const u32x4 *>(lds + T::weights_at(result_row0 + col, 2 * ks + half));
+          for (int r = 0; r < RT; ++r) b[ks][r] = *reinterpret_cast<const u32x4 *>(lds + T::weights_at(result_row0 + r * 32 + col, 2 * ks + half));
+        };
+        if constexpr (kResults) {
+          constexpr int kValues = kSteps * DT, kFirst = M == 128 ? 2 : 4;
+#pragma unroll
+          for (int ks = 0; ks < (M == 128 ? 1 : kSteps); ++ks) weights(ks);
+#pragma unroll
+          for (int k = 0; k < kFlagWords; ++k) moved[k] = flags[result_row0 / 16 + k];
+          Raw v[kFirst];
+#pragma unroll
+          for (int o = 0; o < kFirst && o < kValues; ++o) v[o] = value_operand(values, o / DT, o % DT);
+          uint32_t any = 0u;
+#pragma unroll
+          for (int k = 0; k < kFlagWords; ++k) any |= moved[k];
+          if (__builtin_expect(__builtin_amdgcn_readfirstlane((int)any), 0)) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              const bool is = col < 16 ? moved[2 * r] != 0u : moved[2 * r + 1] != 0u;
+              const float f = is ? factors[result_row0 + r * 32 + col] : 1.f;
+#pragma unroll
+              for (int d = 0; d < DT; ++d) acc[r][d] *= f;
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int o = 0; o < kValues; ++o) {
+            const u32x4 value = operand(v[o % kFirst]);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[r][o % DT] = mfma_32x32x16<OT>(value, b[o / DT][r], acc[r][o % DT]);
+            if (M == 128 && o % DT == DT - 1 && o + 1 < kValues) weights(o / DT + 1);
+            if (o + kFirst < kValues) v[o % kFirst] = value_operand(values, (o + kFirst) / DT, (o + kFirst) % DT);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
         if constexpr (kScores) {
           f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // two, for products that need not wait for each other
@@ -409,54 +541,21 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
           if constexpr (KT == 1) x[0] = sum[0] + sum[1];
           else x[0] = sum[0], x[KT - 1] = sum[1];
         }
-        if constexpr (kResults) {
-          constexpr int kValues = kSteps * DT, kFirst = 4;
-          Raw v[kFirst];
-#pragma unroll
-          for (int o = 0; o < kFirst && o < kValues; ++o) v[o] = value_operand(values, o / DT, o % DT);
-          if (__builtin_expect(__builtin_amdgcn_readfirstlane((int)(moved[0] | moved[1])), 0)) {
-            const bool is = col < 16 ? moved[0] != 0u : moved[1] != 0u;
-            const float f = is ? factors[result_row0 + col] : 1.f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) acc[d] *= f;
-          }
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int o = 0; o < kValues; ++o) {
-            acc[o % DT] = mfma_32x32x16<OT>(operand(v[o % kFirst]), b[o / DT], acc[o % DT]);
-            if (o + kFirst < kValues) v[o % kFirst] = value_operand(values, (o + kFirst) / DT, (o + kFirst) % DT);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
-        if constexpr (kScores) {  // the largest of each row's keys, for the other wavefronts that have keys of it
-          const int t0 = (from + n + 1) * T::kKeys + key0;
-          float top = -INFINITY;
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            if constexpr (KV8) s[kt] = *reinterpret_cast<const f32x4 *>(lds + T::kScales + (next * T::kKeys + key0 + 16 * kt + 4 * quarter) * 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[kt][e] *= KV8 ? p.score_scale_log2 * s[kt][e] : p.score_scale_log2;
-          }
-          if (t0 + 16 * KT - 1 > wave_lo) {
-            const int hi = pos - t0 - 4 * quarter;
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[kt][e] = 16 * kt + e > hi ? -INFINITY : x[kt][e];
-          }
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, KV8 ? x[kt][e] + __builtin_amdgcn_logf(s[kt][e]) : x[kt][e]);
-          top = rows_max(top);
+        if constexpr (kScores && T::kParts > 1) {  // for the other wavefronts that have keys of the row
+          const float top = scaled(n + 1, next);
           if (quarter == 0) tops[key_part * M + my_row] = top;
         }
       };
       // The vector phase: weights of the scores, to LDS.
-      auto softmax = [&]() __attribute__((always_inline)) {
-        float top = tops[my_row];
+      auto softmax = [&](int n, int at) __attribute__((always_inline)) {
+        float top;
+        if constexpr (T::kParts == 1) {
+          top = scaled(n, at);
+        } else {
+          top = tops[my_row];
 #pragma unroll
-        for (int k = 1; k < T::kParts; ++k) top = fmaxf(top, tops[k * M + my_row]);
+          for (int k = 1; k < T::kParts; ++k) top = fmaxf(top, tops[k * M + my_row]);
+        }
         int moved = 0;
         if (__builtin_expect(__any(top - m > kRefresh), 0)) {
           const float to = top - m > kRefresh ? top - kHeadroom : m, alpha = fast_exp2(m - to);
@@ -484,28 +583,35 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (!first_piece) meet();  // LDS of the piece before has been read
       if (steps > 0) {
         constexpr int R = T::kRing;
-        for (int n = 0; n < min(R - 2, steps); ++n) issue(n, n);
-        if (steps > R - 3) wait_loads<(R - 3) * T::kInFlight>();
-        else wait_loads<0>();
-        if (steps == 1) clear_unseen(0, 0);
-        meet();
+        if (loads_here)
+          for (int n = 0; n < min(T::kBefore, steps); ++n) issue(n, n);
+        if (scores_here) load_queries();
+        if (loads_here) {
+          if (!scores_here) wait_steps<T::kBefore - 1, T::kInFlight>(min(T::kBefore, steps) - 1);
+          if (steps == 1) clear_unseen(0, 0);
+        }
+        meet();  // step 0 is there, and the queries' places are free
+        if (loads_here)
+          for (int n = T::kBefore; n < min(R, steps); ++n) issue(n, n);
         if (late) meet();
-        int here = R - 1, next = 0, far = R - 2;  // places in the ring of steps n, n + 1, n + R - 1
-        auto land = [&](int n) __attribute__((always_inline)) {  // step n has landed, those after it are on their way
-          if (n + R - 3 < steps) wait_loads<(R - 3) * T::kInFlight>();
-          else wait_loads<0>();
-          if (n == steps - 1) clear_unseen(n, next + 1 == R ? 0 : next + 1);
+        int here = R - 1, next = 0;  // places in the ring of steps n, n + 1
+        // Step n + 2 has landed, those after it are on their way.  (The late half does this before it asks for step n + R, others after.)
+        auto land = [&](int n) __attribute__((always_inline)) {
+          const int asked = min(max(n + (T::kTurns ? R - 1 : R), R - 1), steps - 1);
+          wait_steps<R - 2, T::kInFlight>(asked - (n + 2));
+          if (n + 2 == steps - 1) clear_unseen(n + 2, next + 1 == R ? 0 : next + 1);
         };
         auto round = [&](int n, auto with_results) __attribute__((always_inline)) {
-          if (n + R - 1 < steps) issue(n + R - 1, far);
           if (scores_here) matrix_phase(n, here, next, std::true_type{}, with_results);
           else matrix_phase(n, here, next, std::false_type{}, with_results);
-          if (late) land(n + 2);
+          if (T::kTurns && loads_here) land(n);
           meet();
-          if (scores_here) softmax();
-          if (!late) land(n + 2);
+          // step n has been read by all
+          if (loads_here && n >= 0 && n + R < steps) issue(n + R, here);
+          if (scores_here) softmax(n + 1, next);
+          if (!T::kTurns && loads_here) land(n);
           meet();
-          here = next, next = next + 1 == R ? 0 : next + 1, far = far + 1 == R ? 0 : far + 1;
+          here = next, next = next + 1 == R ? 0 : next + 1;
         };
         round(-1, std::false_type{});
         for (int n = 0; n < steps - 1; ++n) round(n, std::true_type{});
@@ -514,7 +620,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         meet();
       }
 
-      // ---- results: element e of acc[d] is element slice L / slices + 32 d + 8 (e / 4) + 4 half + e % 4 of row result_row0 + col ----
+      // ---- results: element e of acc[r][d] is element slice L / slices + 32 d + 8 (e / 4) + 4 half + e % 4 of row result_row0 + 32 r + col ----
       float *stats = reinterpret_cast<float *>(lds + T::kWeights);  // references [M], then sums [M] of each part of the keys
       if (scores_here) {
         l = rows_sum(l);
@@ -531,26 +637,31 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         return sum;
       };
       if (whole) {
-        const int out_row = row0 + result_row0 + col, stored = min(out_row, t.rows - 1), token = stored / H;
-        const float sum = sum_of(result_row0 + col), inv = sum == 0.f ? 0.f : 1.0f / sum;
-        char *dst = p.out + (int64_t)(q.first + token) * p.out_token_bytes + (stored - token * H) * p.out_head_bytes + slice * (DT * 64) + half * 8;
-        if (out_row < t.rows) {
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
+        for (int r = 0; r < RT; ++r) {
+          const int of_tile = result_row0 + r * 32 + col, out_row = row0 + of_tile, stored = min(out_row, t.rows - 1), token = stored / H;
+          const float sum = sum_of(of_tile), inv = sum == 0.f ? 0.f : 1.0f / sum;
+          char *dst = p.out + (int64_t)(q.first + token) * p.out_token_bytes + (stored - token * H) * p.out_head_bytes + slice * (DT * 64) + half * 8;
+          if (out_row < t.rows) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<u32x2 *>(dst + d * 64 + k * 16) =
-                  u32x2{pack2<OT>(acc[d][4 * k] * inv, acc[d][4 * k + 1] * inv), pack2<OT>(acc[d][4 * k + 2] * inv, acc[d][4 * k + 3] * inv)};
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<u32x2 *>(dst + d * 64 + k * 16) = u32x2{pack2<OT>(acc[r][d][4 * k] * inv, acc[r][d][4 * k + 1] * inv),
+                                                                          pack2<OT>(acc[r][d][4 * k + 2] * inv, acc[r][d][4 * k + 3] * inv)};
+          }
         }
       } else {
         // a piece: as it lies in the registers, 1 KiB at a time
         const int64_t slot = 2 * (int64_t)part + (first_piece ? 0 : 1);
-        float *dst = p.part_o + (slot * 8 + wave) * (DT * 1024) + lane * 4;
+        float *dst = p.part_o + (slot * 8 + wave) * (RT * DT * 1024) + lane * 4;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<f32x4 *>(dst + d * 1024 + k * 256) = f32x4{acc[d][4 * k], acc[d][4 * k + 1], acc[d][4 * k + 2], acc[d][4 * k + 3]};
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<f32x4 *>(dst + (r * DT + d) * 1024 + k * 256) = f32x4{acc[r][d][4 * k], acc[r][d][4 * k + 1], acc[r][d][4 * k + 2], acc[r][d][4 * k + 3]};
         if (threadIdx.x < M) {
           p.part_ml[slot * 2 * M + threadIdx.x] = stats[threadIdx.x];
           p.part_ml[slot * 2 * M + M + threadIdx.x] = sum_of(threadIdx.x);
@@ -563,46 +674,63 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       team = 0;
       do {
         if (++seq >= p.b.num_seqs) return;  // (not while the arrays stay as they are)
-      } while (latent_tiles<T>(p, ragged_seq_uniform(p.b, seq)).teams == 0);
+        t = latent_tiles<T>(p, ragged_seq_uniform(p.b, seq));
+      } while (t.teams == 0);
     }
   }
 }
 
-// Joins the pieces of cut tiles.  Work-group (share * team + place, x) has the tile whose first cut is the end of that share, if there is
-// one; x: the wavefront whose results it joins.  Its four wavefronts go through the pieces in turn, two at a time so that their loads overlap, and meet in LDS.
+// Joins the pieces of cut tiles.  Work-group (x, y) has the x-th tile that is cut, if there are as many, and of it a product tile (32 rows, 32
+// elements) of one wavefront.  Its four wavefronts go through the pieces in turn, four at a time so that their loads overlap, and meet in
+// LDS.
 template <int L, typename OT, bool KV8, int M>
 __global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentParams p) {
   using T = LatentAbsorbed<L, OT, KV8, M>;
-  constexpr int DT = T::DT;
-  __shared__ float pieces[4][DT * 16][64], refs[4][2][64];
+  constexpr int DT = T::DT, kTiles = DT * T::kResultTiles;
+  __shared__ float pieces[4][16][64], refs[4][2][64];
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if ((int)blockIdx.x >= load_uniform_i32(p.shares) * p.team) return;
-  const LatentJoin join = p.joins[blockIdx.x];
-  const int first = __builtin_amdgcn_readfirstlane(join.first), last = __builtin_amdgcn_readfirstlane(join.last);
-  if (first > last) return;
-  const int of_wave = blockIdx.y, slice = of_wave % T::kSlices, row0 = T::kTurns ? (of_wave >> 2) * 32 : 0, first_slot = join.first_slot;
-  const int place = p.team == 1 ? 0 : (int)blockIdx.x % p.team;
+  LatentJoin join = {1, 0, 0, 0, 0, 0};
+  int found = -1;
+  for (int base = 0, before = 0, all = p.groups * p.team; base < all && found < 0; base += 256) {
+    LatentJoin its[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) its[k] = p.joins[min(base + k * 64 + lane, all - 1)];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool cut = base + k * 64 + lane < all && its[k].first <= its[k].last;
+      const unsigned long long cuts = __ballot(cut), below = cuts & ((1ull << lane) - 1);
+      const unsigned long long here = __ballot(cut && before + __popcll(below) == (int)blockIdx.x);
+      if (found < 0 && here) {
+        const int from = __builtin_ctzll(here);
+        found = __builtin_amdgcn_readfirstlane(base + k * 64 + from);
+        join = {__builtin_amdgcn_readlane(its[k].first, from),       __builtin_amdgcn_readlane(its[k].last, from),
+                __builtin_amdgcn_readlane(its[k].first_slot, from),  __builtin_amdgcn_readlane(its[k].first_token, from),
+                __builtin_amdgcn_readlane(its[k].row, from),         __builtin_amdgcn_readlane(its[k].rows, from)};
+      }
+      before += __popcll(cuts);
+    }
+  }
+  if (found < 0) return;
+  const int first = join.first, last = join.last, place = found % p.team;
+  const int of_wave = blockIdx.y / kTiles, slice = of_wave % T::kSlices, d = blockIdx.y % DT;
+  const int row0 = (T::kTurns ? (of_wave >> 2) * (M / 2) : 0) + blockIdx.y % kTiles / DT * 32;
   float m = kNoReference, l = 0.f;
-  f32x16 acc[DT];
+  f32x16 acc;
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
   struct Piece {
     float m, l;
-    f32x4 o[DT][4];
+    f32x4 o[4];
   };
   auto load = [&](int h) {
     Piece x;
-    const int64_t slot = h == first ? first_slot : 2 * ((int64_t)h * p.team + place);
+    const int64_t slot = h == first ? join.first_slot : 2 * ((int64_t)h * p.team + place);
     const float *ml = p.part_ml + slot * 2 * M + row0 + col;
-    const float *src = p.part_o + (slot * 8 + of_wave) * (DT * 1024) + lane * 4;
+    const float *src = p.part_o + (slot * 8 * kTiles + blockIdx.y) * 1024 + lane * 4;
     x.m = ml[0], x.l = ml[M];
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x.o[d][k] = *reinterpret_cast<const f32x4 *>(src + d * 1024 + k * 256);
+    for (int k = 0; k < 4; ++k) x.o[k] = *reinterpret_cast<const f32x4 *>(src + k * 256);
     return x;
   };
   auto add = [&](const Piece &x) {
@@ -610,22 +738,21 @@ __global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentP
     l = l * mine + x.l * its;
     m = to;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[d][e] = acc[d][e] * mine + x.o[d][e >> 2][e & 3] * its;
+    for (int e = 0; e < 16; ++e) acc[e] = acc[e] * mine + x.o[e >> 2][e & 3] * its;
   };
-  for (int h = first + wave; h <= last; h += 8) {
-    const Piece x = load(h), y = load(min(h + 4, last));
-    add(x);
-    if (h + 4 <= last) add(y);
+  for (int h = first + wave; h <= last; h += 16) {
+    Piece x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = load(min(h + 4 * k, last));
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (h + 4 * k <= last) add(x[k]);
   }
   refs[wave][0][lane] = m, refs[wave][1][lane] = l;
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) pieces[wave][d * 16 + e][lane] = acc[d][e];
+  for (int e = 0; e < 16; ++e) pieces[wave][e][lane] = acc[e];
   __syncthreads();
-  // wavefront w finishes registers 4 w DT .. of the product tiles: elements d = 8 k + 4 half + e of 32 for one k of each tile
+  // wavefront w finishes elements 8 w + 4 half + 0 .. 3
   float to = refs[0][0][lane], sum = 0.f, f[4];
 #pragma unroll
   for (int w = 1; w < 4; ++w) to = fmaxf(to, refs[w][0][lane]);
@@ -634,24 +761,20 @@ __global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentP
     f[w] = fast_exp2(refs[w][0][lane] - to);
     sum += refs[w][1][lane] * f[w];
   }
-  const LatentTiles t = latent_tiles<T>(p, ragged_seq_uniform(p.b, __builtin_amdgcn_readfirstlane(join.seq)));
-  const int row = join.tile * M + row0 + col;
-  if (row >= t.rows) return;
+  const int row = join.row + row0 + col;
+  if (row >= join.rows) return;
   const int token = row / p.num_heads, head = row - token * p.num_heads;
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  char *dst = p.out + (int64_t)(t.q.first + token) * p.out_token_bytes + head * p.out_head_bytes + slice * (DT * 64) + wave * 16 + half * 8;
+  char *dst = p.out + (int64_t)(join.first_token + token) * p.out_token_bytes + head * p.out_head_bytes + slice * (DT * 64) + d * 64 + wave * 16 + half * 8;
+  float o[4];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) {
-    float o[4];
+  for (int e = 0; e < 4; ++e) {
+    o[e] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o[e] = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) o[e] += pieces[w][d * 16 + 4 * wave + e][lane] * f[w];
-      o[e] *= inv;
-    }
-    *reinterpret_cast<u32x2 *>(dst + d * 64) = u32x2{pack2<OT>(o[0], o[1]), pack2<OT>(o[2], o[3])};
+    for (int w = 0; w < 4; ++w) o[e] += pieces[w][4 * wave + e][lane] * f[w];
+    o[e] *= inv;
   }
+  *reinterpret_cast<u32x2 *>(dst) = u32x2{pack2<OT>(o[0], o[1]), pack2<OT>(o[2], o[3])};
 }
 
 }  // namespace fa

@@ -183,11 +183,11 @@ inline fa_status launch_latent_cache_gather(void *out, const void *cache, const 
 // ---- absorbed attention ----
 
 struct LatentPlan {
-  int rows;             // M, of a tile: 32 or 64
+  int rows;             // M, of a tile: 32, 64 or 128
   int64_t tile_bound;   // tiles, at most
   int team;             // tiles side by side on the line
   int groups;           // shares of the line, for `team` work-groups each; 0: a work-group for each tile
-  int64_t part_o, part_ml, joins, shares, bytes;
+  int64_t part_o, part_ml, joins, bytes;
 };
 
 inline fa_status check_latent_attention_shape(const fa_latent_attention_shape *s) {
@@ -199,7 +199,7 @@ inline fa_status check_latent_attention_shape(const fa_latent_attention_shape *s
   if (!is_16bit_dtype(s->q_dtype)) return fail(FA_ERR_UNSUPPORTED_DTYPE, "q_dtype %d is neither fp16 (0) nor bf16 (1)", s->q_dtype);
   if (((int64_t)s->num_tokens + s->num_seqs) * s->num_heads > 0x3fffffffLL) return fail(FA_ERR_BAD_SHAPE, "num_tokens x num_heads is too large");
   // the line of tiles is as long as the sum of their steps, and cut at products with the work-groups' numbers
-  const int64_t steps = (int64_t)s->max_blocks_per_seq * s->block_size / LatentSteps<false>::kKeys + 8;
+  const int64_t steps = (int64_t)s->max_blocks_per_seq * s->block_size / LatentSteps<false, 32>::kKeys + 8;
   if (((int64_t)s->num_tokens * s->num_heads / 32 + s->num_seqs) * steps > (1LL << 41))
     return fail(FA_ERR_BAD_SHAPE, "num_tokens x num_heads x keys is too large");
   return FA_OK;
@@ -212,7 +212,7 @@ inline LatentPlan latent_plan(const fa_latent_attention_shape &s, int cus) {
   if (T == 0 || S == 0) return r;
   const int64_t most = std::min<int64_t>(s.max_query_len, T), table = (int64_t)s.max_blocks_per_seq * s.block_size;
   const int64_t keys = s.max_context_len > 0 ? std::min<int64_t>(s.max_context_len, table) : table;
-  r.rows = most * H <= 32 ? 32 : 64;
+  r.rows = most * H <= 32 ? 32 : most * H <= 64 ? 64 : 128;
   const int64_t each = (most * H + r.rows - 1) / r.rows;
   r.tile_bound = std::min(S * each, T * H / r.rows + S);
   if (keys > 256) {
@@ -228,7 +228,6 @@ inline LatentPlan latent_plan(const fa_latent_attention_shape &s, int cus) {
     r.part_o = take(2 * (int64_t)r.groups * r.team * r.rows * s.latent_dim * 4);
     r.part_ml = take(2 * (int64_t)r.groups * r.team * 2 * r.rows * 4);
     r.joins = take((int64_t)r.groups * r.team * sizeof(LatentJoin));
-    r.shares = take(4);
     r.bytes = at;
   }
   return r;
@@ -240,7 +239,9 @@ inline fa_status launch_latent_tiles(const LatentParams &p, const LatentPlan &pl
   FA_HIP_CHECK(timer.launch(latent_absorbed_kernel<L, OT, KV8, M>, grid, dim3(512), 0, p));
   if (us) FA_HIP_CHECK(timer.accumulate(0, us));
   if (plan.groups > 0) {
-    FA_HIP_CHECK(timer.launch(latent_absorbed_join_kernel<L, OT, KV8, M>, dim3((unsigned)(plan.groups * plan.team), 8), dim3(256), 0, p));
+    // tiles that are cut: no more than there are, and than the shares' ends
+    const int64_t cut = std::min<int64_t>(plan.tile_bound, (int64_t)(plan.groups - 1) * plan.team);
+    FA_HIP_CHECK(timer.launch(latent_absorbed_join_kernel<L, OT, KV8, M>, dim3((unsigned)cut, M * L / 1024), dim3(256), 0, p));
     if (us) FA_HIP_CHECK(timer.accumulate(0, us));
   }
   return FA_OK;
@@ -300,14 +301,15 @@ inline fa_status launch_latent_attention(void *out, const void *query_latent, co
   p.part_o = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + plan.part_o);
   p.part_ml = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + plan.part_ml);
   p.joins = reinterpret_cast<LatentJoin *>(reinterpret_cast<char *>(workspace) + plan.joins);
-  p.shares = reinterpret_cast<int32_t *>(reinterpret_cast<char *>(workspace) + plan.shares);
   float *us = o ? o->elapsed_us : nullptr;
   KernelTimer timer(us != nullptr, o ? reinterpret_cast<hipStream_t>(o->stream) : nullptr);
   const auto of_rows = [&](auto dim, auto type, auto bytes) {
     constexpr int kDim = decltype(dim)::value;
     constexpr bool kBytes = decltype(bytes)::value;
     using Type = decltype(type);
-    return plan.rows == 32 ? launch_latent_tiles<kDim, Type, kBytes, 32>(p, plan, timer, us) : launch_latent_tiles<kDim, Type, kBytes, 64>(p, plan, timer, us);
+    return plan.rows == 32   ? launch_latent_tiles<kDim, Type, kBytes, 32>(p, plan, timer, us)
+           : plan.rows == 64 ? launch_latent_tiles<kDim, Type, kBytes, 64>(p, plan, timer, us)
+                             : launch_latent_tiles<kDim, Type, kBytes, 128>(p, plan, timer, us);
   };
   const auto of_dim = [&](auto type, auto bytes) {
     return s->latent_dim == 512 ? of_rows(std::integral_constant<int, 512>{}, type, bytes) : of_rows(std::integral_constant<int, 256>{}, type, bytes);
