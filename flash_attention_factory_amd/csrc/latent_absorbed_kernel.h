@@ -58,7 +58,7 @@ struct LatentJoin {
 // Keys of a step, what a tile costs apart from its steps, and the smallest share of the line (both in steps).
 template <bool KV8, int M>
 struct LatentSteps {
-  static constexpr int kKeys = KV8 && M < 128 ? 64 : 32, kStart = KV8 && M < 128 ? 4 : 6, kLeast = KV8 && M < 128 ? 4 : 8;
+  static constexpr int kKeys = KV8 && M == 32 ? 64 : 32, kStart = M == 128 ? 12 : KV8 && M == 32 ? 4 : 6, kLeast = KV8 && M == 32 ? 2 : 4;
 };
 constexpr float kNoReference = -1e30f;
 
@@ -172,40 +172,46 @@ template <int L, typename OT, bool KV8, int M>
 struct LatentAbsorbed : LatentSteps<KV8, M> {
   static constexpr int kRows = M, kKeys = LatentSteps<KV8, M>::kKeys;
   static constexpr bool kTurns = M >= 64;
+  static constexpr bool kDecodes = KV8 && kTurns;               // rows of bytes are decoded once, into the ring
+  static constexpr bool kBytes = KV8 && !kDecodes;              // ... or lie there as they are
   static constexpr int kRowElements = L + kLatentRope;
-  static constexpr int kRowBytes = kRowElements * (KV8 ? 1 : 2);
+  static constexpr int kRowBytes = kRowElements * (kBytes ? 1 : 2);
   static constexpr int kStepBytes = kKeys * kRowBytes;
   static constexpr int kParts = kTurns ? 128 / M : kKeys / 16;  // of a step's keys, among wavefronts with the same rows
   static constexpr int kTiles = kKeys / 16 / kParts;            // of 16 keys, in a part
-  static constexpr int kOthers = M * kKeys * 2 + (kParts + 1) * M * 4 + M / 4;  // LDS beside the ring and its scales
-  static constexpr int kRing = (160 * 1024 - kOthers) / (kStepBytes + kKeys * 4) < 7 ? (160 * 1024 - kOthers) / (kStepBytes + kKeys * 4) : 7;
-  static constexpr int kScales = kRing * kStepBytes;            // [ring][key]
-  static constexpr int kWeights = kScales + (KV8 ? kRing * kKeys * 4 : 0);  // [row][key] 16-bit
+  static constexpr int kOwn = kBytes ? 16 : 8;                  // rows of a step that a wavefront loads
+  static constexpr int kLoaders = kKeys / kOwn;                 // wavefronts that load, the last ones
+  static constexpr int kPieces = kRowBytes / 16;                // of 16 bytes, of a row
+  static constexpr int kLine = 64 / kOwn;                       // pieces of a row that one instruction loads
+  static constexpr int kLoads = kDecodes ? (kRowElements + 127) / 128 : kPieces / kLine;  // instructions for the rows
+  static constexpr int kInFlight = kLoads + KV8;                // ... and for their scales
+  static constexpr int kRawStep = kDecodes ? kLoaders * kLoads * 1024 : 0;  // bytes of a step before they are decoded; two steps
+  static constexpr int kOthers = 2 * kRawStep + M * kKeys * 2 + (kParts + 1) * M * 4 + M / 4 + (kDecodes ? 8 * kKeys * 4 : 0);  // LDS beside the ring
+  static constexpr int kSlot = kStepBytes + (kBytes ? kKeys * 4 : 0);
+  static constexpr int kRing = kDecodes ? 3 : (160 * 1024 - kOthers) / kSlot < 7 ? (160 * 1024 - kOthers) / kSlot : 7;
+  static constexpr int kScaleSlots = kDecodes ? 8 : KV8 ? kRing : 0;
+  static constexpr int kScales = kRing * kStepBytes;            // [slot][key]
+  static constexpr int kRaw = kScales + kScaleSlots * kKeys * 4;
+  static constexpr int kWeights = kRaw + 2 * kRawStep;          // [row][key] 16-bit
   static constexpr int kTops = kWeights + M * kKeys * 2;        // [part][row]: maxima
   static constexpr int kFactors = kTops + kParts * M * 4;       // [row]: what sums and results are multiplied with
   static constexpr int kFlags = kFactors + M * 4;               // [strip of 16 rows]: whether there are factors
   static constexpr int kLdsBytes = kFlags + M / 4;
-  static constexpr int kOwn = KV8 ? 16 : 8;                     // rows of a step that a wavefront loads
-  static constexpr int kLoaders = kKeys / kOwn;                 // wavefronts that load, the last ones
-  static constexpr int kPieces = kRowBytes / 16;                // of 16 bytes, of a row
-  static constexpr int kLine = 64 / kOwn;                       // pieces of a row that one instruction loads
-  static constexpr int kBefore = kRing / 2;                     // steps that are asked for before the queries
+  static constexpr int kBefore = kRing / 2;                     // steps in the ring before the queries' place
   static constexpr int kQueryWaves = kTurns ? 8 : 2 * kParts;   // wavefronts with scores
   static constexpr int kQueryRows = (kRing - kBefore) * kStepBytes >= kQueryWaves * 16 * kRowElements * 2 ? 16 : 8;  // in LDS at a time, of a wavefront
-  static constexpr int kLoads = kPieces / kLine;                // instructions for the rows
-  static constexpr int kInFlight = kLoads + KV8;                // ... and for their scales
   static constexpr int kSlices = kTurns ? 4 : 8;                // of the results' elements
   static constexpr int kResultTiles = M == 128 ? 2 : 1;         // of 32 rows
   static constexpr int DT = L / kSlices / 32, KS = kRowElements / 32;
   static_assert((kRing - kBefore) * kStepBytes >= kQueryWaves * kQueryRows * kRowElements * 2, "");
-  static_assert(kLdsBytes <= 160 * 1024 && kRing >= 4 && (kRing - 2) * kInFlight < 64 && kPieces % kLine == 0, "");
+  static_assert(kLdsBytes <= 160 * 1024 && kRing >= (kDecodes ? 3 : 4) && (kRing - 1) * kInFlight < 64 && kPieces % kLine == 0, "");
 
   // Where 16-byte piece c of a row lies in a step's place in LDS: kOwn rows together, of each kLine pieces at a time, as the loads leave
   // them.  Which of the kLine goes by the row: then the 16 lanes of a read of 16 bytes that go together (0 .. 3, 12 .. 15 and 20 .. 27,
   // and the others) meet in no bank where they read two neighbouring pieces of 16 rows, nor do 32 lanes that read 4 rows of 64 bytes
   // (16-bit pools) or 8 rows of 32 bytes (bytes).
   static __device__ __forceinline__ int swizzle(int key) {
-    return KV8 ? ((key >> 2) & 1) * 2 + ((key >> 3) & 1) : ((key >> 1) & 1) * 4 + (((key >> 2) ^ (key >> 3)) & 1) * 2 + ((key >> 3) & 1);
+    return kBytes ? ((key >> 2) & 1) * 2 + ((key >> 3) & 1) : ((key >> 1) & 1) * 4 + (((key >> 2) ^ (key >> 3)) & 1) * 2 + ((key >> 3) & 1);
   }
   static __device__ __forceinline__ int piece_at(int key, int c) {
     return key / kOwn * kOwn * kRowBytes + c / kLine * 1024 + key % kOwn * kLine * 16 + ((c % kLine) ^ swizzle(key)) * 16;
@@ -323,16 +329,18 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   };
 
   // Bytes from a wavefront's first row of a step to the piece that this lane loads first; the next ones are kLine pieces on.
-  const uint32_t load_off = (uint32_t)(lane / T::kLine) * p.token_bytes + ((lane % T::kLine) ^ T::swizzle(lane / T::kLine + loader * T::kOwn)) * 16;
+  // (Rows that are decoded: eight neighbouring pieces of bytes, then the last four, as the lanes come.)
+  const uint32_t load_off = T::kDecodes ? (uint32_t)(lane >> 3) * p.token_bytes + (lane & 7) * 16
+                                        : (uint32_t)(lane / T::kLine) * p.token_bytes + ((lane % T::kLine) ^ T::swizzle(lane / T::kLine + loader * T::kOwn)) * 16;
   // Where this lane reads: a cached row's piece for the scores, its transposed pieces for the results.  Two products or result tiles further on
   // are the next line.
   int row_at[2], value_at[4];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) row_at[k] = KV8 ? T::piece_at(key0 + i16, 2 * k + (quarter >> 1)) + (quarter & 1) * 8 : T::piece_at(key0 + i16, 4 * k + quarter);
+  for (int k = 0; k < 2; ++k) row_at[k] = T::kBytes ? T::piece_at(key0 + i16, 2 * k + (quarter >> 1)) + (quarter & 1) * 8 : T::piece_at(key0 + i16, 4 * k + quarter);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const int key = 8 * half + (KV8 ? i16 >> 1 : (i16 >> 2) + (k >> 1) * 4);
-    const int c = slice * (L / T::kSlices * (KV8 ? 1 : 2) / 16) + (KV8 ? (k & 1) * 2 + ((lane >> 4) & 1) : (k & 1) * 4 + ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1));
+    const int key = 8 * half + (T::kBytes ? i16 >> 1 : (i16 >> 2) + (k >> 1) * 4);
+    const int c = slice * (L / T::kSlices * (T::kBytes ? 1 : 2) / 16) + (T::kBytes ? (k & 1) * 2 + ((lane >> 4) & 1) : (k & 1) * 4 + ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1));
     value_at[k] = T::piece_at(key, c) + (i16 & 1) * 8;
   }
   float *tops = reinterpret_cast<float *>(lds + T::kTops), *factors = reinterpret_cast<float *>(lds + T::kFactors);
@@ -413,12 +421,22 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         const uint32_t id = min((uint32_t)__builtin_amdgcn_readfirstlane(next_id), (uint32_t)p.b.max_block_id);
         const uint32_t r0 = (uint32_t)((from + n) * T::kKeys + loader * T::kOwn) & in_block;
         const char *base = uniform_address(p.cache + ((uint64_t)id * p.block_bytes + (uint64_t)r0 * p.token_bytes));
-        const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane(lds_at) + slot * T::kStepBytes + loader * T::kOwn * T::kRowBytes;
+        const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane(lds_at);
+        if constexpr (T::kDecodes) {
+          const uint32_t to = lds0 + T::kRaw + (n & 1) * T::kRawStep + loader * T::kLoads * 1024;
 #pragma unroll
-        for (int i = 0; i < T::kLoads; ++i) load_to_lds_16(to + i * 1024, load_off, base + i * T::kLine * 16);
+          for (int i = 0; i < T::kLoads - 1; ++i) load_to_lds_16(to + i * 1024, load_off, base + i * 128);
+          int last = lane;  // (computed here, not kept over the steps)
+          asm volatile("" : "+v"(last));
+          if (last < 32) load_to_lds_16(to + (T::kLoads - 1) * 1024, (uint32_t)(last >> 2) * p.token_bytes + (last & 3) * 16, base + (T::kLoads - 1) * 128);
+        } else {
+          const uint32_t to = lds0 + slot * T::kStepBytes + loader * T::kOwn * T::kRowBytes;
+#pragma unroll
+          for (int i = 0; i < T::kLoads; ++i) load_to_lds_16(to + i * 1024, load_off, base + i * T::kLine * 16);
+        }
         if constexpr (KV8) {
           const char *scales = uniform_address(reinterpret_cast<const char *>(p.scales + (((uint64_t)id << p.b.block_shift) + r0)));
-          if (lane < T::kOwn) load_to_lds_4((uint32_t)__builtin_amdgcn_readfirstlane(lds_at) + T::kScales + (slot * T::kKeys + loader * T::kOwn) * 4, lane * 4, scales);
+          if (lane < T::kOwn) load_to_lds_4(lds0 + T::kScales + ((T::kDecodes ? n & 7 : slot) * T::kKeys + loader * T::kOwn) * 4, lane * 4, scales);
         }
         next_id = id_of(n + 1);
       };
@@ -430,25 +448,49 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
           char *dst = lds + slot * T::kStepBytes + loader * T::kOwn * T::kRowBytes + r * T::kLine * 16;
 #pragma unroll 1
           for (int c = lane; c < T::kPieces; c += 64) *reinterpret_cast<u32x4 *>(dst + c / T::kLine * 1024 + c % T::kLine * 16) = u32x4{0u, 0u, 0u, 0u};
-          if (KV8 && lane == 0) *reinterpret_cast<float *>(lds + T::kScales + (slot * T::kKeys + loader * T::kOwn + r) * 4) = 0.f;
+          if (KV8 && lane == 0) *reinterpret_cast<float *>(lds + T::kScales + ((T::kDecodes ? n & 7 : slot) * T::kKeys + loader * T::kOwn + r) * 4) = 0.f;
         }
       };
 
+      // Rows of bytes of step n, which have landed, to their place in the ring; the step after next takes theirs.
+      auto decode = [&](int n, int slot) __attribute__((always_inline)) {
+        wait_steps<1, T::kInFlight>(min(steps - 1 - n, 1));
+        int lane_here = lane;
+        asm volatile("" : "+v"(lane_here));
+        const char *src = lds + T::kRaw + (n & 1) * T::kRawStep + loader * T::kLoads * 1024 + lane_here * 16;
+        char *dst = lds + slot * T::kStepBytes;
+        const int key = loader * 8 + (lane_here >> 3), last_key = loader * 8 + ((lane_here >> 2) & 7);
+        const int at = T::piece_at(key, 2 * (lane_here & 7)), last_at = T::piece_at(last_key, 2 * (lane_here & 3));
+        u32x4 bytes[2] = {*reinterpret_cast<const u32x4 *>(src), *reinterpret_cast<const u32x4 *>(src + 1024)};
+#pragma unroll
+        for (int i = 0; i < T::kLoads; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          const int to = (i < T::kLoads - 1 ? at : last_at) + i * 2048;
+          if (i < T::kLoads - 1 || lane_here < 32) {
+            *reinterpret_cast<u32x4 *>(dst + to) = decoded<OT>(u32x2{bytes[i & 1][0], bytes[i & 1][1]});
+            *reinterpret_cast<u32x4 *>(dst + (to ^ 16)) = decoded<OT>(u32x2{bytes[i & 1][2], bytes[i & 1][3]});
+          }
+          if (i + 2 < T::kLoads) bytes[i & 1] = *reinterpret_cast<const u32x4 *>(src + (i + 2) * 1024);
+        }
+        if (n == steps - 1) clear_unseen(n, slot);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (n + 2 < steps) issue(n + 2, 0);
+      };
       // Operands as LDS has them: 16-bit values, or bytes that are decoded before the product.
-      using Raw = typename std::conditional<KV8, u32x2, u32x4>::type;
+      using Raw = typename std::conditional<T::kBytes, u32x2, u32x4>::type;
       auto operand = [&](Raw a) {
-        if constexpr (KV8) return decoded<OT>(a);
+        if constexpr (T::kBytes) return decoded<OT>(a);
         else return a;
       };
       auto row_operand = [&](const char *rows, int o) {  // product o: k-step o / KT of key tile o % KT
         const int c = o / KT;
         rows += o % KT * 16 * T::kRowBytes;
-        if constexpr (KV8) return *reinterpret_cast<const u32x2 *>(rows + row_at[c & 1] + (c >> 1) * 1024);
+        if constexpr (T::kBytes) return *reinterpret_cast<const u32x2 *>(rows + row_at[c & 1] + (c >> 1) * 1024);
         else return *reinterpret_cast<const u32x4 *>(rows + row_at[c & 1] + (c >> 1) * 1024);
       };
       auto value_operand = [&](const char *rows, int ks, int d) {
         rows += 16 * ks * T::kRowBytes;
-        if constexpr (KV8) {
+        if constexpr (T::kBytes) {
           return lds_read_transposed_bytes(rows + value_at[d & 1] + (d >> 1) * 1024);
         } else {
           const u32x2 a0 = lds_read_transposed(rows + value_at[d & 1] + (d >> 1) * 1024);
@@ -465,7 +507,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         float top = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-          if constexpr (KV8) s[kt] = *reinterpret_cast<const f32x4 *>(lds + T::kScales + (at * T::kKeys + key0 + 16 * kt + 4 * quarter) * 4);
+          if constexpr (KV8) s[kt] = *reinterpret_cast<const f32x4 *>(lds + T::kScales + ((T::kDecodes ? n & 7 : at) * T::kKeys + key0 + 16 * kt + 4 * quarter) * 4);
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[kt][e] *= KV8 ? p.score_scale_log2 * s[kt][e] : p.score_scale_log2;
         }
@@ -584,15 +626,20 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (steps > 0) {
         constexpr int R = T::kRing;
         if (loads_here)
-          for (int n = 0; n < min(T::kBefore, steps); ++n) issue(n, n);
+          for (int n = 0; n < min(T::kDecodes ? 2 : T::kBefore, steps); ++n) issue(n, n);
         if (scores_here) load_queries();
-        if (loads_here) {
+        if constexpr (T::kDecodes) {
+          if (loads_here) decode(0, 0);
+        } else if (loads_here) {
           if (!scores_here) wait_steps<T::kBefore - 1, T::kInFlight>(min(T::kBefore, steps) - 1);
           if (steps == 1) clear_unseen(0, 0);
         }
         meet();  // step 0 is there, and the queries' places are free
-        if (loads_here)
+        if constexpr (T::kDecodes) {
+          if (loads_here && steps > 1) decode(1, 1);
+        } else if (loads_here) {
           for (int n = T::kBefore; n < min(R, steps); ++n) issue(n, n);
+        }
         if (late) meet();
         int here = R - 1, next = 0;  // places in the ring of steps n, n + 1
         // Step n + 2 has landed, those after it are on their way.  (The late half does this before it asks for step n + R, others after.)
@@ -604,11 +651,14 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         auto round = [&](int n, auto with_results) __attribute__((always_inline)) {
           if (scores_here) matrix_phase(n, here, next, std::true_type{}, with_results);
           else matrix_phase(n, here, next, std::false_type{}, with_results);
-          if (T::kTurns && loads_here) land(n);
+          if (T::kTurns && !T::kDecodes && loads_here) land(n);
           meet();
           // step n has been read by all
-          if (loads_here && n >= 0 && n + R < steps) issue(n + R, here);
+          if (!T::kDecodes && loads_here && n >= 0 && n + R < steps) issue(n + R, here);
           if (scores_here) softmax(n + 1, next);
+          if constexpr (T::kDecodes) {
+            if (loads_here && n + R < steps) decode(n + R, here);
+          }
           if (!T::kTurns && loads_here) land(n);
           meet();
           here = next, next = next + 1 == R ? 0 : next + 1;
