@@ -276,7 +276,6 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // this wavefront's rows and keys of the scores, rows and elements of the results
   const int strip = wave / T::kParts, key_part = wave % T::kParts, key0 = key_part * 16 * KT;
-  const bool scores_here = T::kTurns || strip * 16 < M;
   const int result_row0 = T::kTurns ? (wave >> 2) * (M / 2) : 0, slice = wave % T::kSlices;
   const bool late = T::kTurns && wave >= 4, loads_here = wave >= 8 - T::kLoaders;
   const int loader = wave - (8 - T::kLoaders);  // which of those that load
@@ -356,6 +355,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     const bool whole = from == 0 && until == all_steps;
     if (tile < t.tiles && (whole || from < until)) {  // (a tile that sees no keys is whole: its rows get zeros)
       const int steps = until - from, row0 = tile * M;
+      // (M = 32: half of the wavefronts have no scores where there are 16 rows, or 32 keys a step)
+      const bool scores_here = T::kTurns || strip * 16 < min(M, t.rows - row0);
       // this lane's row of the scores (rows past the end repeat the last one and are not stored)
       const int my_row = (strip * 16 + i16) & (M - 1), row = min(row0 + my_row, t.rows - 1);
       const int j = row / H, head = row - j * H, pos = attends_from(q, j);
@@ -528,7 +529,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       // scheduling barriers, since left to itself the compiler asks for as many as there are and spills the rest.
       auto matrix_phase = [&](int n, int here, int next, auto with_scores, auto with_results) __attribute__((always_inline)) {
         constexpr bool kScores = decltype(with_scores)::value, kResults = decltype(with_results)::value;
-        constexpr int kAhead = M == 128 ? 4 : 6, kAll = KS * KT, kSteps = T::kKeys / 16, kFlagWords = M == 128 ? 4 : 2;
+        constexpr int kFirst = M == 128 ? 2 : 4, kAhead = M == 128 ? 4 : 6, kAll = KS * KT, kSteps = T::kKeys / 16, kFlagWords = M == 128 ? 4 : 2;
+        constexpr int kValues = kSteps * DT, kLast = kFirst < kValues ? kFirst : kValues;
         const char *values = lds + here * T::kStepBytes, *rows = lds + next * T::kStepBytes;
         uint32_t moved[kFlagWords] = {};
         u32x4 b[kSteps][RT];
@@ -536,15 +538,20 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
           for (int r = 0; r < RT; ++r) b[ks][r] = *reinterpret_cast<const u32x4 *>(lds + T::weights_at(result_row0 + r * 32 + col, 2 * ks + half));
         };
+        Raw a[kAhead];
+        auto first_rows = [&](int upto) __attribute__((always_inline)) {  // score operands, asked for under the last results
+#pragma unroll
+          for (int o = 0; o < kAhead; ++o)
+            if (o / 2 == upto) a[o] = row_operand(rows, o);
+        };
         if constexpr (kResults) {
-          constexpr int kValues = kSteps * DT, kFirst = M == 128 ? 2 : 4;
 #pragma unroll
           for (int ks = 0; ks < (M == 128 ? 1 : kSteps); ++ks) weights(ks);
 #pragma unroll
           for (int k = 0; k < kFlagWords; ++k) moved[k] = flags[result_row0 / 16 + k];
           Raw v[kFirst];
 #pragma unroll
-          for (int o = 0; o < kFirst && o < kValues; ++o) v[o] = value_operand(values, o / DT, o % DT);
+          for (int o = 0; o < kLast; ++o) v[o] = value_operand(values, o / DT, o % DT);
           uint32_t any = 0u;
 #pragma unroll
           for (int k = 0; k < kFlagWords; ++k) any |= moved[k];
@@ -565,14 +572,15 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
             for (int r = 0; r < RT; ++r) acc[r][o % DT] = mfma_32x32x16<OT>(value, b[o / DT][r], acc[r][o % DT]);
             if (M == 128 && o % DT == DT - 1 && o + 1 < kValues) weights(o / DT + 1);
             if (o + kFirst < kValues) v[o % kFirst] = value_operand(values, (o + kFirst) / DT, (o + kFirst) % DT);
+            else if (kScores) first_rows(o + kLast - kValues);
             __builtin_amdgcn_sched_barrier(0);
           }
         }
         if constexpr (kScores) {
           f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // two, for products that need not wait for each other
-          Raw a[kAhead];
 #pragma unroll
-          for (int o = 0; o < kAhead; ++o) a[o] = row_operand(rows, o);
+          for (int o = 0; o < kAhead; ++o)
+            if (!kResults || o / 2 >= kLast) a[o] = row_operand(rows, o);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int o = 0; o < kAll; ++o) {
@@ -623,6 +631,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 
       // ---- rounds: in round n the scores of step n + 1, the results of step n, and the softmax of step n + 1 ----
       if (!first_piece) meet();  // LDS of the piece before has been read
+      if (threadIdx.x < M / 16) flags[threadIdx.x] = 0;  // (of rows that there are not)
       if (steps > 0) {
         constexpr int R = T::kRing;
         if (loads_here)

@@ -212,12 +212,16 @@ inline LatentPlan latent_plan(const fa_latent_attention_shape &s, int cus) {
   if (T == 0 || S == 0) return r;
   const int64_t most = std::min<int64_t>(s.max_query_len, T), table = (int64_t)s.max_blocks_per_seq * s.block_size;
   const int64_t keys = s.max_context_len > 0 ? std::min<int64_t>(s.max_context_len, table) : table;
-  r.rows = most * H <= 32 ? 32 : most * H <= 64 ? 64 : 128;
+  // Tiles of 128 rows go through the keys in less time for each row (a round of 32 keys 1.9 us, of 64 rows 1.3 us), but what is left of
+  // them to be joined is as much larger (for each work-group 256 KiB to write and to read: 64 heads, 13 sequences of 301 to 9000 FP8 keys, 2 to 6
+  // tokens: 57 us with 128 rows, 53 us with 64; 128 heads, 64 sequences of 512 to 16384 keys: 126 us and 136 us).  They pay from about
+  // 16 rounds for each compute unit on; of the longest context's rounds, four times as many.
+  r.rows = most * H <= 32 ? 32 : most * H <= 64 || (T * H / 128) * (keys / 32) < 64 * cus ? 64 : 128;
   const int64_t each = (most * H + r.rows - 1) / r.rows;
   r.tile_bound = std::min(S * each, T * H / r.rows + S);
   if (keys > 256) {
     const bool equal = S == 1 || T == S * most;  // every sequence brings `most` tokens
-    r.team = equal ? (each % 4 == 0 ? 4 : each % 2 == 0 ? 2 : 1) : T * H >= 128 * S ? 2 : 1;
+    r.team = !equal ? 1 : each % 4 == 0 ? 4 : each % 2 == 0 ? 2 : 1;
     r.groups = std::max(8, cus / r.team / 8 * 8);  // (an eighth of the shares for each XCC)
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
