@@ -715,12 +715,14 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         const int64_t slot = 2 * (int64_t)part + (first_piece ? 0 : 1);
         float *dst = p.part_o + (slot * 8 + wave) * (RT * DT * 1024) + lane * 4;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int r = 0; r < RT; ++r) {
+          if (row0 + result_row0 + r * 32 + col >= t.rows) continue;
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               *reinterpret_cast<f32x4 *>(dst + (r * DT + d) * 1024 + k * 256) = f32x4{acc[r][d][4 * k], acc[r][d][4 * k + 1], acc[r][d][4 * k + 2], acc[r][d][4 * k + 3]};
+        }
         if (threadIdx.x < M) {
           p.part_ml[slot * 2 * M + threadIdx.x] = stats[threadIdx.x];
           p.part_ml[slot * 2 * M + M + threadIdx.x] = sum_of(threadIdx.x);
@@ -774,6 +776,7 @@ __global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentP
   const int first = join.first, last = join.last, place = found % p.team;
   const int of_wave = blockIdx.y / kTiles, slice = of_wave % T::kSlices, d = blockIdx.y % DT;
   const int row0 = (T::kTurns ? (of_wave >> 2) * (M / 2) : 0) + blockIdx.y % kTiles / DT * 32;
+  const int row = join.row + row0 + col;
   float m = kNoReference, l = 0.f;
   f32x16 acc;
 #pragma unroll
@@ -783,7 +786,8 @@ __global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentP
     f32x4 o[4];
   };
   auto load = [&](int h) {
-    Piece x;
+    Piece x = {kNoReference, 0.f, {}};
+    if (row >= join.rows) return x;
     const int64_t slot = h == first ? join.first_slot : 2 * ((int64_t)h * p.team + place);
     const float *ml = p.part_ml + slot * 2 * M + row0 + col;
     const float *src = p.part_o + (slot * 8 * kTiles + blockIdx.y) * 1024 + lane * 4;
@@ -820,7 +824,6 @@ __global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentP
     f[w] = fast_exp2(refs[w][0][lane] - to);
     sum += refs[w][1][lane] * f[w];
   }
-  const int row = join.row + row0 + col;
   if (row >= join.rows) return;
   const int token = row / p.num_heads, head = row - token * p.num_heads;
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
