@@ -198,12 +198,11 @@ struct LatentAbsorbed : LatentSteps<KV8, M> {
   static constexpr int kFlags = kFactors + M * 4;               // [strip of 16 rows]: whether there are factors
   static constexpr int kLdsBytes = kFlags + M / 4;
   static constexpr int kBefore = kRing / 2;                     // steps in the ring before the queries' place
-  static constexpr int kQueryWaves = kTurns ? 8 : 2 * kParts;   // wavefronts with scores
-  static constexpr int kQueryRows = (kRing - kBefore) * kStepBytes >= kQueryWaves * 16 * kRowElements * 2 ? 16 : 8;  // in LDS at a time, of a wavefront
+  static constexpr int kQueryRows = kParts == 1 ? 8 : 16;       // of a strip, in LDS at a time
   static constexpr int kSlices = kTurns ? 4 : 8;                // of the results' elements
   static constexpr int kResultTiles = M == 128 ? 2 : 1;         // of 32 rows
   static constexpr int DT = L / kSlices / 32, KS = kRowElements / 32;
-  static_assert((kRing - kBefore) * kStepBytes >= kQueryWaves * kQueryRows * kRowElements * 2, "");
+  static_assert((kRing - kBefore) * kStepBytes >= M / 16 * kQueryRows * kRowElements * 2, "");
   static_assert(kLdsBytes <= 160 * 1024 && kRing >= (kDecodes ? 3 : 4) && (kRing - 1) * kInFlight < 64 && kPieces % kLine == 0, "");
 
   // Where 16-byte piece c of a row lies in a step's place in LDS: kOwn rows together, of each kLine pieces at a time, as the loads leave
@@ -362,9 +361,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       const int j = row / H, head = row - j * H, pos = attends_from(q, j);
       const int wave_lo = attends_from(q, min(row0 + strip * 16, t.rows - 1) / H);
 
-      // This lane's row of queries.  It comes by way of LDS, where a wavefront has a place of its own behind the steps that are asked for first:
+      // This lane's row of queries.  It comes by way of LDS, where a strip of 16 rows has a place behind the steps that are asked for first:
       // rows may lie a power of two apart (heads outermost), and then 16 rows' same pieces, as the products take them, come from few
-      // channels; a whole row at a time does not (128 heads of 64 tokens: 10 us less for each tile).
+      // channels; a whole row at a time does not (128 heads of 64 tokens: 10 us less for each tile).  Two wavefronts of a strip load
+      // eight rows each; one alone loads and takes eight after the other.
       u32x4 qv[KS];
       const char *ql = p.query_latent + (int64_t)(q.first + j) * p.ql_token_bytes + head * p.ql_head_bytes;
       const char *qr = p.query_rope + (int64_t)(q.first + j) * p.qr_token_bytes + head * p.qr_head_bytes;
@@ -373,31 +373,41 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         int lane_here = lane;  // (addresses are computed here, not kept over the steps)
         asm volatile("" : "+v"(lane_here));
         const int i16 = lane_here & 15, quarter = lane_here >> 4;
-        const int place_at = T::kBefore * T::kStepBytes + wave * kPer * T::kRowElements * 2;
+        const int place_at = T::kBefore * T::kStepBytes + strip * kPer * T::kRowElements * 2;
         const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane(lds_at) + place_at;
+        auto rows_to_lds = [&](int first, int at_row) __attribute__((always_inline)) {  // eight, to rows at_row .. of the place
 #pragma unroll
-        for (int first = 0; first < 16; first += kPer) {
-#pragma unroll
-          for (int i = 0; i < kPer / kRows1; ++i) {
+          for (int i = 0; i < 8 / kRows1; ++i) {
             const int r = first + i * kRows1, piece = lane_here % kOfRow;
             uint64_t at = (uint64_t)readlane64((int64_t)(uintptr_t)ql, r);
             if (kRows1 == 2 && lane_here >= 32) at = (uint64_t)readlane64((int64_t)(uintptr_t)ql, r + 1);
-            load_to_lds_16_from(to + i * 1024, at + ((piece ^ ((r + lane_here / kOfRow) & 7)) * 16));
+            load_to_lds_16_from(to + (at_row + i * kRows1) * L * 2, at + ((piece ^ ((r + lane_here / kOfRow) & 7)) * 16));
           }
+          const int r = first + (lane_here >> 3);
+          load_to_lds_16_from(to + kPer * L * 2 + at_row * 128, (uint64_t)__shfl((long long)(uintptr_t)qr, r) + (((lane_here & 7) ^ (r & 7)) * 16));
+        };
+        auto from_lds = [&]() __attribute__((always_inline)) {
+          const char *latent = lds + place_at + i16 % kPer * L * 2, *rope = lds + place_at + kPer * L * 2 + i16 % kPer * 128;
 #pragma unroll
-          for (int i = 0; i < kPer / 8; ++i) {
-            const int r = first + i * 8 + (lane_here >> 3);
-            load_to_lds_16_from(to + kPer * L * 2 + i * 1024, (uint64_t)__shfl((long long)(uintptr_t)qr, r) + (((lane_here & 7) ^ (r & 7)) * 16));
+          for (int c = 0; c < KS; ++c)
+            qv[c] = c < L / 32 ? *reinterpret_cast<const u32x4 *>(latent + ((4 * c + quarter) ^ (i16 & 7)) * 16)
+                               : *reinterpret_cast<const u32x4 *>(rope + ((4 * (c - L / 32) + quarter) ^ (i16 & 7)) * 16);
+        };
+        if constexpr (kPer == 16) {
+          if (scores_here && key_part < 2) {
+            rows_to_lds(key_part * 8, key_part * 8);
+            wait_loads<0>();
           }
+          meet();
+          if (scores_here) from_lds();
+        } else {
+          rows_to_lds(0, 0);
           wait_loads<0>();
-          if (i16 / kPer == first / kPer) {
-            const char *from_lds = lds + place_at + i16 % kPer * L * 2, *rope = lds + place_at + kPer * L * 2 + i16 % kPer * 128;
-#pragma unroll
-            for (int c = 0; c < KS; ++c)
-              qv[c] = c < L / 32 ? *reinterpret_cast<const u32x4 *>(from_lds + ((4 * c + quarter) ^ (i16 & 7)) * 16)
-                                 : *reinterpret_cast<const u32x4 *>(rope + ((4 * (c - L / 32) + quarter) ^ (i16 & 7)) * 16);
-          }
+          if (i16 < 8) from_lds();
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next rows go to the same place
+          rows_to_lds(8, 0);
+          wait_loads<0>();
+          if (i16 >= 8) from_lds();
         }
 #pragma unroll
         for (int c = 0; c < KS; ++c)
@@ -636,7 +646,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         constexpr int R = T::kRing;
         if (loads_here)
           for (int n = 0; n < min(T::kDecodes ? 2 : T::kBefore, steps); ++n) issue(n, n);
-        if (scores_here) load_queries();
+        load_queries();
         if constexpr (T::kDecodes) {
           if (loads_here) decode(0, 0);
         } else if (loads_here) {
@@ -696,18 +706,30 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         return sum;
       };
       if (whole) {
+        // by way of LDS, whole rows of the wavefront's elements at a time
+        constexpr int kOfRow = DT * 4;  // 16-byte pieces, and lanes, of a row
+        int lane_here = lane;           // (addresses are computed here, not kept over the steps)
+        asm volatile("" : "+v"(lane_here));
+        char *mine = lds + wave * 32 * DT * 64;
+        const int row_in = lane_here / kOfRow, piece = lane_here % kOfRow;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const int of_tile = result_row0 + r * 32 + col, out_row = row0 + of_tile, stored = min(out_row, t.rows - 1), token = stored / H;
-          const float sum = sum_of(of_tile), inv = sum == 0.f ? 0.f : 1.0f / sum;
-          char *dst = p.out + (int64_t)(q.first + token) * p.out_token_bytes + (stored - token * H) * p.out_head_bytes + slice * (DT * 64) + half * 8;
-          if (out_row < t.rows) {
+          const int of_tile = result_row0 + r * 32;
+          const float sum = sum_of(of_tile + (lane_here & 31)), inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+          for (int d = 0; d < DT; ++d)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<u32x2 *>(dst + d * 64 + k * 16) = u32x2{pack2<OT>(acc[r][d][4 * k] * inv, acc[r][d][4 * k + 1] * inv),
-                                                                          pack2<OT>(acc[r][d][4 * k + 2] * inv, acc[r][d][4 * k + 3] * inv)};
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<u32x2 *>(mine + (lane_here & 31) * (DT * 64) + (((4 * d + k) ^ ((lane_here & 31) & (kOfRow - 1))) * 16) + (lane_here >> 5) * 8) =
+                  u32x2{pack2<OT>(acc[r][d][4 * k] * inv, acc[r][d][4 * k + 1] * inv), pack2<OT>(acc[r][d][4 * k + 2] * inv, acc[r][d][4 * k + 3] * inv)};
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll
+          for (int r0 = 0; r0 < 32; r0 += 64 / kOfRow) {
+            const int of_wave = r0 + row_in, out_row = row0 + of_tile + of_wave;
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + of_wave * (DT * 64) + ((piece ^ (of_wave & (kOfRow - 1))) * 16));
+            const int token = out_row / H;
+            if (out_row < t.rows)
+              *reinterpret_cast<u32x4 *>(p.out + (int64_t)(q.first + token) * p.out_token_bytes + (out_row - token * H) * p.out_head_bytes + slice * (DT * 64) + piece * 16) = v;
           }
         }
       } else {
@@ -743,7 +765,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 
 // Joins the pieces of cut tiles.  Work-group (x, y) has the x-th tile that is cut, if there are as many, and of it a product tile (32 rows, 32
 // elements) of one wavefront.  Its four wavefronts go through the pieces in turn, four at a time so that their loads overlap, and meet in
-// LDS.
+// LDS.  (Sixteen wavefronts take as long, also where a tile has a hundred pieces.)
 template <int L, typename OT, bool KV8, int M>
 __global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentParams p) {
   using T = LatentAbsorbed<L, OT, KV8, M>;
@@ -816,6 +838,7 @@ __global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentP
   for (int e = 0; e < 16; ++e) pieces[wave][e][lane] = acc[e];
   __syncthreads();
   // wavefront w finishes elements 8 w + 4 half + 0 .. 3
+  if (row >= join.rows) return;
   float to = refs[0][0][lane], sum = 0.f, f[4];
 #pragma unroll
   for (int w = 1; w < 4; ++w) to = fmaxf(to, refs[w][0][lane]);
@@ -824,7 +847,6 @@ __global__ void __launch_bounds__(256) latent_absorbed_join_kernel(const LatentP
     f[w] = fast_exp2(refs[w][0][lane] - to);
     sum += refs[w][1][lane] * f[w];
   }
-  if (row >= join.rows) return;
   const int token = row / p.num_heads, head = row - token * p.num_heads;
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   char *dst = p.out + (int64_t)(join.first_token + token) * p.out_token_bytes + head * p.out_head_bytes + slice * (DT * 64) + d * 64 + wave * 16 + half * 8;
