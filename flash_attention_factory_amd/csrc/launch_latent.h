@@ -205,6 +205,9 @@ inline fa_status check_latent_attention_shape(const fa_latent_attention_shape *s
   return FA_OK;
 }
 
+// Up to as many keys tiles are not cut.
+constexpr int kLatentWhole = 256;
+
 inline LatentPlan latent_plan(const fa_latent_attention_shape &s, int cus) {
   LatentPlan r = {};
   r.team = 1;
@@ -212,14 +215,20 @@ inline LatentPlan latent_plan(const fa_latent_attention_shape &s, int cus) {
   if (T == 0 || S == 0) return r;
   const int64_t most = std::min<int64_t>(s.max_query_len, T), table = (int64_t)s.max_blocks_per_seq * s.block_size;
   const int64_t keys = s.max_context_len > 0 ? std::min<int64_t>(s.max_context_len, table) : table;
-  // Tiles of 128 rows go through the keys in less time for each row (a round of 32 keys 1.9 us, of 64 rows 1.3 us), but what is left of
-  // them to be joined is as much larger (for each work-group 256 KiB to write and to read: 64 heads, 13 sequences of 301 to 9000 FP8 keys, 2 to 6
-  // tokens: 57 us with 128 rows, 53 us with 64; 128 heads, 64 sequences of 512 to 16384 keys: 126 us and 136 us).  They pay from about
-  // 16 rounds for each compute unit on; of the longest context's rounds, four times as many.
-  r.rows = most * H <= 32 ? 32 : most * H <= 64 || (T * H / 128) * (keys / 32) < 64 * cus ? 64 : 128;
+  auto tiles_of = [&](int64_t rows) { return std::min(S * ((most * H + rows - 1) / rows), T * H / rows + S); };
+  auto passes = [&](int64_t rows) { return (tiles_of(rows) + cus - 1) / cus; };
+  // Tiles of 128 rows go through the keys in less time for each row (a round of 32 keys 1.9 us, of 64 rows 1.3 us).  But what is left of
+  // cut ones to be joined is twice as large (256 KiB for each work-group to write and to read), and so is what one alone costs at its
+  // start and end (64 heads, 13 sequences of 301 to 9000 FP8 keys, 2 to 6 tokens: 57 us with 128 rows, 53 us with 64; 128 heads, 64
+  // sequences of 512 to 16384 keys: 126 us and 136 us).  Cut tiles pay from about 16 rounds for each compute unit on; of the longest
+  // context's rounds, four times as many.  Whole ones (short contexts) pay where they save a pass over the compute units.
+  bool tall = most * H > 64;
+  if (tall && keys > kLatentWhole) tall = (T * H / 128) * (keys / 32) >= 64 * cus;
+  else if (tall) tall = passes(128) * (11 + 1.9 * (keys / 32 + 1)) < passes(64) * (8 + 1.3 * (keys / 32 + 1));
+  r.rows = most * H <= 32 ? 32 : tall ? 128 : 64;
   const int64_t each = (most * H + r.rows - 1) / r.rows;
-  r.tile_bound = std::min(S * each, T * H / r.rows + S);
-  if (keys > 256) {
+  r.tile_bound = tiles_of(r.rows);
+  if (keys > kLatentWhole) {
     const bool equal = S == 1 || T == S * most;  // every sequence brings `most` tokens
     r.team = !equal ? 1 : each % 4 == 0 ? 4 : each % 2 == 0 ? 2 : 1;
     r.groups = std::max(8, cus / r.team / 8 * 8);  // (an eighth of the shares for each XCC)
