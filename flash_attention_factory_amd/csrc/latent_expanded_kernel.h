@@ -69,7 +69,8 @@ struct ExpandedTile {
   static constexpr int kKeyBytes = kTileKeys * D * 2, kRopeBytes = kTileKeys * kLatentRope * 2;
   static constexpr int kRopeAt = kRing * kKeyBytes, kValuesAt = kRopeAt + kRing * kRopeBytes;
   static constexpr int kLdsBytes = kValuesAt + kRing * kKeyBytes;
-  static constexpr int kOwn = kTileKeys / NW;               // rows of a step that a wavefront loads
+  static constexpr int kLoaders = 4;                        // wavefronts that load, the last ones
+  static constexpr int kOwn = kTileKeys / kLoaders;         // rows of a step that one of them loads
   static constexpr int kPieces = D / 8;                     // of 16 bytes, of an expanded row
   static constexpr int kLoads = kOwn * kPieces / 64, kRopeLoads = kOwn * 8 / 64;
   static constexpr int kInFlight = 2 * kLoads + kRopeLoads;
@@ -117,6 +118,8 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2,
 
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool late = NW == 8 && wave >= 4, loads_here = wave >= NW - T::kLoaders;
+  const int loader = wave - (NW - T::kLoaders);  // which of those that load
   const int H = p.num_kv_heads;
 
   // This work-group's tiles: one, longest sequences first, the last tiles of a sequence first, since they see the most keys; or a share
@@ -199,7 +202,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
 
-      // ---- loads: a wavefront's kOwn rows of a step ----
+      // ---- loads: a wavefront's kOwn rows of a step; of eight wavefronts the second four's, in their vector phase ----
       const int64_t k0 = min(max(load_uniform_i32(p.b.key_start + seq), 0), p.b.num_keys);
       const char *const key_rows = p.key + k0 * p.k_token_bytes + head * p.k_head_bytes;
       const char *const rope_rows = p.rope_key + k0 * p.r_token_bytes;
@@ -213,29 +216,30 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int i = 0; i < decltype(loads)::value; ++i) {
           const int r = i * (64 / kPer) + lane / kPer, c = lane & (kPer - 1);
-          load_to_lds_16(__builtin_amdgcn_readfirstlane(to + i * 1024), (uint32_t)min(r, left) * token_bytes + ((c ^ swizzle(wave * T::kOwn + r)) * 16), base);
+          load_to_lds_16(__builtin_amdgcn_readfirstlane(to + i * 1024), (uint32_t)min(r, left) * token_bytes + ((c ^ swizzle(loader * T::kOwn + r)) * 16), base);
         }
       };
       using Pieces = std::integral_constant<int, T::kPieces>;
       using Loads = std::integral_constant<int, T::kLoads>;
       auto issue_keys = [&](int n, int slot) __attribute__((always_inline)) {
-        const int key = (from + n) * kTileKeys + wave * T::kOwn;
-        rows_to_lds(key_rows, p.k_token_bytes, key, lds_at + slot * T::kKeyBytes + wave * T::kOwn * D * 2, Pieces{}, Loads{}, T::key_swizzle);
-        rows_to_lds(rope_rows, p.r_token_bytes, key, lds_at + T::kRopeAt + slot * T::kRopeBytes + wave * T::kOwn * 128, std::integral_constant<int, 8>{},
+        const int key = (from + n) * kTileKeys + loader * T::kOwn;
+        rows_to_lds(key_rows, p.k_token_bytes, key, lds_at + slot * T::kKeyBytes + loader * T::kOwn * D * 2, Pieces{}, Loads{}, T::key_swizzle);
+        rows_to_lds(rope_rows, p.r_token_bytes, key, lds_at + T::kRopeAt + slot * T::kRopeBytes + loader * T::kOwn * 128, std::integral_constant<int, 8>{},
                     std::integral_constant<int, T::kRopeLoads>{}, T::rope_swizzle);
       };
       auto issue_values = [&](int n, int slot) __attribute__((always_inline)) {
-        rows_to_lds(value_rows, p.v_token_bytes, (from + n) * kTileKeys + wave * T::kOwn, lds_at + T::kValuesAt + slot * T::kKeyBytes + wave * T::kOwn * D * 2,
+        rows_to_lds(value_rows, p.v_token_bytes, (from + n) * kTileKeys + loader * T::kOwn, lds_at + T::kValuesAt + slot * T::kKeyBytes + loader * T::kOwn * D * 2,
                     Pieces{}, Loads{}, T::value_swizzle);
       };
       // Rows that no token of the tile sees may hold anything: values of zero instead.  By the wavefront that has loaded them.
       auto clear_unseen = [&](int n, int slot) {
-        const int key = (from + n) * kTileKeys + wave * T::kOwn;
+        const int key = (from + n) * kTileKeys + loader * T::kOwn;
         for (int r = min(max(keys - key, 0), T::kOwn); r < T::kOwn; ++r)
           if (lane < T::kPieces)
-            *reinterpret_cast<u32x4 *>(lds + T::kValuesAt + slot * T::kKeyBytes + (wave * T::kOwn + r) * D * 2 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4 *>(lds + T::kValuesAt + slot * T::kKeyBytes + (loader * T::kOwn + r) * D * 2 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
       };
-      // Round n issues the values of step n + R - 1 and the keys of n + R; at its end those of n + 1 and n + 2 have landed.
+      // Round n asks for the values of step n + R - 1 and the keys of n + R (the second half of eight wavefronts at the end of round n - 1,
+      // beside its softmax, when nobody reads their places any more); at its end those of n + 1 and n + 2 have landed.
       int slot_k = 0, slot_v = 0;  // of keys of step n + 1, of values of step n
       auto later = [&](int slot, int by) { return slot + by >= R ? slot + by - R : slot + by; };
       auto issue = [&](int n) __attribute__((always_inline)) {
@@ -344,20 +348,30 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2,
       if (LINE && !first_piece) meet();  // LDS of the piece before has been read
       if (steps > 0) {
         constexpr bool kTurns = NW == 8;
-        const bool late = kTurns && wave >= 4;
-        issue_keys(0, 0);
-        for (int n = 0; n < R - 2; ++n) {
-          if (n < steps) issue_values(n, n);
-          if (n + 1 < steps) issue_keys(n + 1, n + 1);
+        if (loads_here) {
+          issue_keys(0, 0);
+          for (int n = 0; n < R - 2; ++n) {
+            if (n < steps) issue_values(n, n);
+            if (n + 1 < steps) issue_keys(n + 1, n + 1);
+          }
+          if (R - 2 < steps) wait_loads<(R - 2) * T::kInFlight>();
+          else wait_loads<0>();
+          // the wait for the queries, which is one for all loads, before there are more
+#pragma unroll
+          for (int c = 0; c < KS; ++c) asm volatile("" : "+v"(qv[c]));
         }
-        if (R - 2 < steps) wait_loads<(R - 2) * T::kInFlight>();
-        else wait_loads<0>();
         meet();
-        if (late) meet();
         slot_v = R - 1;  // round -1 has no values
+        if (late) {
+          issue(-1);
+          meet();
+        }
         auto advance = [&]() {
           slot_v = slot_k;
           slot_k = later(slot_k, 1);
+        };
+        auto before = [&](int n) __attribute__((always_inline)) {
+          if (!kTurns) issue(n);
         };
         auto between = [&](int n) __attribute__((always_inline)) {  // the two phases of round n
           if (kTurns) {
@@ -366,28 +380,38 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2,
           }
         };
         auto after = [&](int n) __attribute__((always_inline)) {
-          if (!late) land(n);
+          if (!kTurns) land(n);
           meet();
           advance();
         };
+        // the loads of round n + 1: their places are those that round n + 1 has for them
+        auto ask = [&](int n) __attribute__((always_inline)) {
+          if (late) {
+            if (n + R < steps) issue_values(n + R, slot_v);
+            if (n + R + 1 < steps) issue_keys(n + R + 1, slot_k);
+          }
+        };
         int n = -1;
         if (see_hi > 0) {
-          issue(n);
+          before(n);
           matrix_phase(std::true_type{}, std::false_type{});
           between(n);
+          ask(n);
           softmax(n + 1);
           after(n);
           for (++n; n + 1 < see_hi; ++n) {
-            issue(n);
+            before(n);
             matrix_phase(std::true_type{}, std::true_type{});
             between(n);
+            ask(n);
             softmax(n + 1);
             after(n);
           }
-          issue(n);
+          before(n);
           matrix_phase(std::false_type{}, std::true_type{});
           if (n + 1 < steps) {
             between(n);
+            ask(n);
             after(n);
             ++n;
           }
@@ -395,8 +419,9 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2,
         // rounds that the wavefront has no part in
         if (see_hi < steps)
           for (; n + 1 < steps; ++n) {
-            issue(n);
+            before(n);
             between(n);
+            ask(n);
             after(n);
           }
         if (kTurns && !late) meet();
