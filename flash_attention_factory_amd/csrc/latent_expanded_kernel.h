@@ -76,7 +76,7 @@ struct ExpandedTile {
   static constexpr int kInFlight = 2 * kLoads + kRopeLoads;
   static_assert(kLdsBytes <= 160 * 1024 && kRows * D * 2 <= kLdsBytes, "");
 
-  // exclusive-or of a row's pieces: neither 16 rows' same piece (keys) nor 4 rows of 64 bytes (values) meet in a bank
+  // exclusive-or of a row's pieces (the same for rows 16 apart): neither 16 rows' same piece (keys) nor 4 rows of 64 bytes (values) meet in a bank
   static __device__ __forceinline__ int key_swizzle(int key) { return D == 128 ? key & 15 : (key >> 1) & 7; }
   static __device__ __forceinline__ int rope_swizzle(int key) { return (key >> 1) & 7; }
   static __device__ __forceinline__ int value_swizzle(int key) { return D == 128 ? ((key & 3) << 2) ^ (key & 1) : ((key >> 1) & 1) * 5; }
@@ -208,28 +208,38 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2,
       const char *const rope_rows = p.rope_key + k0 * p.r_token_bytes;
       const char *const value_rows = p.value + k0 * p.v_token_bytes + head * p.v_head_bytes;
       const int last_key = max(q.ctx - 1, 0);
-      // Load i of a wavefront covers its rows from i * (64 / pieces) on, `kPer` lanes a row; rows past the last key repeat it.
-      auto rows_to_lds = [&](const char *rows, uint32_t token_bytes, int key, uint32_t to, auto per, auto loads, auto &&swizzle) __attribute__((always_inline)) {
-        constexpr int kPer = decltype(per)::value;
-        const int base_key = min(key, last_key), left = last_key - base_key;
-        const char *base = uniform_address(rows + (int64_t)base_key * token_bytes);
+      // Load i of a wavefront covers its rows from i * (64 / pieces) on, `kPer` lanes a row; rows past the last key repeat it.  The swizzle of
+      // load i's rows is that of load 0's with `turn` * i.
+      auto rows_to_lds = [&](const char *rows, uint32_t token_bytes, int key, uint32_t to, auto per, auto loads, auto turn, auto &&swizzle) __attribute__((always_inline)) {
+        constexpr int kPer = decltype(per)::value, kRows = 64 / kPer;
+        const int r0 = lane / kPer, piece = (lane & (kPer - 1)) ^ swizzle(r0);
+        if (key + T::kOwn - 1 <= last_key) {
+          const char *base = uniform_address(rows + (int64_t)key * token_bytes);
+          const uint32_t row = (uint32_t)r0 * token_bytes;
 #pragma unroll
-        for (int i = 0; i < decltype(loads)::value; ++i) {
-          const int r = i * (64 / kPer) + lane / kPer, c = lane & (kPer - 1);
-          load_to_lds_16(__builtin_amdgcn_readfirstlane(to + i * 1024), (uint32_t)min(r, left) * token_bytes + ((c ^ swizzle(loader * T::kOwn + r)) * 16), base);
+          for (int i = 0; i < decltype(loads)::value; ++i)
+            load_to_lds_16(__builtin_amdgcn_readfirstlane(to + i * 1024), row + (piece ^ (decltype(turn)::value * i)) * 16, base + (uint64_t)token_bytes * (i * kRows));
+        } else {
+          const int base_key = min(key, last_key), left = last_key - base_key;
+          const char *base = uniform_address(rows + (int64_t)base_key * token_bytes);
+#pragma unroll
+          for (int i = 0; i < decltype(loads)::value; ++i)
+            load_to_lds_16(__builtin_amdgcn_readfirstlane(to + i * 1024), (uint32_t)min(i * kRows + r0, left) * token_bytes + (piece ^ (decltype(turn)::value * i)) * 16, base);
         }
       };
+      using Turn = std::integral_constant<int, 4>;
+      using NoTurn = std::integral_constant<int, 0>;
       using Pieces = std::integral_constant<int, T::kPieces>;
       using Loads = std::integral_constant<int, T::kLoads>;
       auto issue_keys = [&](int n, int slot) __attribute__((always_inline)) {
         const int key = (from + n) * kTileKeys + loader * T::kOwn;
-        rows_to_lds(key_rows, p.k_token_bytes, key, lds_at + slot * T::kKeyBytes + loader * T::kOwn * D * 2, Pieces{}, Loads{}, T::key_swizzle);
+        rows_to_lds(key_rows, p.k_token_bytes, key, lds_at + slot * T::kKeyBytes + loader * T::kOwn * D * 2, Pieces{}, Loads{}, Turn{}, T::key_swizzle);
         rows_to_lds(rope_rows, p.r_token_bytes, key, lds_at + T::kRopeAt + slot * T::kRopeBytes + loader * T::kOwn * 128, std::integral_constant<int, 8>{},
-                    std::integral_constant<int, T::kRopeLoads>{}, T::rope_swizzle);
+                    std::integral_constant<int, T::kRopeLoads>{}, Turn{}, T::rope_swizzle);
       };
       auto issue_values = [&](int n, int slot) __attribute__((always_inline)) {
         rows_to_lds(value_rows, p.v_token_bytes, (from + n) * kTileKeys + loader * T::kOwn, lds_at + T::kValuesAt + slot * T::kKeyBytes + loader * T::kOwn * D * 2,
-                    Pieces{}, Loads{}, T::value_swizzle);
+                    Pieces{}, Loads{}, NoTurn{}, T::value_swizzle);
       };
       // Rows that no token of the tile sees may hold anything: values of zero instead.  By the wavefront that has loaded them.
       auto clear_unseen = [&](int n, int slot) {
