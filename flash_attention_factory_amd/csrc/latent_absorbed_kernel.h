@@ -5,14 +5,25 @@
 //   S^T[key, row] = [c, r] Q^T      MFMA 16x16x32, A = cached rows from LDS, B = queries, in registers for good
 //   O^T[d, row]  += c^T P^T         MFMA 32x32x16, A = the same rows by transposing LDS reads, B = weights from LDS
 //
-// A work-group of eight wavefronts takes a tile of M rows (32 or 64) and goes through 32 keys a step (bytes: 64).  Cached rows go from memory
-// to LDS by themselves (loads that write LDS), into a ring of steps, bytes of FP8 pools as they are: they are decoded on their way
-// into the products.  A round is a matrix phase -- scores of the next step, results of this one -- and a vector phase, the softmax:
-//   M = 64: four wavefronts, one on each SIMD, have the first 32 rows, the other four the others, one phase later, so that one
-//           wavefront of a SIMD is in its matrix phase while the other is in its vector phase.  Of its rows a wavefront has scores for 16 of them
-//           and half of the keys, and results for a quarter of the elements.
-//   M = 32: all wavefronts are in the same phase; 16 rows and 16 keys (with 32 keys a step, four wavefronts have none), an eighth of the elements.
-// Weights go through LDS, and so do the maxima of a row's keys, which several wavefronts have.
+// A work-group of eight wavefronts takes a tile of M rows (32, 64 or 128) and goes through 32 keys a step (bytes, M = 32: 64).  Cached rows go
+// from memory to LDS by themselves (loads that write LDS), into a ring of steps.  A round is a matrix phase -- results of this step, scores of the
+// next -- and a vector phase, the softmax:
+//   M = 64, 128: four wavefronts, one on each SIMD, have the first half of the rows, the other four the second, one phase later, so that
+//           one wavefront of a SIMD is in its matrix phase while the other is in its vector phase.  The second half loads, at the start of its
+//           vector phase, where it has time (at the start of the matrix phase the same loads cost 350 of 1700 cycles).  A wavefront
+//           has scores of 16 rows (M = 64: and half of the keys), and results of a half's rows for a quarter of the elements.
+//   M = 32: all wavefronts are in the same phase; 16 rows and 16 keys (wavefronts without any load instead, where they can), an eighth of the
+//           elements.
+// Weights go through LDS, and so do the maxima of a row's keys where several wavefronts have them.
+//
+// Bytes of FP8 pools: M = 32 takes them from the ring as they are, and every wavefront decodes what it reads, half the LDS for
+// a step of memory; M = 64 and 128 would decode each value four times in the time that the products take, so the wavefronts that load decode a
+// step once, into a ring of 16-bit rows (64 heads, 13 sequences of 301 to 9000 keys, 2 to 6 tokens: a round of 32 keys and 128 rows
+// 6000 -> 3900 cycles).
+//
+// Bound by memory where contexts are long (a round of 128 rows reads its 36 KiB at 5.0 TB/s over all compute units, of 32 rows of bytes at 6.0),
+// by starts, ends and the join where they are short.  MI355X, both kernels: 128 heads over 64 sequences of 512 to 16384 keys 127 us, 16 heads over
+// 128 FP8 sequences of 512 to 32768 keys 122 us, three users with 16 heads 15 us.
 //
 // Softmax against a reference m of each row that follows the maximum only where weights would pass 2^14 (kRefresh), and is set 2^6 below
 // it then (kHeadroom); what there is of sums and results is multiplied then.  Weights carry the scale of their cached row (FP8 pools): w =
@@ -21,7 +32,7 @@
 // All tiles of the batch lie end to end on a line, each as long as its steps, and every work-group takes an equal share (LatentLine);
 // pieces of cut tiles are joined by a second kernel.  Where sequences have several tiles, `team` of them lie side by side, and a share is
 // that of as many work-groups, on one XCC: they go through the same keys at the same time, which come from memory once (64
-// sequences of 512 to 16384 keys, 128 heads: 145 us and 15 us for the join).
+// sequences of 512 to 16384 keys, 128 heads as two tiles of 64 rows: 352 MB fetched, and the pool has 346).
 #pragma once
 
 #include "latent_cache_kernel.h"
@@ -55,7 +66,8 @@ struct LatentJoin {
   int32_t first_token, row, rows;   // of the sequence; the tile's first row, the sequence's rows
 };
 
-// Keys of a step, what a tile costs apart from its steps, and the smallest share of the line (both in steps).
+// Keys of a step, what a tile costs apart from its steps, and the smallest share of the line (both in steps; 128 heads over 64 long sequences:
+// kernel 108 us with kStart = 6, 103 with 12; three users with 16 heads: 14.4 us with kLeast = 8, 10.8 with 4).
 template <bool KV8, int M>
 struct LatentSteps {
   static constexpr int kKeys = KV8 && M == 32 ? 64 : 32, kStart = M == 128 ? 12 : KV8 && M == 32 ? 4 : 6, kLeast = KV8 && M == 32 ? 2 : 4;
@@ -363,7 +375,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 
       // This lane's row of queries.  It comes by way of LDS, where a strip of 16 rows has a place behind the steps that are asked for first:
       // rows may lie a power of two apart (heads outermost), and then 16 rows' same pieces, as the products take them, come from few
-      // channels; a whole row at a time does not (128 heads of 64 tokens: 10 us less for each tile).  Two wavefronts of a strip load
+      // channels; a whole row at a time does not (128 heads of 64 tokens: a tile's start takes 17 000 cycles instead of 24 000).  Two wavefronts of a strip load
       // eight rows each; one alone loads and takes eight after the other.
       u32x4 qv[KS];
       const char *ql = p.query_latent + (int64_t)(q.first + j) * p.ql_token_bytes + head * p.ql_head_bytes;

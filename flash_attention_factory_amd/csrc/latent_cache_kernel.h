@@ -7,6 +7,9 @@
 //   r' as rotate_pair turns it
 //   E4M3 pools: scale = the least power of two, 2^-100 or more, with max(|c'|, |r'|) / scale <= 448; bytes = e4m3(x / scale).  A power
 //   of two leaves the values as they are, so the bytes' rounding is the only one.
+//
+// Bound by memory, few tokens by the launch.  MI355X: 14052 tokens of 32 heads into an FP8 pool 35 us (4.0 TB/s of what has to move); 142335 FP8
+// rows back 57 us (4.3 TB/s; a device copy moves 4.8 to 5.1); one token of each of 128 sequences, 128 heads, 5.8 us.
 #pragma once
 
 #include "kv_cache_append_kernel.h"
@@ -130,7 +133,7 @@ struct LatentGatherParams {
   int64_t block_bytes, token_bytes, out_bytes;
   int32_t rows_per_group;
 };
-constexpr int kGatherMaxRows = 32;
+constexpr int kGatherMaxRows = 16;
 
 template <int L, typename OT, bool KV8>
 __global__ void __launch_bounds__(256) latent_cache_gather_kernel(const LatentGatherParams p) {

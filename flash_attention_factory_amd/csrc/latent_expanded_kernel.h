@@ -14,7 +14,13 @@
 // and the reads of values follow it, so weights never move between lanes.
 //
 // Eight wavefronts: two on each SIMD, the second four one phase behind the first, so that one is in its matrix phase while the other is in its
-// vector phase.  Four wavefronts (short calls) take no turns; two such work-groups share a compute unit.
+// vector phase.  The second four load, in their vector phase: by all, at the start of the matrix phase, the loads cost 400 to 800 cycles of
+// 2300 (4096 tokens after 12288, 32 heads: 1.16 ms -> 1.04 ms).  Four wavefronts (short calls) take no turns; two such work-groups
+// share a compute unit (MI355X, D = 128, 32 heads, four prompts of 1024: 67 us and 69 with eight; of 2048: 214 us and 185).
+//
+// With eight wavefronts the matrix cores are busy for 61 % of the time in long calls, and the clock falls to 1.6 GHz: fewer cycles
+// (887 000 of once 1 116 000) have saved less time than cycles.  MI355X: 4096 tokens after 12288 1.02 ms (1.18 PFLOP/s), six prompts of 513 to
+// 4003 tokens 241 us (0.87 PFLOP/s: steps on the diagonal, start and end of a tile).
 #pragma once
 
 #include "latent_absorbed_kernel.h"
