@@ -20,7 +20,8 @@
  * Pools: row t of block b begins at base + b * block_stride + t * token_stride (elements) and holds latent_dim +
  * rope_dim contiguous ones: 16-bit of the queries' type, or E4M3 bytes, each standing for itself times its row's
  * scale, scales[b * block_size + t].  Rows of the pool that no token sees, and their scales, may hold
- * anything.  Scales are positive.  latent_dim is 256 or 512, rope_dim 64.
+ * anything.  A row of a new token that holds infinities or NaN can reach earlier new tokens of its sequence
+ * in the same call.  Scales are positive.  latent_dim is 256 or 512, rope_dim 64.
  *
  * Nothing but kernel launches is put on options->stream unless options->elapsed_us is given.  Of options these entries read
  * stream, elapsed_us (1 float) and validate_only.  No exception crosses this boundary.
