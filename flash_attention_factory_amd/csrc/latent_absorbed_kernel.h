@@ -217,6 +217,17 @@ struct LatentAbsorbed : LatentSteps<KV8, M> {
   static_assert((kRing - kBefore) * kStepBytes >= M / 16 * kQueryRows * kRowElements * 2, "");
   static_assert(kLdsBytes <= 160 * 1024 && kRing >= (kDecodes ? 3 : 4) && (kRing - 1) * kInFlight < 64 && kPieces % kLine == 0, "");
 
+  // The wavefronts' parts: a strip of 16 rows and a part of a step's keys for the scores, and whether a wavefront loads.
+  static constexpr int strip_of(int wave) { return wave / kParts; }
+  static constexpr int key_part_of(int wave) { return wave % kParts; }
+  static constexpr bool loads(int wave) { return wave >= 8 - kLoaders; }
+  // (M = 32: half of the wavefronts have no scores where there are 16 rows, or 32 keys a step)
+  static constexpr bool has_scores(int strip, int rows) { return kTurns || strip * 16 < (M < rows ? M : rows); }
+  // The first two wavefronts of a strip ask for its queries (one alone for all of them), and wait for whatever they have asked for, steps
+  // of the ring among it.  Any other wavefront that loads waits for the first step by itself: it is read behind the next barrier.
+  static constexpr bool asks_for_queries(bool scores, int key_part) { return kParts == 1 || (scores && key_part < 2); }
+  static constexpr bool waits_for_first_step(bool scores, int key_part) { return !asks_for_queries(scores, key_part); }
+
   // Where 16-byte piece c of a row lies in a step's place in LDS: kOwn rows together, of each kLine pieces at a time, as the loads leave
   // them.  Which of the kLine goes by the row: then the 16 lanes of a read of 16 bytes that go together (0 .. 3, 12 .. 15 and 20 .. 27,
   // and the others) meet in no bank where they read two neighbouring pieces of 16 rows, nor do 32 lanes that read 4 rows of 64 bytes
@@ -286,9 +297,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, quarter = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // this wavefront's rows and keys of the scores, rows and elements of the results
-  const int strip = wave / T::kParts, key_part = wave % T::kParts, key0 = key_part * 16 * KT;
+  const int strip = T::strip_of(wave), key_part = T::key_part_of(wave), key0 = key_part * 16 * KT;
   const int result_row0 = T::kTurns ? (wave >> 2) * (M / 2) : 0, slice = wave % T::kSlices;
-  const bool late = T::kTurns && wave >= 4, loads_here = wave >= 8 - T::kLoaders;
+  const bool late = T::kTurns && wave >= 4, loads_here = T::loads(wave);
   const int loader = wave - (8 - T::kLoaders);  // which of those that load
   const int H = p.num_heads;
 
@@ -366,8 +377,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     const bool whole = from == 0 && until == all_steps;
     if (tile < t.tiles && (whole || from < until)) {  // (a tile that sees no keys is whole: its rows get zeros)
       const int steps = until - from, row0 = tile * M;
-      // (M = 32: half of the wavefronts have no scores where there are 16 rows, or 32 keys a step)
-      const bool scores_here = T::kTurns || strip * 16 < min(M, t.rows - row0);
+      const bool scores_here = T::has_scores(strip, t.rows - row0);
       // this lane's row of the scores (rows past the end repeat the last one and are not stored)
       const int my_row = (strip * 16 + i16) & (M - 1), row = min(row0 + my_row, t.rows - 1);
       const int j = row / H, head = row - j * H, pos = attends_from(q, j);
@@ -406,7 +416,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
                                : *reinterpret_cast<const u32x4 *>(rope + ((4 * (c - L / 32) + quarter) ^ (i16 & 7)) * 16);
         };
         if constexpr (kPer == 16) {
-          if (scores_here && key_part < 2) {
+          if (T::asks_for_queries(scores_here, key_part)) {
             rows_to_lds(key_part * 8, key_part * 8);
             wait_loads<0>();
           }
@@ -662,7 +672,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         if constexpr (T::kDecodes) {
           if (loads_here) decode(0, 0);
         } else if (loads_here) {
-          if (!scores_here) wait_steps<T::kBefore - 1, T::kInFlight>(min(T::kBefore, steps) - 1);
+          if (T::waits_for_first_step(scores_here, key_part)) wait_steps<T::kBefore - 1, T::kInFlight>(min(T::kBefore, steps) - 1);
           if (steps == 1) clear_unseen(0, 0);
         }
         meet();  // step 0 is there, and the queries' places are free
