@@ -115,6 +115,26 @@ __device__ __forceinline__ int64_t wave_sums64(int64_t v) {
   v += lanes_moved<0x143, 0xc>(v);  // lane 31, to the last 32
   return v;
 }
+// Where share g of the line begins.  (Lengths on the line pass 32 bits, lengths of tiles do not.)
+__host__ __device__ __forceinline__ int64_t latent_cut(int64_t total, int groups, int g) { return divide(total * g, groups); }
+// The step that a cut `off` into a tile of `steps` steps lies before.
+template <typename T>
+__host__ __device__ __forceinline__ int latent_cut_step(int64_t off, int steps) {
+  const int64_t step = off - T::kStart;
+  return step <= 0 ? 0 : step < steps ? (int)step : steps;
+}
+// The shares that have steps of the tile of `steps` steps that begins at `start`, and whose first cut is the end of share g.
+struct LatentShares {
+  int first, last;
+};
+template <typename T>
+__host__ __device__ __forceinline__ LatentShares latent_shares(int64_t total, int groups, int g, int64_t start, int steps) {
+  const int64_t guess = divide((start + T::kStart + steps - 1) * groups, total) + 1;  // the last one, or one too many
+  LatentShares s = {g, guess < groups ? (int)guess : groups - 1};
+  while (latent_cut_step<T>(latent_cut(total, groups, s.first + 1) - start, steps) == 0) ++s.first;
+  while (latent_cut(total, groups, s.last) - start - T::kStart >= steps) --s.last;
+  return s;
+}
 template <typename T>
 struct LatentPlace {
   int seq, team;  // team: which of the sequence's
@@ -143,7 +163,7 @@ struct LatentLine {
     const LatentTiles t = latent_tiles<T>(p, q);
     return t.teams * t.cost;
   }
-  __device__ __forceinline__ int64_t cut(int g) const { return divide(total * g, groups); }
+  __device__ __forceinline__ int64_t cut(int g) const { return latent_cut(total, groups, g); }
   // `at` < total
   __device__ __forceinline__ LatentPlace<T> find(const LatentParams &p, int64_t at, int lane) const {
     LatentPlace<T> r;
@@ -174,11 +194,6 @@ struct LatentLine {
     return r;
   }
 };
-// The step that a cut `off` into a tile of `steps` steps lies before.
-template <typename T>
-__device__ __forceinline__ int latent_cut_step(int64_t off, int steps) {
-  return min(max((int)off - T::kStart, 0), steps);
-}
 
 template <int L, typename OT, bool KV8, int M>
 struct LatentAbsorbed : LatentSteps<KV8, M> {
@@ -329,10 +344,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       LatentJoin join = {1, 0, 0, t1.q.first, end_tile * M, t1.rows};
       const int64_t start = line.cut(g + 1) - 1 - to.off;
       if (to.off + 1 < t1.cost && line.cut(g) <= start && end_steps > 0) {
-        int first = g, last = min((int)divide((start + T::kStart + end_steps - 1) * line.groups, line.total) + 1, line.groups - 1);
-        while (latent_cut_step<T>(line.cut(first + 1) - start, end_steps) == 0) ++first;
-        while (line.cut(last) - start - T::kStart >= end_steps) --last;
-        if (first < last) join.first = first, join.last = last, join.first_slot = 2 * (first * p.team + place) + (first == g && line.cut(g) < start);
+        const LatentShares s = latent_shares<T>(line.total, line.groups, g, start, end_steps);
+        if (s.first < s.last)
+          join.first = s.first, join.last = s.last, join.first_slot = 2 * (s.first * p.team + place) + (s.first == g && line.cut(g) < start);
       }
       if (lane == 0) p.joins[part] = join;
     }

@@ -148,8 +148,9 @@ struct TilePlace {
   int seq, kvh, tile;
   int64_t off;  // cost units from the tile's start
 };
-// n / d for n < 2^53, without the 64-bit division's two hundred instructions.
-__device__ __forceinline__ int64_t divide(int64_t n, int d) {
+// n / d for n and d below 2^53, without the 64-bit division's two hundred instructions.
+template <typename Divisor>
+__host__ __device__ __forceinline__ int64_t divide(int64_t n, Divisor d) {
   int64_t q = (int64_t)((double)n / (double)d);
   if (q * d > n) --q;
   if ((q + 1) * d <= n) ++q;
