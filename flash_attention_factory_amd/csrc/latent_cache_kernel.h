@@ -32,11 +32,11 @@ struct LatentAppendParams {
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 
-// Exponent of the scale of a row whose largest magnitude is `most`: 448 is 1.75 * 2^8.
-__device__ __forceinline__ int row_scale_exponent(float most) {
+// Exponent of the scale of a row whose largest magnitude is `most`: 448 is 1.75 * 2^8.  At most 120: the reciprocal is a normal number.
+__host__ __device__ __forceinline__ int row_scale_exponent(float most) {
   const uint32_t bits = __builtin_bit_cast(uint32_t, most);
   const int e = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
-  return min(max(e, -100), 100);
+  return e < -100 ? -100 : e;
 }
 
 template <int N, typename ST>

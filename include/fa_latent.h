@@ -21,7 +21,8 @@
  * rope_dim contiguous ones: 16-bit of the queries' type, or E4M3 bytes, each standing for itself times its row's
  * scale, scales[b * block_size + t].  Rows of the pool that no token sees, and their scales, may hold
  * anything.  A row of a new token that holds infinities or NaN can reach earlier new tokens of its sequence
- * in the same call.  Scales are positive.  latent_dim is 256 or 512, rope_dim 64.
+ * in the same call.  Scales are positive; next to a row whose scale is 2^100 attention counts weights
+ * down to 2^-32 of the largest, next to one of 2^120 down to 2^-12.  latent_dim is 256 or 512, rope_dim 64.
  *
  * Nothing but kernel launches is put on options->stream unless options->elapsed_us is given.  Of options these entries read
  * stream, elapsed_us (1 float) and validate_only.  No exception crosses this boundary.
