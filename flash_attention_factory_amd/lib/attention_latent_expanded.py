@@ -7,6 +7,7 @@ up to its own:
 
     s = scale (query[:D] . key + query[D:] . rope_key),   out = sum of softmax(s) value
 
+Values of a new token that are infinite or NaN can reach earlier new tokens of its sequence, nothing reaches another sequence.
 ``max_query_len`` and ``max_key_len`` (0: all keys) are bounds the host knows.  The form for prompts, where expanding every key once costs less
 than attending latents that are four times as wide.  Upstream has no such kernel.
 

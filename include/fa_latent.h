@@ -165,7 +165,8 @@ int64_t fa_attention_latent_expanded_workspace_bytes(const fa_latent_expanded_sh
  *   s   = scale (query[:head_size] . key + query[head_size:] . rope_key)
  *   out = sum of softmax(s) value
  * A token that sees no key gets zeros.  Tokens beyond max_query_len of their sequence are left out, their rows of out stay as they are;
- * of keys beyond max_key_len nothing is read.
+ * of keys beyond max_key_len nothing is read.  Values of a new token that are infinite or NaN can reach earlier new tokens
+ * of its sequence (their weight is zero, and the product is not); nothing reaches another sequence.
  */
 int32_t fa_attention_latent_expanded(void *out, const void *query, const void *key, const void *rope_key, const void *value,
                                      const int32_t *query_start, const int32_t *key_start, float scale, void *workspace,
