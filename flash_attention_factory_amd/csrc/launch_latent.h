@@ -223,6 +223,11 @@ inline LatentPlan latent_plan(const fa_latent_attention_shape &s, int cus) {
   // start and end (64 heads, 13 sequences of 301 to 9000 FP8 keys, 2 to 6 tokens: 57 us with 128 rows, 53 us with 64; 128 heads, 64
   // sequences of 512 to 16384 keys: 126 us and 136 us).  Cut tiles pay from about 16 rounds for each compute unit on; of the longest
   // context's rounds, four times as many.  Whole ones (short contexts) pay where they save a pass over the compute units.
+  // The host knows the longest context only, and the four fit contexts that are spread.  Where they are equal, 64 rows are taken for longer
+  // than they pay: 128 heads, us with 64 and 128 rows, 16-bit pools 67 and 77 at 16 rounds, 113 and 116 at 32, 213 and 188 at 64 (where the
+  // rule changes over); FP8 57 and 56 at 8, 81 and 76 at 16, 131 and 110 at 32.
+  // One height serves the whole batch, by its longest piece: 16 heads, 128 sequences of 512 to 16384 keys with a token each beside a piece of
+  // 64 tokens take 157 us (16-bit; as two calls 179), with FP8 pools, whose 32-row tiles are the faster ones, 159 us (as two calls 121).
   bool tall = most * H > 64;
   if (tall && keys > kLatentWhole) tall = (T * H / 128) * (keys / 32) >= 64 * cus;
   else if (tall) tall = passes(128) * (11 + 1.9 * (keys / 32 + 1)) < passes(64) * (8 + 1.3 * (keys / 32 + 1));
