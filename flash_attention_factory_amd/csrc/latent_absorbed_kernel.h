@@ -23,7 +23,7 @@
 //
 // Bound by memory where contexts are long (a round of 128 rows reads its 36 KiB at 5.0 TB/s over all compute units, of 32 rows of bytes at 6.0),
 // by starts, ends and the join where they are short.  MI355X, both kernels: 128 heads over 64 sequences of 512 to 16384 keys 127 to 130 us (over
-// boxes), 16 heads over 128 FP8 sequences of 512 to 32768 keys 122 to 124 us, three users with 16 heads 15 us.
+// machines), 16 heads over 128 FP8 sequences of 512 to 32768 keys 122 to 124 us, three users with 16 heads 15 us.
 //
 // Softmax against a reference m of each row that follows the maximum only where weights would pass 2^14 (kRefresh), and is set 2^6 below
 // it then (kHeadroom); what there is of sums and results is multiplied then.  Weights carry the scale of their cached row (FP8 pools): w =

@@ -19,7 +19,7 @@
 // share a compute unit (MI355X, D = 128, 32 heads, four prompts of 1024: 67 us and 69 with eight; of 2048: 214 us and 185).
 //
 // With eight wavefronts the matrix cores are busy for 61 % of the time in long calls, and the clock falls to 1.6 GHz: fewer cycles
-// (887 000 of once 1 116 000) have saved less time than cycles.  MI355X, over boxes: 4096 tokens after 12288 0.965 to 1.02 ms (1.25 to 1.18
+// (887 000 of once 1 116 000) have saved less time than cycles.  MI355X, over machines: 4096 tokens after 12288 0.965 to 1.02 ms (1.25 to 1.18
 // PFLOP/s), six prompts of 513 to 4003 tokens 226 to 241 us (0.93 to 0.87 PFLOP/s: steps on the diagonal, start and end of a tile).
 //
 // Weights are rounded to the queries' type, which the matrix cores take, and their sum is that of the rounded ones: the result's error against
